@@ -352,13 +352,19 @@ int piekv_prefill_export_mask(const int32_t *qo_indptr, const int32_t *kv_indptr
  *                its request; for decode p = kv_len - 1) sees keys p - window_left .. only, on top of
  *                whatever the causal flag or the mask allows.  The decode kernel then streams only the
  *                pages that hold such keys.
+ *   first_tokens 0: none.  n > 0 together with a window: keys 0 .. n - 1 stay visible to every query at or
+ *                behind them however far the window has moved on.  Pages between the first tokens and the
+ *                window are never read (their entries in kv_indices may be stale or -1).  Not taken together
+ *                with a mask (bytes or run lengths), nor by the fused step.  A decode call needs
+ *                piekv_decode_first_tokens_workspace_bytes; a prefill call is planned without a mask and
+ *                without a window (piekv_prefill_plan), the run applies both.
  *   sinks        nullable device fp32 [num_qo_heads]: softmax is taken over the scaled scores AND the
  *                head's sink logit (not scaled); the sink has no value row, so it only takes
  *                probability mass: out = sum_t exp(s_t) v_t / (sum_t exp(s_t) + exp(sink_h)).
  *                `lse` then includes the sink term.  A query without any visible key gives zeros. */
 typedef struct piekv_attn_options {
   int32_t window_left;
-  int32_t reserved; /* 0 */
+  int32_t first_tokens;
   const float *sinks;
 } piekv_attn_options;
 
@@ -379,6 +385,11 @@ int piekv_decode_step_fused_opt(const void *q, const void *k, const void *v, int
                                 const piekv_rope_params *rope, float sm_scale, void *workspace,
                                 int64_t workspace_bytes, int32_t *err, void *stream,
                                 const piekv_attn_options *opt);
+
+/* Workspace of piekv_decode_run_opt with first_tokens > 0 (the first piekv_decode_counter_bytes zero, as
+ * for every decode call, and left zero). */
+int64_t piekv_decode_first_tokens_workspace_bytes(int32_t batch, int32_t num_qo_heads, int32_t num_kv_heads,
+                                                  int32_t head_dim);
 
 /* piekv_prefill_plan and piekv_prefill_plan_brle in one call, plus the window: the mask comes as bytes
  * (`custom_mask`), as run lengths (`brle_runs` / `brle_indptr`) or not at all, and `window_left` >= 0 is
@@ -401,6 +412,100 @@ int piekv_prefill_run_opt(const void *q, int64_t q_stride_n, int64_t q_stride_h,
                           int32_t num_kv_heads, int32_t head_dim, int32_t page_size, int32_t num_pages,
                           int32_t dtype, float sm_scale, void *workspace, int64_t workspace_bytes,
                           int32_t *err, void *stream, const piekv_attn_options *opt);
+
+/* ---- decode for requests that share the leading pages of their contexts ------------------------------
+ *
+ * Forked contexts keep their parent's full pages (sdk/rust/inferlet/src/context.rs:147-225; the page tables
+ * of piekv_pagestate_fork do the same), so the requests of a beam search, or all chats behind one system
+ * prompt, list the same physical pages first.  A plain decode call reads those pages once per request; these
+ * entry points read them once per group and join the two parts of every softmax in fp32.
+ *
+ * Groups are runs of consecutive requests: group g holds requests group_indptr[g] .. group_indptr[g + 1),
+ * group_indptr[0] = 0, group_indptr[num_groups] = batch.  What a group shares is found on the device by
+ * comparing the page lists (full pages only), so the result equals piekv_decode_run's for any grouping; a
+ * grouping that shares nothing only costs the comparison.  A group_indptr that is not monotone from 0 to
+ * batch sets PIEKV_ERR_INDPTR and shares nothing.
+ *
+ * piekv_shared_prefix_plan compares the lists and builds the work list in `plan`
+ * (piekv_shared_prefix_plan_bytes, 256-byte aligned, private to the caller's batch); piekv_shared_prefix_run
+ * uses it for every layer until the page table changes.  `max_splits` (1 ..
+ * PIEKV_SHARED_PREFIX_MAX_SPLITS) bounds into how many pieces a prefix is cut; pass the same number to the
+ * workspace size, the plan and the run.  The workspace starts with piekv_decode_counter_bytes zeros, left
+ * zero.  Shapes the tuned kernels do not cover (fp32, head_dim other than 128, page size other than 16, more
+ * than 16 query heads per kv head) run the general kernel, request by request. */
+#define PIEKV_SHARED_PREFIX_MAX_SPLITS 64
+typedef struct piekv_shared_prefix_args {
+  const void *q; /* [batch, num_qo_heads, head_dim], strides in elements */
+  int64_t q_stride_n, q_stride_h;
+  const void *pool;
+  void *out;  /* [batch, num_qo_heads, head_dim] contiguous */
+  float *lse; /* nullable [batch, num_qo_heads] */
+  const int32_t *kv_indptr, *kv_indices, *kv_last_page_len;
+  const int32_t *group_indptr; /* [num_groups + 1] */
+  const float *sinks;          /* nullable fp32 [num_qo_heads], as in piekv_attn_options */
+  void *plan;
+  int64_t plan_bytes;
+  void *workspace;
+  int64_t workspace_bytes;
+  int32_t *err;
+  int32_t batch, num_groups, num_qo_heads, num_kv_heads, head_dim, page_size, num_pages, dtype;
+  int32_t max_splits;
+  float sm_scale;
+} piekv_shared_prefix_args;
+
+int64_t piekv_shared_prefix_plan_bytes(int32_t batch, int32_t num_groups, int32_t num_qo_heads,
+                                       int32_t num_kv_heads);
+int64_t piekv_shared_prefix_workspace_bytes(int32_t batch, int32_t num_qo_heads, int32_t num_kv_heads,
+                                            int32_t head_dim, int32_t max_splits);
+/* reads kv_indptr, kv_indices, kv_last_page_len, group_indptr, plan and the sizes of `args` (a host struct);
+ * num_pages is not used */
+int piekv_shared_prefix_plan(const piekv_shared_prefix_args *args, void *stream);
+int piekv_shared_prefix_run(const piekv_shared_prefix_args *args, void *stream);
+
+/* ---- rotary positions on several axes, with the append -------------------------------------------------
+ *
+ * For contexts that hold images or video a token has one position per axis (time, height, width; text has
+ * them equal), and every (cos, sin) pair of a head row belongs to one axis.  The rotary width is
+ * rotary_dim = 2 * sum(sections) <= head_dim; elements behind it are copied.  With the pair index
+ * i = 0 .. rotary_dim / 2 - 1 the axis of pair i is
+ *   cyclic = 0   blocks in order: the first sections[0] pairs axis 0, the next sections[1] axis 1, ...
+ *   cyclic = 1   i mod num_axes for pairs below num_axes * sections[i mod num_axes], else axis 0
+ * and its angle pos[axis][token] * f_i with the f_i of `rope` taken over rotary_dim.  The angle is formed as
+ * a 64-bit fixed-point fraction of a turn, so it is as exact at position 10^6 as at 10.  rope->mode PLAIN,
+ * LLAMA31 or TABLE (rows of rotary_dim floats; pair i reads row pos[axis]).
+ *
+ * piekv_rope_axes_prepare lays the pairs out once per configuration (host only, no launch); `table` is a
+ * host struct that every later call of that configuration takes. */
+#define PIEKV_MAX_ROPE_AXES 4
+typedef struct piekv_rope_axes_table {
+  uint64_t turn[128]; /* f_i / (2 pi) in units of 2^-64 */
+  uint8_t axis[128];
+  const float *cos_sin_table; /* nullable */
+  int32_t table_len, num_axes, half, interleave;
+} piekv_rope_axes_table;
+
+int piekv_rope_axes_prepare(const piekv_rope_params *rope, const int32_t *sections, int32_t num_axes,
+                            int32_t cyclic, piekv_rope_axes_table *table);
+
+typedef struct piekv_rope_axes_args {
+  const void *q;  /* nullable [nnz, num_qo_heads, head_dim], strides in elements */
+  const void *k;  /* [nnz, num_kv_heads, head_dim]                             */
+  const void *v;  /* as k; nullable without a pool                             */
+  void *q_out;    /* nullable without q: [nnz, num_qo_heads, head_dim] with q_out strides; may be q */
+  void *k_out;    /* nullable: rotated k, k_out strides; may be k              */
+  int64_t q_stride_n, q_stride_h, k_stride_n, k_stride_h, v_stride_n, v_stride_h;
+  int64_t q_out_stride_n, q_out_stride_h, k_out_stride_n, k_out_stride_h;
+  const int32_t *pos;           /* axis a of token t at pos[a * pos_stride + t] */
+  int64_t pos_stride;
+  const int32_t *batch_indices; /* these five are read only with a pool, as in piekv_rope_append */
+  const int32_t *positions;
+  void *pool;                   /* nullable: no append                         */
+  const int32_t *kv_indices, *kv_indptr;
+  int32_t *err;
+  int32_t nnz, batch, num_qo_heads, num_kv_heads, head_dim, page_size, num_pages, dtype;
+} piekv_rope_axes_args;
+
+int piekv_rope_axes(const piekv_rope_axes_args *args, const piekv_rope_axes_table *table, void *stream);
 
 /* ---- head-sharded decode over the GPUs of one node: results stored straight to every GPU ----
  *
@@ -512,7 +617,8 @@ int piekv_oproj_allreduce(const void *a, int64_t a_stride_n, const void *w_o, in
 
 /* sizeof of the structs that cross this boundary, for bindings to check their mirrors against:
  * which = 0: piekv_rope_params, 1: piekv_peer_outputs, 2: piekv_attn_options, 3: piekv_wire_batch,
- * 4: piekv_qkv_options, 5: piekv_peer_reduce; anything else: -1. */
+ * 4: piekv_qkv_options, 5: piekv_peer_reduce, 6: piekv_shared_prefix_args, 7: piekv_rope_axes_args,
+ * 8: piekv_rope_axes_table; anything else: -1. */
 int32_t piekv_abi_sizeof(int32_t which);
 
 /* ---- page copy (fork with copy-on-write of a partial page) ----------------------- */

@@ -9,23 +9,31 @@ __version__ = "0.1.0"
 
 from . import ops  # noqa: F401  (loads libpiekv.so; raises ImportError if it is not built)
 from .ops import (  # noqa: F401
+    AxisRopeConfig,
     BatchDecodeWithPagedKVCacheWrapper,
     BatchPrefillWithPagedKVCacheWrapper,
+    BatchSharedPrefixDecodeWrapper,
     RopeConfig,
     append_paged_kv_cache,
     apply_llama31_rope_pos_ids_inplace,
+    apply_rope_axes_inplace,
     apply_rope_pos_ids_inplace,
     copy_kv_pages,
     device_error,
     get_batch_indices_positions,
     get_seq_lens,
     rope_append_paged_kv_cache,
+    rope_axes_append_paged_kv_cache,
 )
 
 __all__ = [
     "ops",
     "BatchPrefillWithPagedKVCacheWrapper",
     "BatchDecodeWithPagedKVCacheWrapper",
+    "BatchSharedPrefixDecodeWrapper",
+    "apply_rope_axes_inplace",
+    "rope_axes_append_paged_kv_cache",
+    "AxisRopeConfig",
     "apply_rope_pos_ids_inplace",
     "apply_llama31_rope_pos_ids_inplace",
     "append_paged_kv_cache",

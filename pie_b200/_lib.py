@@ -51,7 +51,7 @@ class RopeParams(C.Structure):
 class AttnOptions(C.Structure):
     """Mirror of `piekv_attn_options`."""
 
-    _fields_ = [("window_left", C.c_int32), ("reserved", C.c_int32), ("sinks", C.c_void_p)]
+    _fields_ = [("window_left", C.c_int32), ("first_tokens", C.c_int32), ("sinks", C.c_void_p)]
 
 
 class WireBatch(C.Structure):
@@ -68,6 +68,41 @@ class QkvOptions(C.Structure):
     _fields_ = [("bias", C.c_void_p), ("q_norm_weight", C.c_void_p), ("k_norm_weight", C.c_void_p),
                 ("rms_eps", C.c_float), ("reserved", C.c_int32)]
 
+
+class SharedPrefixArgs(C.Structure):
+    """Mirror of `piekv_shared_prefix_args`."""
+
+    _fields_ = [("q", C.c_void_p), ("q_stride_n", C.c_int64), ("q_stride_h", C.c_int64), ("pool", C.c_void_p),
+                ("out", C.c_void_p), ("lse", C.c_void_p), ("kv_indptr", C.c_void_p), ("kv_indices", C.c_void_p),
+                ("kv_last_page_len", C.c_void_p), ("group_indptr", C.c_void_p), ("sinks", C.c_void_p),
+                ("plan", C.c_void_p), ("plan_bytes", C.c_int64), ("workspace", C.c_void_p),
+                ("workspace_bytes", C.c_int64), ("err", C.c_void_p)] + \
+               [(n, C.c_int32) for n in ("batch", "num_groups", "num_qo_heads", "num_kv_heads", "head_dim", "page_size",
+                                         "num_pages", "dtype", "max_splits")] + [("sm_scale", C.c_float)]
+
+
+class RopeAxesArgs(C.Structure):
+    """Mirror of `piekv_rope_axes_args`."""
+
+    _fields_ = [(n, C.c_void_p) for n in ("q", "k", "v", "q_out", "k_out")] + \
+               [(n, C.c_int64) for n in ("q_stride_n", "q_stride_h", "k_stride_n", "k_stride_h", "v_stride_n",
+                                         "v_stride_h", "q_out_stride_n", "q_out_stride_h", "k_out_stride_n",
+                                         "k_out_stride_h")] + \
+               [("pos", C.c_void_p), ("pos_stride", C.c_int64)] + \
+               [(n, C.c_void_p) for n in ("batch_indices", "positions", "pool", "kv_indices", "kv_indptr", "err")] + \
+               [(n, C.c_int32) for n in ("nnz", "batch", "num_qo_heads", "num_kv_heads", "head_dim", "page_size",
+                                         "num_pages", "dtype")]
+
+
+class RopeAxesTable(C.Structure):
+    """Mirror of `piekv_rope_axes_table`."""
+
+    _fields_ = [("turn", C.c_uint64 * 128), ("axis", C.c_uint8 * 128), ("cos_sin_table", C.c_void_p)] + \
+               [(n, C.c_int32) for n in ("table_len", "num_axes", "half", "interleave")]
+
+
+MAX_ROPE_AXES = 4
+SHARED_PREFIX_MAX_SPLITS = 64
 
 MAX_PEERS = 8
 PEER_HANDLE_BYTES = 64
@@ -140,6 +175,14 @@ SIGNATURES = {
         [_p, _i64, _p, _i64, _p, _p, _p, _p, _p, _p, _p, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32,
          C.POINTER(RopeParams), _p, _p, C.POINTER(QkvOptions)],
     ),
+    "piekv_decode_first_tokens_workspace_bytes": (_i64, [_i32, _i32, _i32, _i32]),
+    "piekv_shared_prefix_plan_bytes": (_i64, [_i32, _i32, _i32, _i32]),
+    "piekv_shared_prefix_workspace_bytes": (_i64, [_i32, _i32, _i32, _i32, _i32]),
+    "piekv_shared_prefix_plan": (C.c_int, [C.POINTER(SharedPrefixArgs), _p]),
+    "piekv_shared_prefix_run": (C.c_int, [C.POINTER(SharedPrefixArgs), _p]),
+    "piekv_rope_axes_prepare": (C.c_int, [C.POINTER(RopeParams), C.POINTER(C.c_int32), _i32, _i32,
+                                          C.POINTER(RopeAxesTable)]),
+    "piekv_rope_axes": (C.c_int, [C.POINTER(RopeAxesArgs), C.POINTER(RopeAxesTable), _p]),
     "piekv_oproj_allreduce_sizes": (C.c_int, [_i32, _i32, _i32, C.POINTER(C.c_int64)]),
     "piekv_oproj_tile_cols": (_i32, [_i32, _i32]),
     "piekv_oproj_allreduce": (

@@ -24,6 +24,8 @@ struct AttnArgs {
   // -1: no window.  The decode and generic kernels apply it themselves; the tensor-core prefill kernels
   // get it through the packed mask their plan builds.
   int window_left = -1;
+  // With a window: keys 0 .. first_tokens - 1 stay visible behind it (0: none).
+  int first_tokens = 0;
   // Attention sinks: nullable fp32 [Hq].  The head's sink logit joins the softmax normaliser (it takes
   // probability mass) but has no value row.
   const float *sinks = nullptr;

@@ -52,10 +52,20 @@ extern "C" int64_t piekv_decode_workspace_bytes(int32_t batch, int32_t num_qo_he
   return a > b ? a : b;
 }
 
+extern "C" int64_t piekv_decode_first_tokens_workspace_bytes(int32_t batch, int32_t num_qo_heads,
+                                                             int32_t num_kv_heads, int32_t head_dim) {
+  (void)head_dim;
+  if (batch < 0 || num_qo_heads <= 0 || num_kv_heads <= 0) return 0;
+  return kCounterBytes;
+}
+
 static int apply_options(AttnArgs &a, const piekv_attn_options *opt, const char *who) {
   if (opt == nullptr) return 0;
   PIEKV_REQUIRE(opt->window_left >= -1, "%s: window_left %d (use -1 for no window)", who, opt->window_left);
+  PIEKV_REQUIRE(opt->first_tokens >= 0, "%s: first_tokens %d is negative", who, opt->first_tokens);
   a.window_left = opt->window_left;
+  // without a window nothing is hidden that the first tokens could keep visible
+  a.first_tokens = opt->window_left >= 0 ? opt->first_tokens : 0;
   a.sinks = opt->sinks;
   return 0;
 }
@@ -91,6 +101,7 @@ extern "C" int piekv_decode_run_opt(const void *q, int64_t q_stride_n, int64_t q
   if (int rc = check_common(a, dtype, "decode_run")) return rc;
   if (int rc = apply_options(a, opt, "decode_run")) return rc;
   if (batch == 0) return 0;
+  if (a.first_tokens > 0) return launch_attn_generic(a, dtype, (cudaStream_t)stream);
   if (decode_tma_supported(a, dtype)) return launch_decode_tma(a, dtype, workspace, workspace_bytes, (cudaStream_t)stream);
   return launch_attn_generic(a, dtype, (cudaStream_t)stream);
 }
@@ -135,6 +146,7 @@ static int decode_step_fused_impl(const void *q, const void *k, const void *v, i
   a.err = err;
   if (int rc = check_common(a, dtype, "decode_step_fused")) return rc;
   if (int rc = apply_options(a, opt, "decode_step_fused")) return rc;
+  PIEKV_REQUIRE(a.first_tokens == 0, "decode_step_fused: first_tokens is not taken by the fused step (append, then decode_run)");
   if (int rc = check_rope(rope, head_dim, "decode_step_fused")) return rc;
   if (batch == 0) return 0;
   PIEKV_REQUIRE(k && v, "decode_step_fused: null k / v");
@@ -356,6 +368,8 @@ extern "C" int piekv_prefill_run_opt(const void *q, int64_t q_stride_n, int64_t 
                     sm_scale, err);
   if (int rc = check_common(a, dtype, "prefill_run")) return rc;
   if (int rc = apply_options(a, opt, "prefill_run")) return rc;
+  PIEKV_REQUIRE(a.first_tokens == 0 || (custom_mask == nullptr && planned != 2),
+                "prefill_run: first_tokens cannot be combined with a mask");
   PIEKV_REQUIRE(nnz == 0 || qo_indptr != nullptr, "prefill_run: qo_indptr is null");
   if (batch == 0 || nnz == 0) return 0;
   if (planned == 2) {
@@ -364,7 +378,7 @@ extern "C" int piekv_prefill_run_opt(const void *q, int64_t q_stride_n, int64_t 
     a.mask = reinterpret_cast<const uint8_t *>(workspace);  // marks "masked"; the packed form is what is read
     a.causal = 0;
   }
-  if (prefill_tc_supported(a, dtype)) {
+  if (a.first_tokens == 0 && prefill_tc_supported(a, dtype)) {
     if (!planned) {
       if (int rc = launch_prefill_plan(a, mask_bytes, workspace, workspace_bytes, (cudaStream_t)stream)) return rc;
     }

@@ -57,7 +57,7 @@ __global__ void __launch_bounds__(128) attn_generic_kernel(AttnArgs a) {
     int c = kv_len - qo_len + j + 1;
     limit = c < limit ? c : limit;
   }
-  // sliding window: keys before (position of this query) - window_left are not seen
+  // sliding window: keys before (position of this query) - window_left are not seen, except the first tokens
   int t_first = 0;
   if (a.window_left >= 0) {
     const int first = kv_len - qo_len + j - a.window_left;
@@ -92,7 +92,12 @@ __global__ void __launch_bounds__(128) attn_generic_kernel(AttnArgs a) {
   const size_t half_page = (size_t)a.page_size * row_elems;
   const T *pool = reinterpret_cast<const T *>(a.pool);
 
-  for (int t = t_first; t < limit; ++t) {
+  const int front = a.window_left >= 0 ? (a.first_tokens < t_first ? a.first_tokens : t_first) : 0;
+  for (int t = front > 0 ? 0 : t_first; t < limit; ++t) {
+    if (front > 0 && t == front) {  // behind the first tokens: on to the window
+      t = t_first;
+      if (t >= limit) break;
+    }
     if (mrow != nullptr && mrow[t] == 0) continue;
     int page = a.kv_indices[p0 + t / a.page_size];
     if (page < 0 || page >= a.num_pages) {

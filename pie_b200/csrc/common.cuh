@@ -61,6 +61,8 @@ enum KernelId : int {
   KID_PREFILL = 7,
   KID_PEER = 8,
   KID_PAGES = 9,
+  KID_SHARED_PREFIX = 10,
+  KID_ROPE_AXES = 11,
 };
 
 // ---- device side -------------------------------------------------------------------

@@ -457,6 +457,26 @@ __global__ void __launch_bounds__(256) append_tokens_warp_kernel(AppendArgs a) {
 // Per-pair frequencies in double, rounded once to fp32.  Formula of
 // pie/src/flashinfer_metal/kernels/metal_rope.metal:66-89 with the low/high/old_context
 // parameters the reference passes at pie/src/pie_worker/model/llama3.py:660-669.
+double pair_frequency(const piekv_rope_params *rope, int head_dim, int i) {
+  const double two_pi = 6.283185307179586476925286766559;
+  double f = pow((double)rope->theta, -2.0 * (double)i / (double)head_dim);
+  if (rope->mode == PIEKV_ROPE_PLAIN && rope->scale > 0.f) f = f / (double)rope->scale;
+  if (rope->mode == PIEKV_ROPE_LLAMA31) {
+    double scale = rope->scale, lowf = rope->low_freq_factor, highf = rope->high_freq_factor;
+    double old = rope->old_context_len;
+    double wavelen = two_pi / f;
+    if (wavelen > old / lowf) {
+      f = f / scale;
+    } else if (wavelen < old / highf) {
+      // unchanged
+    } else {
+      double smooth = (old / wavelen - lowf) / (highf - lowf);
+      f = (1.0 - smooth) * (f / scale) + smooth * f;
+    }
+  }
+  return f;
+}
+
 void fill_inv_freq(const piekv_rope_params *rope, int head_dim, RopeDev *out) {
   const int half = head_dim / 2;
   out->mode = rope ? rope->mode : PIEKV_ROPE_NONE;
@@ -465,25 +485,7 @@ void fill_inv_freq(const piekv_rope_params *rope, int head_dim, RopeDev *out) {
   out->table = rope ? rope->cos_sin_table : nullptr;
   for (int i = 0; i < kMaxHalfDim; ++i) out->inv_freq[i] = 0.f;
   if (!rope || (rope->mode != PIEKV_ROPE_PLAIN && rope->mode != PIEKV_ROPE_LLAMA31)) return;
-  const double two_pi = 6.283185307179586476925286766559;
-  for (int i = 0; i < half; ++i) {
-    double f = pow((double)rope->theta, -2.0 * (double)i / (double)head_dim);
-    if (rope->mode == PIEKV_ROPE_PLAIN && rope->scale > 0.f) f = f / (double)rope->scale;
-    if (rope->mode == PIEKV_ROPE_LLAMA31) {
-      double scale = rope->scale, lowf = rope->low_freq_factor, highf = rope->high_freq_factor;
-      double old = rope->old_context_len;
-      double wavelen = two_pi / f;
-      if (wavelen > old / lowf) {
-        f = f / scale;
-      } else if (wavelen < old / highf) {
-        // unchanged
-      } else {
-        double smooth = (old / wavelen - lowf) / (highf - lowf);
-        f = (1.0 - smooth) * (f / scale) + smooth * f;
-      }
-    }
-    out->inv_freq[i] = (float)f;
-  }
+  for (int i = 0; i < half; ++i) out->inv_freq[i] = (float)pair_frequency(rope, head_dim, i);
 }
 
 static bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }

@@ -62,6 +62,9 @@ extern "C" int32_t piekv_abi_sizeof(int32_t which) {
   if (which == 3) return (int32_t)sizeof(piekv_wire_batch);
   if (which == 4) return (int32_t)sizeof(piekv_qkv_options);
   if (which == 5) return (int32_t)sizeof(piekv_peer_reduce);
+  if (which == 6) return (int32_t)sizeof(piekv_shared_prefix_args);
+  if (which == 7) return (int32_t)sizeof(piekv_rope_axes_args);
+  if (which == 8) return (int32_t)sizeof(piekv_rope_axes_table);
   return -1;
 }
 

@@ -14,6 +14,8 @@ struct RopeDev {
   float inv_freq[kMaxHalfDim];  // final per-pair frequency (plain or Llama-3.1 scaled), fp32
 };
 
+// Frequency of pair i of a rotary width `head_dim` (plain or Llama-3.1 scaled), in double (host).
+double pair_frequency(const piekv_rope_params *rope, int head_dim, int i);
 // Per-pair frequencies evaluated in double and rounded once to fp32 (host).
 void fill_inv_freq(const piekv_rope_params *rope, int head_dim, RopeDev *out);
 // Host-side validation shared by the entry points; 0 or a >0 status with the error text set.

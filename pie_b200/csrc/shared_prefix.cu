@@ -1,0 +1,238 @@
+// Decode attention for groups of requests that share the leading pages of their contexts.
+#include "attn.cuh"
+#include "common.cuh"
+#include "shared_prefix.cuh"
+
+namespace piekv {
+
+using namespace sprefix;
+
+namespace {
+
+constexpr int64_t kCounterBytes = 65536;
+// A prefix shorter than this is left to the requests: reading it once saves less than joining two parts costs.
+constexpr int kMinSharedPages = 4;
+constexpr int kMinTilesPerItem = 2;
+
+// Full pages of request b (the partly filled last page of a fork is a copy of its own).
+__device__ __forceinline__ int full_pages(const int32_t *kv_indptr, const int32_t *last, int b, int page_size) {
+  const int np = kv_indptr[b + 1] - kv_indptr[b];
+  return np <= 0 ? 0 : (last[b] >= page_size ? np : np - 1);
+}
+
+// How many leading full pages request b has in common with its group's first request.  One block per request.
+__global__ void __launch_bounds__(128) sp_match_kernel(const int32_t *__restrict__ kv_indptr,
+                                                       const int32_t *__restrict__ kv_indices,
+                                                       const int32_t *__restrict__ last,
+                                                       const int32_t *__restrict__ group_indptr, int batch, int groups,
+                                                       int page_size, int *match) {
+  __shared__ int sh_first;
+  const int b = blockIdx.x;
+  int lo = 0, hi = groups - 1;  // first g with group_indptr[g + 1] > b
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (group_indptr[mid + 1] > b)
+      hi = mid;
+    else
+      lo = mid + 1;
+  }
+  const int leader = min(max(group_indptr[lo], 0), batch - 1);  // (a bad grouping is refused by the plan kernel)
+  const int n = min(full_pages(kv_indptr, last, b, page_size), full_pages(kv_indptr, last, leader, page_size));
+  const int32_t *x = kv_indices + kv_indptr[b], *y = kv_indices + kv_indptr[leader];
+  if (threadIdx.x == 0) sh_first = n;
+  __syncthreads();
+  if (b != leader) {
+    for (int base = 0; base < n; base += 4 * 128) {
+      int bad = n;
+#pragma unroll
+      for (int u = 3; u >= 0; --u) {
+        const int j = base + u * 128 + threadIdx.x;
+        if (j < n && x[j] != y[j]) bad = j;
+      }
+      if (__syncthreads_or(bad < n)) {
+        if (bad < n) atomicMin(&sh_first, bad);
+        break;
+      }
+    }
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) match[b] = sh_first;
+}
+
+// Checks the grouping, decides what every group reads once and lists the pieces of work.  One block.
+__global__ void __launch_bounds__(1024) sp_plan_kernel(const int32_t *__restrict__ group_indptr, int batch, int groups,
+                                                       int page_size, int heads_per_kv, int hkv, int max_splits,
+                                                       int sms, PlanView v, int32_t *err) {
+  __shared__ long long sh_tiles;
+  __shared__ int sh_base, sh_most, sh_per, sh_used, sh_count;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (tid == 0) {
+    sh_tiles = 0;
+    sh_base = sh_most = sh_used = sh_count = 0;
+    sh_per = 1 << 30;
+  }
+  int bad = -1;
+  for (int g = tid; g < groups; g += 1024) {
+    const int a = group_indptr[g], e = group_indptr[g + 1];
+    if (a > e || a < 0 || e > batch || (g == 0 && a != 0) || (g == groups - 1 && e != batch)) bad = g;
+  }
+  if (bad >= 0) report_error(err, PIEKV_ERR_INDPTR, KID_SHARED_PREFIX, bad, group_indptr[bad]);
+  const bool refused = __syncthreads_or(bad >= 0) != 0;
+  if (refused) {  // every request on its own
+    for (int b = tid; b < batch; b += 1024) v.requests[b] = make_int2(0, 0);
+    if (tid == 0) v.header[0] = v.header[1] = 0;
+    return;
+  }
+  // ---- a warp per group: pages common to all its requests
+  for (int g = warp; g < groups; g += 32) {
+    const int a = group_indptr[g], m = group_indptr[g + 1] - a;
+    int pages = 1 << 30;
+    for (int i = lane; i < m; i += 32) pages = min(pages, v.match[a + i]);
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) pages = min(pages, __shfl_xor_sync(0xffffffffu, pages, d));
+    if (m < 2 || pages < kMinSharedPages) pages = 0;
+    for (int i = lane; i < m; i += 32) v.requests[a + i] = make_int2(pages, g);
+    if (lane == 0) {
+      v.groups[g] = Group{a, m, pages, 0};
+      if (pages > 0) {
+        const int tiles = (pages * page_size + kTileTokens - 1) / kTileTokens;
+        const int blocks = (int)(((long long)m * heads_per_kv + kRowsPerItem - 1) / kRowsPerItem) * hkv;
+        atomicAdd(reinterpret_cast<unsigned long long *>(&sh_tiles), (unsigned long long)tiles * blocks);
+        atomicAdd(&sh_base, blocks);
+        atomicMax(&sh_most, tiles);
+        atomicAdd(&sh_used, 1);
+      }
+    }
+  }
+  __syncthreads();
+  // ---- tiles per piece: one piece per SM where that is possible (each thread tries a length), four rounds of
+  // pieces where there are more (group, kv head, row block) triples than SMs
+  const long long total = sh_tiles;
+  const int base = sh_base, most = sh_most;
+  auto blocks_of = [&](const Group &g) {
+    return (int)(((long long)g.members * heads_per_kv + kRowsPerItem - 1) / kRowsPerItem) * hkv;
+  };
+  auto tiles_of = [&](const Group &g) { return (g.pages * page_size + kTileTokens - 1) / kTileTokens; };
+  if (base > sms) {
+    if (tid == 0) sh_per = max(kMinTilesPerItem, (int)((total + 4 * sms - 1) / (4 * sms)));
+  } else if (base > 0) {
+    const int least = max(kMinTilesPerItem, (int)((total + sms - 1) / sms));
+    for (int per = least + tid; per < most && per < sh_per; per += 1024) {
+      int n = 0;
+      for (int g = 0; g < groups && n <= sms; ++g) {
+        const Group gr = v.groups[g];
+        if (gr.pages > 0) n += blocks_of(gr) * ((tiles_of(gr) + per - 1) / per);
+      }
+      if (n <= sms) {
+        atomicMin(&sh_per, per);
+        break;
+      }
+    }
+  }
+  __syncthreads();
+  const int per = min(sh_per, max(most, 1));
+  const int max_chunks = max(1, max_splits / 2);
+  for (int g = warp; g < groups; g += 32) {
+    Group gr = v.groups[g];
+    if (gr.pages == 0) continue;
+    const int blocks = blocks_of(gr) / hkv;
+    int chunks = min((tiles_of(gr) + per - 1) / per, max_chunks);
+    int at = 0;
+    if (lane == 0) {
+      at = atomicAdd(&sh_count, blocks * hkv * chunks);
+      if (at + blocks * hkv * chunks > v.max_items) {  // (cannot happen: kept so that nothing is written out of range)
+        report_error(err, PIEKV_ERR_PAGE_CAPACITY, KID_SHARED_PREFIX, g, chunks);
+        chunks = 0;
+      }
+      v.groups[g].chunks = chunks;
+    }
+    at = __shfl_sync(0xffffffffu, at, 0);
+    chunks = __shfl_sync(0xffffffffu, chunks, 0);
+    for (int i = lane; i < blocks * hkv * chunks; i += 32)
+      v.items[at + i] = Item{g, i % hkv, (i / hkv) % blocks, i / (hkv * blocks)};
+  }
+  __syncthreads();
+  if (tid == 0) {
+    v.header[0] = min(sh_count, v.max_items);
+    v.header[1] = sh_used;
+  }
+}
+
+int check_args(const piekv_shared_prefix_args *a, const char *who) {
+  PIEKV_REQUIRE(a != nullptr, "%s: null arguments", who);
+  PIEKV_REQUIRE(a->dtype >= PIEKV_F32 && a->dtype <= PIEKV_BF16, "%s: unknown dtype %d", who, a->dtype);
+  PIEKV_REQUIRE(a->batch >= 0 && a->num_groups >= 0, "%s: negative batch / num_groups", who);
+  PIEKV_REQUIRE(a->num_qo_heads > 0 && a->num_kv_heads > 0 && a->num_qo_heads % a->num_kv_heads == 0,
+                "%s: num_qo_heads %d not a multiple of num_kv_heads %d", who, a->num_qo_heads, a->num_kv_heads);
+  PIEKV_REQUIRE(a->head_dim > 0 && a->page_size > 0, "%s: bad head_dim / page_size", who);
+  PIEKV_REQUIRE(a->max_splits >= 1 && a->max_splits <= PIEKV_SHARED_PREFIX_MAX_SPLITS, "%s: max_splits %d not in 1..%d", who,
+                a->max_splits, PIEKV_SHARED_PREFIX_MAX_SPLITS);
+  if (a->batch == 0) return 0;
+  PIEKV_REQUIRE(a->num_groups > 0, "%s: no groups for %d requests", who, a->batch);
+  PIEKV_REQUIRE(a->kv_indptr && a->kv_indices && a->kv_last_page_len && a->group_indptr, "%s: null pointer", who);
+  const int64_t need = piekv_shared_prefix_plan_bytes(a->batch, a->num_groups, a->num_qo_heads, a->num_kv_heads);
+  PIEKV_REQUIRE(a->plan != nullptr && a->plan_bytes >= need, "%s: plan too small (%lld < %lld bytes)", who,
+                (long long)a->plan_bytes, (long long)need);
+  PIEKV_REQUIRE((reinterpret_cast<uintptr_t>(a->plan) & 255) == 0, "%s: plan must be 256-byte aligned", who);
+  return 0;
+}
+
+}  // namespace
+}  // namespace piekv
+
+using namespace piekv;
+
+extern "C" int64_t piekv_shared_prefix_plan_bytes(int32_t batch, int32_t num_groups, int32_t num_qo_heads,
+                                                  int32_t num_kv_heads) {
+  if (batch < 0 || num_groups < 0 || num_qo_heads <= 0 || num_kv_heads <= 0) return 0;
+  return plan_view(nullptr, batch, num_groups, num_qo_heads, num_kv_heads).bytes;
+}
+
+extern "C" int64_t piekv_shared_prefix_workspace_bytes(int32_t batch, int32_t num_qo_heads, int32_t num_kv_heads,
+                                                       int32_t head_dim, int32_t max_splits) {
+  (void)head_dim;
+  if (batch < 0 || num_qo_heads <= 0 || num_kv_heads <= 0 || max_splits < 1) return 0;
+  return kCounterBytes;
+}
+
+extern "C" int piekv_shared_prefix_plan(const piekv_shared_prefix_args *args, void *stream) {
+  if (int rc = check_args(args, "shared_prefix_plan")) return rc;
+  const piekv_shared_prefix_args &a = *args;
+  if (a.batch == 0) return 0;
+  const PlanView v = plan_view(a.plan, a.batch, a.num_groups, a.num_qo_heads, a.num_kv_heads);
+  cudaStream_t st = (cudaStream_t)stream;
+  sp_match_kernel<<<a.batch, 128, 0, st>>>(a.kv_indptr, a.kv_indices, a.kv_last_page_len, a.group_indptr, a.batch,
+                                           a.num_groups, a.page_size, v.match);
+  PIEKV_LAUNCH_CHECK("sp_match_kernel");
+  sp_plan_kernel<<<1, 1024, 0, st>>>(a.group_indptr, a.batch, a.num_groups, a.page_size, a.num_qo_heads / a.num_kv_heads,
+                                     a.num_kv_heads, a.max_splits, sm_count(), v, a.err);
+  PIEKV_LAUNCH_CHECK("sp_plan_kernel");
+  return 0;
+}
+
+extern "C" int piekv_shared_prefix_run(const piekv_shared_prefix_args *args, void *stream) {
+  if (int rc = check_args(args, "shared_prefix_run")) return rc;
+  if (args->batch == 0) return 0;
+  PIEKV_REQUIRE(args->num_pages > 0, "shared_prefix_run: bad num_pages");
+  PIEKV_REQUIRE(args->q && args->pool && args->out, "shared_prefix_run: null pointer");
+  AttnArgs a{};
+  a.q = args->q;
+  a.q_sn = args->q_stride_n;
+  a.q_sh = args->q_stride_h;
+  a.pool = args->pool;
+  a.out = args->out;
+  a.lse = args->lse;
+  a.kv_indptr = args->kv_indptr;
+  a.kv_indices = args->kv_indices;
+  a.kv_last_page_len = args->kv_last_page_len;
+  a.batch = a.nnz = args->batch;
+  a.hq = args->num_qo_heads;
+  a.hkv = args->num_kv_heads;
+  a.dim = args->head_dim;
+  a.page_size = args->page_size;
+  a.num_pages = args->num_pages;
+  a.sm_scale = args->sm_scale;
+  a.err = args->err;
+  a.sinks = args->sinks;
+  return launch_attn_generic(a, args->dtype, (cudaStream_t)stream);
+}

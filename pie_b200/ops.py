@@ -41,6 +41,10 @@ __all__ = [
     "get_seq_lens",
     "get_batch_indices_positions",
     "rope_append_paged_kv_cache",
+    "BatchSharedPrefixDecodeWrapper",
+    "apply_rope_axes_inplace",
+    "rope_axes_append_paged_kv_cache",
+    "AxisRopeConfig",
     "copy_kv_pages",
     "RopeConfig",
     "device_error",
@@ -446,6 +450,123 @@ def qkv_rope_append_paged_kv_cache(x: torch.Tensor, w_qkv: torch.Tensor, pos_ids
     return q_out
 
 
+@dataclass
+class AxisRopeConfig(RopeConfig):
+    """Rotary parameters for positions on several axes (time, height, width of images and video).
+
+    `sections` says how many (cos, sin) pairs of a head row belong to each axis; the rotary width is twice their sum
+    and may be smaller than head_dim (the elements behind it stay as they are).  `cyclic=False`: the pairs are dealt
+    out in blocks, the first sections[0] to axis 0 and so on; `cyclic=True`: in turn (pair i to axis i mod axes while
+    that axis has pairs left, the rest to axis 0).  `mode`: "plain" | "llama31" | "table"; a `cos_sin_table` has rows
+    of the rotary width and pair i reads the row of its own axis' position."""
+
+    sections: Tuple[int, ...] = ()
+    cyclic: bool = False
+
+    def prepared(self) -> "_lib.RopeAxesTable":
+        """The host table the kernels take, laid out once per set of parameters."""
+        t = self.cos_sin_table if self.mode == "table" else None
+        key = (self.mode, self.theta, self.scale, self.low_freq_factor, self.high_freq_factor, self.old_context_len,
+               self.interleave, tuple(self.sections), self.cyclic,
+               None if t is None else (t.data_ptr(), tuple(t.shape), t.dtype, t.device, t.is_contiguous()))
+        have = self.__dict__.get("_prepared")
+        if have is not None and have[0] == key:
+            return have[1]
+        sections = [int(x) for x in self.sections]
+        if not 1 <= len(sections) <= _lib.MAX_ROPE_AXES:
+            raise ValueError(f"sections must name 1 to {_lib.MAX_ROPE_AXES} axes, got {len(sections)}")
+        if self.mode == "none":
+            raise ValueError("rope mode 'none' has no angles; use append_paged_kv_cache")
+        rp = self.to_c(2 * sum(sections))
+        table = _lib.RopeAxesTable()
+        check(lib.piekv_rope_axes_prepare(C.byref(rp), (C.c_int32 * len(sections))(*sections), len(sections),
+                                          1 if self.cyclic else 0, C.byref(table)), "AxisRopeConfig")
+        self.__dict__["_prepared"] = (key, table)
+        return table
+
+
+def _rope_axes(q, k, v, pos_ids, rope: AxisRopeConfig, q_out, k_out, who: str, append=None) -> None:
+    if not isinstance(rope, AxisRopeConfig):
+        raise ValueError(f"{who}: rope must be an AxisRopeConfig")
+    _require_cuda(k, "k")
+    _require_cuda(pos_ids, "pos_ids")
+    table = rope.prepared()
+    n, hkv, d = k.shape if k.dim() == 3 else (0, 0, 0)
+    a = _lib.RopeAxesArgs()
+    a.k_stride_n, a.k_stride_h = _rows(k, "k")
+    a.k = k.data_ptr()
+    if pos_ids.dtype != torch.int32 or pos_ids.dim() != 2 or pos_ids.shape[0] != table.num_axes or \
+            pos_ids.shape[1] < n or (n > 1 and pos_ids.stride(1) != 1):
+        raise ValueError(f"{who}: pos_ids must be int32 [{table.num_axes} axes, {n} tokens] with contiguous rows, got "
+                         f"{tuple(pos_ids.shape)} {pos_ids.dtype}")
+    a.pos, a.pos_stride = pos_ids.data_ptr(), pos_ids.stride(0)
+    if 2 * table.half > d:
+        raise ValueError(f"{who}: sections of {table.half} pairs do not fit head_dim {d}")
+    same = [k, pos_ids]
+    if q is not None:
+        _require_cuda(q, "q")
+        a.q_stride_n, a.q_stride_h = _rows(q, "q")
+        if q.shape[0] != n or q.shape[2] != d or q.dtype != k.dtype:
+            raise ValueError(f"{who}: q {tuple(q.shape)} {q.dtype} does not match k {tuple(k.shape)} {k.dtype}")
+        if q_out.shape != q.shape or q_out.dtype != q.dtype:
+            raise ValueError(f"{who}: q_out must be shaped and typed like q")
+        a.q_out_stride_n, a.q_out_stride_h = _rows(q_out, "q_out")
+        a.q, a.q_out, a.num_qo_heads = q.data_ptr(), q_out.data_ptr(), q.shape[1]
+        same += [q, q_out]
+    if k_out is not None:
+        a.k_out, (a.k_out_stride_n, a.k_out_stride_h) = k_out.data_ptr(), _rows(k_out, "k_out")
+    if append is not None:
+        batch_indices, positions, pool, kv_indices, kv_indptr = append
+        _require_cuda(v, "v")
+        a.v_stride_n, a.v_stride_h = _rows(v, "v")
+        num_pages, page_size, pool_heads, pool_dim = _check_pool(pool)
+        if (hkv, d) != (pool_heads, pool_dim) or v.shape != k.shape:
+            raise ValueError(f"{who}: key {tuple(k.shape)} / value {tuple(v.shape)} do not match the cache "
+                             f"[*, {pool_heads}, {pool_dim}]")
+        if k.dtype != pool.dtype or v.dtype != pool.dtype:
+            raise ValueError(f"{who}: key/value dtype {k.dtype}/{v.dtype} differs from the cache dtype {pool.dtype}")
+        for t, name in ((batch_indices, "batch_indices"), (positions, "positions"), (kv_indices, "kv_indices"),
+                        (kv_indptr, "kv_indptr")):
+            _require_i32(t, name)
+        if batch_indices.shape[0] < n or positions.shape[0] < n:
+            raise ValueError(f"{who}: batch_indices / positions shorter than the number of tokens")
+        a.v, a.pool = v.data_ptr(), pool.data_ptr()
+        a.batch_indices, a.positions = batch_indices.data_ptr(), positions.data_ptr()
+        a.kv_indices, a.kv_indptr, a.batch = kv_indices.data_ptr(), kv_indptr.data_ptr(), kv_indptr.shape[0] - 1
+        a.num_pages, a.page_size = num_pages, page_size
+        same += [v, pool, batch_indices, positions, kv_indices, kv_indptr]
+    for t in same:
+        if t.device != k.device:
+            raise ValueError(f"{who}: tensors on {t.device} and {k.device}")
+    if rope.mode == "table" and rope.cos_sin_table.device != k.device:
+        raise ValueError(f"{who}: cos_sin_table on {rope.cos_sin_table.device}, k on {k.device}")
+    a.nnz, a.num_kv_heads, a.head_dim, a.dtype = n, hkv, d, _dtype_code(k.dtype, who)
+    a.err = _err_word(k.device).data_ptr()
+    check(lib.piekv_rope_axes(C.byref(a), C.byref(table), _stream(k.device)), who)
+
+
+def apply_rope_axes_inplace(q: Optional[torch.Tensor], k: torch.Tensor, pos_ids: torch.Tensor, rope: AxisRopeConfig) -> None:
+    """Rotary embedding in place with one position per axis: `pos_ids` int32 [axes, tokens].  The angles are formed
+    in 64-bit fixed point, as exact at position 10^6 as at 10."""
+    _rope_axes(q, k, None, pos_ids, rope, q, k, "apply_rope_axes_inplace")
+
+
+def rope_axes_append_paged_kv_cache(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, pos_ids: torch.Tensor,
+                                    batch_indices: torch.Tensor, positions: torch.Tensor, paged_kv_cache: torch.Tensor,
+                                    kv_indices: torch.Tensor, kv_indptr: torch.Tensor, kv_last_page_len: torch.Tensor,
+                                    rope: AxisRopeConfig, q_out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+    """`rope_append_paged_kv_cache` for tokens with a position per axis (`pos_ids` int32 [axes, tokens]): k is rotated
+    on its way into the paged cache, v is copied, rotated q is returned (in `q_out`, which may be q itself; k, v and,
+    with another q_out, q are read only).  `positions` are the tokens' slots in their contexts, as in
+    append_paged_kv_cache; a token whose request, slot or page does not exist is skipped and reported
+    (`device_error`), its q is still rotated."""
+    if q is not None and q_out is None:
+        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    _rope_axes(q, k, v, pos_ids, rope, q_out, None, "rope_axes_append_paged_kv_cache",
+               (batch_indices, positions, paged_kv_cache, kv_indices, kv_indptr))
+    return q_out
+
+
 def copy_kv_pages(kv_cache_at_layer: Sequence[torch.Tensor], src_pages: torch.Tensor, dst_pages: torch.Tensor,
                   valid_len: Optional[torch.Tensor] = None) -> None:
     """Copy the first `valid_len[j]` token rows (default: all) of page src[j] to page dst[j] in every
@@ -490,22 +611,33 @@ def _check_workspace(ws: torch.Tensor) -> None:
         raise ValueError(f"workspace_buffer must hold at least {COUNTER_BYTES} bytes")
 
 
-def _attn_options(window_left: int, sinks: Optional[torch.Tensor], num_qo_heads: int):
+def _attn_options(window_left: int, sinks: Optional[torch.Tensor], num_qo_heads: int, first_tokens: int = 0):
     """ctypes `piekv_attn_options` (or None when there is neither a window nor sinks)."""
     if window_left < 0 and sinks is None:
         return None
     o = _lib.AttnOptions()
     o.window_left = int(window_left) if window_left >= 0 else -1
-    o.reserved = 0
-    o.sinks = None
-    if sinks is not None:
-        _require_cuda(sinks, "sinks")
-        if sinks.dtype != torch.float32 or sinks.dim() != 1 or sinks.shape[0] != num_qo_heads or \
-                not sinks.is_contiguous():
-            raise ValueError(f"sinks must be a contiguous float32 tensor of {num_qo_heads} entries (one per query "
-                             f"head), got {tuple(sinks.shape)} {sinks.dtype}")
-        o.sinks = sinks.data_ptr()
+    o.first_tokens = int(first_tokens) if window_left >= 0 else 0
+    o.sinks = _sink_ptr(sinks, num_qo_heads)
     return o
+
+
+def _sink_ptr(sinks: Optional[torch.Tensor], num_qo_heads: int) -> Optional[int]:
+    if sinks is None:
+        return None
+    _require_cuda(sinks, "sinks")
+    if sinks.dtype != torch.float32 or sinks.dim() != 1 or sinks.shape[0] != num_qo_heads or not sinks.is_contiguous():
+        raise ValueError(f"sinks must be a contiguous float32 tensor of {num_qo_heads} entries (one per query "
+                         f"head), got {tuple(sinks.shape)} {sinks.dtype}")
+    return sinks.data_ptr()
+
+
+def _check_first_tokens(first_tokens: int, window_left: int) -> int:
+    """Validated `first_tokens`; 0 without a window, which then hides nothing that they could keep visible."""
+    n = int(first_tokens)
+    if n < 0:
+        raise ValueError(f"first_tokens must be >= 0, got {n}")
+    return n if window_left >= 0 else 0
 
 
 class BatchDecodeWithPagedKVCacheWrapper:
@@ -543,7 +675,11 @@ class BatchDecodeWithPagedKVCacheWrapper:
              num_kv_heads: int, head_dim: int, page_size: int, pos_encoding_mode: str = "NONE",
              window_left: int = -1, logits_soft_cap: Optional[float] = None,
              q_data_type: torch.dtype = torch.float16, kv_data_type: Optional[torch.dtype] = None,
-             data_type: Optional[torch.dtype] = None, sm_scale: Optional[float] = None, **_ignored) -> None:
+             data_type: Optional[torch.dtype] = None, sm_scale: Optional[float] = None, first_tokens: int = 0,
+             **_ignored) -> None:
+        """`first_tokens` (an extension, with `window_left` >= 0): tokens 0 .. first_tokens - 1 of every context stay
+        visible behind the window.  Pages between them and the window are not read: their entries in `indices` may
+        be stale."""
         _require_i32(indptr, "indptr")
         _require_i32(indices, "indices")
         _require_i32(last_page_len, "last_page_len")
@@ -553,6 +689,7 @@ class BatchDecodeWithPagedKVCacheWrapper:
             raise ValueError("logits_soft_cap is not supported")
         if window_left is None or window_left < -1:
             raise ValueError("window_left must be -1 (no window) or >= 0")
+        first_tokens = _check_first_tokens(first_tokens, window_left)
         if num_qo_heads % num_kv_heads != 0:
             raise ValueError(f"num_qo_heads {num_qo_heads} is not a multiple of num_kv_heads {num_kv_heads}")
         if kv_data_type is not None and kv_data_type != q_data_type:
@@ -574,11 +711,13 @@ class BatchDecodeWithPagedKVCacheWrapper:
                 fl[:batch].copy_(last_page_len[:batch], non_blocking=True)
             indptr, indices, last_page_len = fi, fx, fl
         need = lib.piekv_decode_workspace_bytes(batch, num_qo_heads, num_kv_heads, head_dim)
+        if first_tokens > 0:
+            need = lib.piekv_decode_first_tokens_workspace_bytes(batch, num_qo_heads, num_kv_heads, head_dim)
         if self.workspace_buffer.numel() < need:
             raise ValueError(f"workspace_buffer too small: {self.workspace_buffer.numel()} < {need} bytes")
         self._plan = dict(indptr=indptr, indices=indices, last_page_len=last_page_len, batch=batch,
                           hq=int(num_qo_heads), hkv=int(num_kv_heads), d=int(head_dim), page_size=int(page_size),
-                          dtype=q_data_type, window_left=int(window_left),
+                          dtype=q_data_type, window_left=int(window_left), first_tokens=first_tokens,
                           sm_scale=float(sm_scale) if sm_scale is not None else 1.0 / math.sqrt(head_dim))
 
     def run(self, q: torch.Tensor, paged_kv_cache: torch.Tensor, out: Optional[torch.Tensor] = None,
@@ -604,7 +743,7 @@ class BatchDecodeWithPagedKVCacheWrapper:
             raise ValueError("out must be a contiguous tensor shaped and typed like q")
         lse = torch.empty((pl["batch"], pl["hq"]), dtype=torch.float32, device=q.device) if return_lse else None
         ws = self.workspace_buffer
-        opt = _attn_options(pl["window_left"], sinks, pl["hq"])
+        opt = _attn_options(pl["window_left"], sinks, pl["hq"], pl["first_tokens"])
         check(lib.piekv_decode_run_opt(q.data_ptr(), qs[0], qs[1], paged_kv_cache.data_ptr(), out.data_ptr(),
                                        lse.data_ptr() if lse is not None else None, pl["indptr"].data_ptr(),
                                        pl["indices"].data_ptr(), pl["last_page_len"].data_ptr(), pl["batch"],
@@ -622,6 +761,8 @@ class BatchDecodeWithPagedKVCacheWrapper:
         if self._plan is None:
             raise RuntimeError("Must call plan() before run()")
         pl = self._plan
+        if pl["first_tokens"] > 0:
+            raise ValueError("first_tokens is not taken by the fused step; append the new tokens, then run()")
         for t, name in ((q, "q"), (k, "k"), (v, "v")):
             _require_cuda(t, name)
         _require_i32(pos_ids, "pos_ids")
@@ -711,6 +852,143 @@ class BatchDecodeWithPagedKVCacheWrapper:
         return peers.full(b)
 
 
+class BatchSharedPrefixDecodeWrapper:
+    """One query token per request for requests that share the leading pages of their contexts: beams and forks of one
+    context (`pages.KvPageList.fork`, `pages.DevicePageTable.fork`), or chats behind one system prompt.  The shared
+    pages are read once per group of requests instead of once per request; what every request has of its own follows,
+    and both parts of a softmax are joined in 32 bits.  The result is `BatchDecodeWithPagedKVCacheWrapper.run`'s
+    within rounding, for any grouping.
+
+    `plan()` takes the page table of the decode wrapper and `group_indptr` (int32 [groups + 1]: group g holds the
+    consecutive requests group_indptr[g] .. group_indptr[g + 1) - 1; None: the whole batch is one group).  How many
+    full pages the requests of a group share is found on the device by comparing their page lists; nothing is read
+    back.  The plan holds until the page table's contents change; `replan()` rebuilds it from the same tensors.  Both
+    only launch kernels on the current stream, so plan / replan and any number of run() calls (one per layer) can be
+    captured in a CUDA graph together.  The plan lives in a buffer of its own; the workspace may be shared with other
+    wrappers whose calls are ordered on the same stream."""
+
+    def __init__(self, float_workspace_buffer: torch.Tensor, kv_layout: str = "NHD") -> None:
+        if kv_layout != "NHD":
+            raise ValueError(f"kv_layout {kv_layout!r} is not supported (NHD only)")
+        _check_workspace(float_workspace_buffer)
+        self.workspace_buffer = float_workspace_buffer
+        self.kv_layout = kv_layout
+        float_workspace_buffer[:COUNTER_BYTES].zero_()
+        self._plan = None
+        self._args = None
+        self._buffers = []  # plan buffers; earlier ones stay alive, a captured graph may still use them
+
+    def plan(self, indptr: torch.Tensor, indices: torch.Tensor, last_page_len: torch.Tensor, num_qo_heads: int,
+             num_kv_heads: int, head_dim: int, page_size: int, group_indptr: Optional[torch.Tensor] = None,
+             pos_encoding_mode: str = "NONE", window_left: int = -1, logits_soft_cap: Optional[float] = None,
+             q_data_type: torch.dtype = torch.float16, kv_data_type: Optional[torch.dtype] = None,
+             sm_scale: Optional[float] = None) -> None:
+        _require_i32(indptr, "indptr")
+        _require_i32(indices, "indices")
+        _require_i32(last_page_len, "last_page_len")
+        if pos_encoding_mode != "NONE":
+            raise ValueError("pos_encoding_mode other than 'NONE' is not supported; apply RoPE before the append")
+        if logits_soft_cap not in (None, 0.0):
+            raise ValueError("logits_soft_cap is not supported")
+        if window_left != -1:
+            raise ValueError("a sliding window is not supported here; use BatchDecodeWithPagedKVCacheWrapper")
+        if num_qo_heads % num_kv_heads != 0:
+            raise ValueError(f"num_qo_heads {num_qo_heads} is not a multiple of num_kv_heads {num_kv_heads}")
+        if kv_data_type is not None and kv_data_type != q_data_type:
+            raise ValueError("kv_data_type must equal q_data_type")
+        batch = indptr.shape[0] - 1
+        if batch < 0:
+            raise ValueError("indptr must hold batch + 1 entries")
+        if last_page_len.shape[0] < batch:
+            raise ValueError("last_page_len shorter than the batch")
+        dev = indptr.device
+        if group_indptr is None:
+            group_indptr = torch.empty(2, dtype=torch.int32, device=dev)
+            group_indptr[:1].zero_()
+            group_indptr[1:].fill_(batch)
+        _require_i32(group_indptr, "group_indptr")
+        groups = group_indptr.shape[0] - 1
+        if groups < (1 if batch > 0 else 0):
+            raise ValueError("group_indptr must hold groups + 1 entries")
+        for t, name in ((indices, "indices"), (last_page_len, "last_page_len"), (group_indptr, "group_indptr"),
+                        (self.workspace_buffer, "workspace_buffer")):
+            if t.device != dev:
+                raise ValueError(f"{name} is on {t.device}, indptr on {dev}")
+        # as many pieces per prefix as the workspace has room for
+        base = lib.piekv_shared_prefix_workspace_bytes(batch, num_qo_heads, num_kv_heads, head_dim, 1)
+        each = lib.piekv_shared_prefix_workspace_bytes(batch, num_qo_heads, num_kv_heads, head_dim, 2) - base
+        have = self.workspace_buffer.numel()
+        if have < base:
+            raise ValueError(f"workspace_buffer too small: {have} < {base} bytes")
+        splits = min(_lib.SHARED_PREFIX_MAX_SPLITS, 1 + (have - base) // each if each > 0 else 1)
+        plan_bytes = lib.piekv_shared_prefix_plan_bytes(batch, groups, num_qo_heads, num_kv_heads)
+        if not self._buffers or self._buffers[-1].numel() < plan_bytes or self._buffers[-1].device != dev:
+            self._buffers.append(torch.empty(max(plan_bytes, 4096), dtype=torch.uint8, device=dev))
+        a = _lib.SharedPrefixArgs()
+        a.kv_indptr = indptr.data_ptr()
+        a.kv_indices = indices.data_ptr()
+        a.kv_last_page_len = last_page_len.data_ptr()
+        a.group_indptr = group_indptr.data_ptr()
+        a.plan = self._buffers[-1].data_ptr()
+        a.plan_bytes = self._buffers[-1].numel()
+        a.workspace = self.workspace_buffer.data_ptr()
+        a.workspace_bytes = have
+        a.err = _err_word(dev).data_ptr()
+        a.batch, a.num_groups = batch, groups
+        a.num_qo_heads, a.num_kv_heads = int(num_qo_heads), int(num_kv_heads)
+        a.head_dim, a.page_size = int(head_dim), int(page_size)
+        a.dtype = _dtype_code(q_data_type, "plan")
+        a.max_splits = splits
+        a.sm_scale = float(sm_scale) if sm_scale is not None else 1.0 / math.sqrt(head_dim)
+        self._args = a
+        self._plan = dict(shape=(batch, int(num_qo_heads), int(head_dim)), dtype=q_data_type, device=dev,
+                          cache=(int(page_size), int(num_kv_heads), int(head_dim)), sm_scale=a.sm_scale,
+                          keep=(indptr, indices, last_page_len, group_indptr))
+        self.replan()
+
+    def replan(self) -> None:
+        """Rebuild the plan from the tensors of the last plan() call, whose contents may have changed."""
+        if self._plan is None:
+            raise RuntimeError("Must call plan() before run()")
+        check(lib.piekv_shared_prefix_plan(C.byref(self._args), _stream(self._plan["device"])), "BatchSharedPrefixDecode.plan")
+
+    def run(self, q: torch.Tensor, paged_kv_cache: torch.Tensor, out: Optional[torch.Tensor] = None,
+            return_lse: bool = False, sinks: Optional[torch.Tensor] = None, sm_scale: Optional[float] = None):
+        """`sinks` (float32 [num_qo_heads]) and `sm_scale` as in the decode wrapper's run()."""
+        if self._plan is None:
+            raise RuntimeError("Must call plan() before run()")
+        pl = self._plan
+        _require_cuda(q, "q")
+        num_pages, page_size, hkv, d = _check_pool(paged_kv_cache)
+        qs = _rows(q, "q")
+        if tuple(q.shape) != pl["shape"]:
+            raise ValueError(f"q shape {tuple(q.shape)} differs from the plan {pl['shape']}")
+        if (page_size, hkv, d) != pl["cache"]:
+            raise ValueError("paged_kv_cache shape differs from the plan")
+        if q.dtype != pl["dtype"] or q.dtype != paged_kv_cache.dtype:
+            raise ValueError(f"q dtype {q.dtype}, cache dtype {paged_kv_cache.dtype}, planned {pl['dtype']}")
+        if q.device != pl["device"] or paged_kv_cache.device != pl["device"]:
+            raise ValueError(f"q is on {q.device}, the cache on {paged_kv_cache.device}, the plan on {pl['device']}")
+        if out is None:
+            out = torch.empty(pl["shape"], dtype=q.dtype, device=q.device)
+        elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous():
+            raise ValueError("out must be a contiguous tensor shaped and typed like q")
+        lse = torch.empty(pl["shape"][:2], dtype=torch.float32, device=q.device) if return_lse else None
+        a = _lib.SharedPrefixArgs.from_buffer_copy(self._args)  # host threads may run the same plan
+        a.q = q.data_ptr()
+        a.q_stride_n, a.q_stride_h = qs
+        a.pool = paged_kv_cache.data_ptr()
+        a.num_pages = num_pages
+        a.out = out.data_ptr()
+        a.lse = lse.data_ptr() if return_lse else None
+        a.sm_scale = float(sm_scale) if sm_scale is not None else pl["sm_scale"]
+        a.sinks = _sink_ptr(sinks, pl["shape"][1])
+        check(lib.piekv_shared_prefix_run(C.byref(a), _stream(q.device)), "BatchSharedPrefixDecode.run")
+        return (out, lse) if return_lse else out
+
+    forward = run
+
+
 class BatchPrefillWithPagedKVCacheWrapper:
     """Packed variable-length (prefill / chunked / multi-token) attention over paged K/V.
 
@@ -737,7 +1015,10 @@ class BatchPrefillWithPagedKVCacheWrapper:
              packed_custom_mask: Optional[torch.Tensor] = None, causal: bool = False,
              pos_encoding_mode: str = "NONE", window_left: int = -1, logits_soft_cap: Optional[float] = None,
              sm_scale: Optional[float] = None, q_data_type: torch.dtype = torch.float16,
-             kv_data_type: Optional[torch.dtype] = None, brle_mask=None, **_ignored) -> None:
+             kv_data_type: Optional[torch.dtype] = None, brle_mask=None, first_tokens: int = 0, **_ignored) -> None:
+        """`first_tokens` (an extension, with `window_left` >= 0 and without a mask): tokens 0 .. first_tokens - 1 of
+        every context stay visible behind the window.  Nothing is packed and nothing is read back for it; pages that
+        no query token of a tile sees are not read."""
         _require_i32(qo_indptr, "qo_indptr")
         _require_i32(paged_kv_indptr, "paged_kv_indptr")
         _require_i32(paged_kv_indices, "paged_kv_indices")
@@ -748,6 +1029,9 @@ class BatchPrefillWithPagedKVCacheWrapper:
             raise ValueError("logits_soft_cap is not supported")
         if window_left < -1:
             raise ValueError("window_left must be -1 (no window) or >= 0")
+        first_tokens = _check_first_tokens(first_tokens, window_left)
+        if first_tokens > 0 and (custom_mask is not None or brle_mask is not None):
+            raise ValueError("first_tokens cannot be combined with custom_mask or brle_mask")
         if packed_custom_mask is not None:
             raise ValueError("packed_custom_mask is not supported; pass the boolean custom_mask")
         if head_dim_vo is not None and head_dim_vo != head_dim_qk:
@@ -781,7 +1065,7 @@ class BatchPrefillWithPagedKVCacheWrapper:
             brle = (runs, run_indptr, int(mask_bits))
             causal = False
         window_entries = 0
-        if window_left >= 0 and custom_mask is None and brle is None:
+        if window_left >= 0 and custom_mask is None and brle is None and first_tokens == 0:
             # A window without a mask becomes a packed mask on the device (the query at position p sees keys
             # p - window_left .. p, or .. kv_len - 1 when not causal); kv tiles outside every window of a query
             # tile are then skipped through the mask summary.  Its size needs sum(qo_len * kv_len): one small
@@ -796,7 +1080,7 @@ class BatchPrefillWithPagedKVCacheWrapper:
                           hkv=int(num_kv_heads), d=int(head_dim_qk), page_size=int(page_size), mask=mask,
                           mask_bytes=int(mask.numel()) if mask is not None else (brle[2] if brle else window_entries),
                           brle=brle, causal=bool(causal), dtype=q_data_type, planned_for=None,
-                          window_left=int(window_left),
+                          window_left=int(window_left), first_tokens=first_tokens,
                           sm_scale=float(sm_scale) if sm_scale is not None else 1.0 / math.sqrt(head_dim_qk))
 
     def _device_plan(self, n: int, num_pages: int) -> None:
@@ -820,7 +1104,8 @@ class BatchPrefillWithPagedKVCacheWrapper:
         check(lib.piekv_prefill_plan_opt(pl["qo_indptr"].data_ptr(), pl["indptr"].data_ptr(),
                                          pl["last_page_len"].data_ptr(),
                                          pl["mask"].data_ptr() if pl["mask"] is not None else None, runs_ptr, rptr_ptr,
-                                         pl["mask_bytes"], 1 if pl["causal"] else 0, pl["window_left"], pl["batch"], n,
+                                         pl["mask_bytes"], 1 if pl["causal"] else 0,
+                                         pl["window_left"] if pl["first_tokens"] == 0 else -1, pl["batch"], n,
                                          pl["page_size"], num_pages, ws.data_ptr(), ws.numel(),
                                          _err_word(dev).data_ptr(), _stream(dev)), "BatchPrefill.plan")
         pl["planned_for"] = key
@@ -848,7 +1133,7 @@ class BatchPrefillWithPagedKVCacheWrapper:
         lse = torch.empty((n, pl["hq"]), dtype=torch.float32, device=q.device) if return_lse else None
         ws = self.workspace_buffer
         self._device_plan(n, num_pages)
-        opt = _attn_options(pl["window_left"], sinks, pl["hq"])
+        opt = _attn_options(pl["window_left"], sinks, pl["hq"], pl["first_tokens"])
         check(lib.piekv_prefill_run_opt(q.data_ptr(), qs[0], qs[1], paged_kv_cache.data_ptr(), out.data_ptr(),
                                         lse.data_ptr() if lse is not None else None, pl["qo_indptr"].data_ptr(),
                                         pl["indptr"].data_ptr(), pl["indices"].data_ptr(),
@@ -871,6 +1156,8 @@ class BatchPrefillWithPagedKVCacheWrapper:
         if self._plan is None:
             raise RuntimeError("Must call plan() before run()")
         pl = self._plan
+        if pl["first_tokens"] > 0:
+            raise ValueError("a plan with first_tokens holds no packed mask")
         if pl["page_size"] != 16:
             raise ValueError("the packed mask exists for page size 16 only")
         self._device_plan(int(num_query_tokens), int(num_pages))
