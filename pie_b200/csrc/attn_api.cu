@@ -1,6 +1,7 @@
 // C ABI of the attention entry points: argument checks and kernel selection.
 #include "attn.cuh"
 #include "common.cuh"
+#include "decode_span.cuh"
 #include "rope.cuh"
 
 namespace piekv {
@@ -56,7 +57,7 @@ extern "C" int64_t piekv_decode_first_tokens_workspace_bytes(int32_t batch, int3
                                                              int32_t num_kv_heads, int32_t head_dim) {
   (void)head_dim;
   if (batch < 0 || num_qo_heads <= 0 || num_kv_heads <= 0) return 0;
-  return kCounterBytes;
+  return kCounterBytes + decode_span_scratch_bytes(num_qo_heads, num_kv_heads);
 }
 
 static int apply_options(AttnArgs &a, const piekv_attn_options *opt, const char *who) {
@@ -101,7 +102,11 @@ extern "C" int piekv_decode_run_opt(const void *q, int64_t q_stride_n, int64_t q
   if (int rc = check_common(a, dtype, "decode_run")) return rc;
   if (int rc = apply_options(a, opt, "decode_run")) return rc;
   if (batch == 0) return 0;
-  if (a.first_tokens > 0) return launch_attn_generic(a, dtype, (cudaStream_t)stream);
+  if (a.first_tokens > 0) {
+    if (decode_span_supported(a, dtype))
+      return launch_decode_span(a, dtype, SpanPrefix{}, workspace, workspace_bytes, (cudaStream_t)stream);
+    return launch_attn_generic(a, dtype, (cudaStream_t)stream);
+  }
   if (decode_tma_supported(a, dtype)) return launch_decode_tma(a, dtype, workspace, workspace_bytes, (cudaStream_t)stream);
   return launch_attn_generic(a, dtype, (cudaStream_t)stream);
 }

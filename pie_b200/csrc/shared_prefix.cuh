@@ -31,6 +31,13 @@ struct PlanView {
   int64_t bytes;
 };
 
+// How many partial results the row `row` (request * heads_per_kv + head of the kv head) of a group has: one per
+// chunk, or two where its row block has at most 128 rows, whose other half then works on the rest of the chunk.
+__host__ __device__ inline int partials_of(const Group &g, int row, int heads_per_kv, int max_splits) {
+  const int left = g.members * heads_per_kv - row / kRowsPerItem * kRowsPerItem;
+  return left <= kRowsPerItem / 2 && max_splits >= 2 ? 2 * g.chunks : g.chunks;
+}
+
 __host__ __device__ inline PlanView plan_view(void *plan, int batch, int groups, int hq, int hkv) {
   PlanView v;
   const int64_t rows = (int64_t)batch * (hq / hkv);
