@@ -67,6 +67,33 @@ __device__ __forceinline__ bool wait_or_abort(uint64_t *bar, uint32_t parity, vo
   }
 }
 
+// ---- window with first tokens (kBand kernels): the query at position p sees keys [0, first) and
+// [p - window_left, limit], limit = p (causal) or the last key.  Nothing is packed: a row's 128 mask bits of a tile
+// follow from three numbers.
+__device__ __forceinline__ uint32_t ones_below(int n) { return n <= 0 ? 0u : (n >= 32 ? 0xffffffffu : (1u << n) - 1u); }
+// mask bits of keys t .. t + 31 for a row that sees [0, first), [low, limit]
+__device__ __forceinline__ uint32_t band_word(int t, int first, int low, int limit) {
+  return (ones_below(first - t) | ~ones_below(low - t)) & ones_below(limit + 1 - t);
+}
+__device__ __forceinline__ uint4 band_bits(int t, int first, int low, int limit) {
+  return make_uint4(band_word(t, first, low, limit), band_word(t + 32, first, low, limit),
+                    band_word(t + 64, first, low, limit), band_word(t + 96, first, low, limit));
+}
+// The kv tiles of a query tile: [0, front) and [low_tile, n_tiles); `low` is the lowest window start of its rows.
+struct Band {
+  int first, low, front, low_tile;
+};
+__device__ __forceinline__ Band band_of(const AttnArgs &a, int kv_len, int qo_len, int r0, int n_tiles) {
+  Band w;
+  w.first = min(a.first_tokens, kv_len);
+  w.low = max(0, kv_len - qo_len + r0 - a.window_left);
+  w.front = min((w.first + kBN - 1) / kBN, n_tiles);
+  w.low_tile = min(max(w.low / kBN, w.front), n_tiles);
+  return w;
+}
+// page `pi` of the request's list holds a key that some row of the query tile may see
+__device__ __forceinline__ bool band_page(const Band &w, int pi) { return pi * kPage < w.first || pi * kPage + kPage > w.low; }
+
 // Zero the rows of a staged V tile that belong to the request's last page but lie beyond its last
 // token (rows [first, end) of the 128-token tile; a row is 128 bytes in each 64-column half,
 // whatever the swizzle does inside it).  Their probabilities are zero, but 0 x NaN is NaN, and a
@@ -78,6 +105,34 @@ __device__ __forceinline__ void zero_v_rows(uint32_t v_tile_smem, int first, int
                  "r"(0)
                  : "memory");
   }
+}
+
+// The same for a band: keys of loaded pages between the first tokens and the window, and behind the context.
+// Tells whether tile j has any; with `zero` it clears them.
+__device__ __forceinline__ bool band_unseen_v_rows(const Band &w, int kv_len, int j, uint32_t v_tile_smem, int lane, bool zero) {
+  const int t0 = j * kBN;
+  bool any = false;
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+    int a, e;
+    if (i == 0) {  // rest of the page of the last first token
+      a = w.first;
+      e = min((w.first + kPage - 1) / kPage * kPage, w.low);
+    } else if (i == 1) {  // start of the window's first page
+      a = max(w.low / kPage * kPage, w.first);
+      e = w.low;
+    } else {
+      a = kv_len;
+      e = (kv_len + kPage - 1) / kPage * kPage;
+    }
+    a = max(a - t0, 0);
+    e = min(e - t0, kBN);
+    if (a < e) {
+      any = true;
+      if (zero) zero_v_rows(v_tile_smem, a, e, lane);
+    }
+  }
+  return any;
 }
 
 }  // namespace prefill

@@ -380,7 +380,8 @@ __global__ void prefill_plan_kernel(const int32_t *__restrict__ qo_indptr, const
   }
 }
 
-template <typename T>
+// kBand: window with first tokens instead of the causal bound or a packed mask
+template <typename T, bool kBand>
 __global__ void __launch_bounds__(kThreads, 1)
     prefill_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_kv,
                       const __grid_constant__ PrefillParams p) {
@@ -414,14 +415,20 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   const int kv_len = np > 0 ? (np - 1) * kPage + last_len : 0;
   const int rows = min(kBM, qo_len - r0);  // valid query rows of this tile
-  const bool has_mask = p.has_mask != 0;
+  const bool has_mask = !kBand && p.has_mask != 0;
   const int kv_hi = (a.causal && !has_mask) ? min(kv_len, kv_len - qo_len + r0 + kBM) : kv_len;
   const int n_tiles = kv_hi > 0 ? (kv_hi + kBN - 1) / kBN : 0;
   const int groups = (kv_len + kBN - 1) / kBN;  // 128-bit mask groups per query row
   // with a custom mask, kv tiles without a single allowed pair are skipped by every role
   const uint32_t *srow = has_mask ? p.summary + (size_t)(p.tile_base[b] + r0 / kBM) * p.sw : nullptr;
-  auto active = [&](int j) { return !has_mask || ((__ldg(srow + (j >> 5)) >> (j & 31)) & 1u) != 0; };
+  Band band{};
+  if (kBand) band = band_of(a, kv_len, qo_len, r0, n_tiles);
+  auto active = [&](int j) {
+    if (kBand) return j < band.front || j >= band.low_tile;
+    return !has_mask || ((__ldg(srow + (j >> 5)) >> (j & 31)) & 1u) != 0;
+  };
   int n_active = n_tiles;
+  if (kBand) n_active = band.front + n_tiles - band.low_tile;
   if (has_mask) {
     n_active = 0;
     for (int w = 0; w < (n_tiles + 31) / 32; ++w) n_active += __popc(__ldg(srow + w));
@@ -483,14 +490,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     // K and V have their own rings and cursors, so K runs ahead of V by the depth of its ring
     int k_armed = 0, v_armed = 0;  // K / V tiles issued so far
     int jk = 0, jv = 0;            // next kv tile index to consider for K / for V
+    int lands = 0;                 // uses of v_land
     if (lane == 0) {
       mbar_arrive_expect_tx(&q_full, kTileBytes);
       tma_load_4d(q_smem, &tmap_q, 0, q0 + r0, 0, h, &q_full);
     }
     auto page_of = [&](int j) {
       const int pi = j * 8 + lane;
-      int page = (lane < 8 && pi < np) ? __ldg(a.kv_indices + p0 + pi) : a.num_pages;
-      if (lane < 8 && pi < np && (page < 0 || page >= a.num_pages)) {
+      const bool wanted = lane < 8 && pi < np && (!kBand || band_page(band, pi));
+      int page = wanted ? __ldg(a.kv_indices + p0 + pi) : a.num_pages;
+      if (wanted && (page < 0 || page >= a.num_pages)) {
         report_error(a.err, PIEKV_ERR_PAGE_ID, KID_PREFILL, p0 + pi, page);
         page = a.num_pages;  // outside the tensor map: zero fill
       }
@@ -522,8 +531,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           while (!active(jv)) ++jv;
           const int page = page_of(jv);
           // The tile that holds a partly filled last page lands on a barrier of its own, has its stale
-          // rows zeroed, and only then is handed to the MMA warp (at most once per CTA).
-          const bool partial = (kv_len & (kPage - 1)) != 0 && jv == (kv_len - 1) / kBN;
+          // rows zeroed, and only then is handed to the MMA warp (at most once per CTA without a band).
+          const bool partial = kBand ? band_unseen_v_rows(band, kv_len, jv, 0u, lane, false)
+                                     : (kv_len & (kPage - 1)) != 0 && jv == (kv_len - 1) / kBN;
           uint64_t *land = partial ? &v_land : &v_full[vs];
           if (lane == 0) mbar_arrive_expect_tx(land, kTileBytes);
           __syncwarp();
@@ -533,13 +543,18 @@ __global__ void __launch_bounds__(kThreads, 1)
             tma_load_5d(vdst + kHalfBytes, &tmap_kv, 0, 0, 1, hk, page * 2 + 1, land);
           }
           if (partial) {
-            if (!wait_or_abort(&v_land, 0, abort_flag)) {
+            if (!wait_or_abort(&v_land, lands & 1, abort_flag)) {
               if (lane == 0 && !*abort_flag) report_error(a.err, PIEKV_ERR_WAIT_TIMEOUT, KID_PREFILL, blockIdx.x, 110);
               if (lane == 0) atomicExch(&sh_abort, 1);
               break;
             }
-            const int first = kv_len - jv * kBN;
-            zero_v_rows(v_smem0 + vs * kTileBytes, first, min(kBN, (first + kPage - 1) / kPage * kPage), lane);
+            ++lands;
+            if (kBand) {
+              band_unseen_v_rows(band, kv_len, jv, v_smem0 + vs * kTileBytes, lane, true);
+            } else {
+              const int first = kv_len - jv * kBN;
+              zero_v_rows(v_smem0 + vs * kTileBytes, first, min(kBN, (first + kPage - 1) / kPage * kPage), lane);
+            }
             fence_proxy_async_smem();  // generic-proxy stores before the tensor core's reads
             __syncwarp();
             if (lane == 0) mbar_arrive(&v_full[vs]);
@@ -628,6 +643,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const bool row_valid = row < rows;
     // last allowed token of this row (inclusive)
     const int limit = row_valid ? ((a.causal && !has_mask) ? min(kv_len - 1, kv_len - qo_len + r0 + row) : kv_len - 1) : -1;
+    const int low = max(0, kv_len - qo_len + r0 + row - a.window_left);  // kBand: the row's window
     const uint4 *mrow = has_mask ? p.packed + p.poff[b] + (long long)(r0 + (row_valid ? row : 0)) * groups : nullptr;
     const float c = a.sm_scale * 1.4426950408889634f;
     float m_ref = -INFINITY, l = 0.f;
@@ -647,6 +663,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!active(j)) continue;
       const int sb = it & 1;
       uint4 mw4 = make_uint4(0, 0, 0, 0);
+      if (kBand) mw4 = band_bits(j * kBN, band.first, low, limit);
       if (has_mask && row_valid) mw4 = __ldg(mrow + j);  // in flight while we wait for S
       ok = wait_or_abort(&s_full[sb], (it >> 1) & 1, abort_flag);
       if (!ok) break;
@@ -668,8 +685,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int t1 = j * kBN + (hh ^ 1) * 64;  // first token of the other half
       const uint32_t mown[2] = {hh ? mw4.z : mw4.x, hh ? mw4.w : mw4.y};
       const uint32_t moth[2] = {hh ? mw4.x : mw4.z, hh ? mw4.y : mw4.w};
-      const bool full_own = has_mask ? (mown[0] & mown[1]) == 0xffffffffu : t0 + 63 <= limit;
-      const bool full_oth = has_mask ? (moth[0] & moth[1]) == 0xffffffffu : t1 + 63 <= limit;
+      const bool full_own = kBand || has_mask ? (mown[0] & mown[1]) == 0xffffffffu : t0 + 63 <= limit;
+      const bool full_oth = kBand || has_mask ? (moth[0] & moth[1]) == 0xffffffffu : t1 + 63 <= limit;
       float mxa[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
       if (full_own) {
 #pragma unroll
@@ -677,7 +694,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       } else {
 #pragma unroll
         for (int i = 0; i < 64; ++i) {
-          const bool allow = has_mask ? ((mown[i >> 5] >> (i & 31)) & 1u) != 0 : t0 + i <= limit;
+          const bool allow = kBand || has_mask ? ((mown[i >> 5] >> (i & 31)) & 1u) != 0 : t0 + i <= limit;
           const float v = allow ? __uint_as_float(sreg[i]) : -INFINITY;
           sreg[i] = __float_as_uint(v);
           mxa[i & 3] = fmaxf(mxa[i & 3], v);
@@ -689,7 +706,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       } else {
 #pragma unroll
         for (int i = 0; i < 64; ++i) {
-          const bool allow = has_mask ? ((moth[i >> 5] >> (i & 31)) & 1u) != 0 : t1 + i <= limit;
+          const bool allow = kBand || has_mask ? ((moth[i >> 5] >> (i & 31)) & 1u) != 0 : t1 + i <= limit;
           mxa[i & 3] = fmaxf(mxa[i & 3], allow ? __uint_as_float(oth[i]) : -INFINITY);
         }
       }
@@ -863,15 +880,15 @@ int launch_prefill_export_mask(const AttnArgs &a, int64_t mask_bytes, void *work
   return 0;
 }
 
-template <typename T>
+template <typename T, bool kBand>
 static int launch_prefill_t(const AttnArgs &a, const CUtensorMap &tq, const CUtensorMap &tkv, const PrefillParams &p,
                             int max_tiles, cudaStream_t st) {
   static unsigned char configured[kMaxDevices] = {0};
-  if (int rc = opt_in_dynamic_smem(prefill_tc_kernel<T>, kSmemBytes, configured, "prefill: cudaFuncSetAttribute"))
+  if (int rc = opt_in_dynamic_smem(prefill_tc_kernel<T, kBand>, kSmemBytes, configured, "prefill: cudaFuncSetAttribute"))
     return rc;
   const long long blocks = (long long)max_tiles * a.hq;
   PIEKV_REQUIRE(blocks < (1ll << 31), "prefill: too many tiles");
-  prefill_tc_kernel<T><<<(unsigned)blocks, kThreads, kSmemBytes, st>>>(tq, tkv, p);
+  prefill_tc_kernel<T, kBand><<<(unsigned)blocks, kThreads, kSmemBytes, st>>>(tq, tkv, p);
   PIEKV_LAUNCH_CHECK("prefill_tc_kernel");
   return 0;
 }
@@ -901,8 +918,11 @@ int launch_prefill_tc(const AttnArgs &a, int dtype, int64_t mask_bytes, void *wo
   CUtensorMap tq, tkv;
   if (int rc = make_q_tensor_map(&tq, a.q, a.nnz, a.hq, a.q_sn, a.q_sh, dtype, kBM)) return rc;
   if (int rc = make_page_tensor_map(&tkv, a.pool, a.num_pages, a.hkv, dtype, 1, 1, 1)) return rc;
-  if (dtype == PIEKV_BF16) return launch_prefill_t<__nv_bfloat16>(a, tq, tkv, p, v.max_tiles, st);
-  return launch_prefill_t<__half>(a, tq, tkv, p, v.max_tiles, st);
+  if (a.first_tokens > 0)
+    return dtype == PIEKV_BF16 ? launch_prefill_t<__nv_bfloat16, true>(a, tq, tkv, p, v.max_tiles, st)
+                               : launch_prefill_t<__half, true>(a, tq, tkv, p, v.max_tiles, st);
+  if (dtype == PIEKV_BF16) return launch_prefill_t<__nv_bfloat16, false>(a, tq, tkv, p, v.max_tiles, st);
+  return launch_prefill_t<__half, false>(a, tq, tkv, p, v.max_tiles, st);
 }
 
 }  // namespace piekv

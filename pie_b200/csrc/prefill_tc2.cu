@@ -81,6 +81,7 @@ struct Item {
   int groups;        // 128-bit groups per row of the packed mask
   int srow;          // row of the (query tile, kv tile) summary
   int pad;
+  Band band;         // window with first tokens
   long long poff;    // the request's first 128-bit group in the packed mask
 };
 
@@ -123,7 +124,9 @@ __device__ __forceinline__ void issue_pv_half(uint32_t d_tmem, uint32_t p_tmem, 
     tc::mma_ts(d_tmem, p_tmem + ks * 8, v_desc + (uint64_t)((ks * 2048) >> 4), idesc, (accumulate_first || ks > 0) ? 1u : 0u);
 }
 
-template <typename T>
+// kBand: window with first tokens (a.window_left, a.first_tokens) instead of the causal bound or a packed mask; tiles
+// between the first tokens and the window are skipped by every role, mask bits are computed where a tile needs them.
+template <typename T, bool kBand>
 __global__ void __launch_bounds__(k2Threads, 1)
     prefill_tc2_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_kv,
                        const __grid_constant__ PrefillParams p) {
@@ -137,7 +140,7 @@ __global__ void __launch_bounds__(k2Threads, 1)
   const AttnArgs &a = p.a;
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  const bool has_mask = p.has_mask != 0;
+  const bool has_mask = !kBand && p.has_mask != 0;
   T *out = reinterpret_cast<T *>(a.out);
 
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -182,7 +185,8 @@ __global__ void __launch_bounds__(k2Threads, 1)
   constexpr bool kBf16 = !std::is_same<T, __half>::value;
 
   // kv tile j of the query tile whose summary row is `srow` has at least one allowed pair
-  auto tile_active = [&](const uint32_t *srow, int j) {
+  auto tile_active = [&](const uint32_t *srow, const Band &band, int j) {
+    if (kBand) return j < band.front || j >= band.low_tile;
     return !has_mask || ((__ldg(srow + (j >> 5)) >> (j & 31)) & 1u) != 0;
   };
   auto give_up = [&](int where) {
@@ -239,6 +243,10 @@ __global__ void __launch_bounds__(k2Threads, 1)
           it.poff = has_mask ? p.poff[it.b] : 0;
           it.pad = 0;
           it.n_active = it.n_tiles;
+          if (kBand) {
+            it.band = band_of(a, it.kv_len, it.qo_len, it.r0, it.n_tiles);
+            it.n_active = it.band.front + it.n_tiles - it.band.low_tile;
+          }
           if (has_mask) {
             const uint32_t *srow = p.summary + (size_t)it.srow * p.sw;
             int cnt = 0;
@@ -334,6 +342,8 @@ __global__ void __launch_bounds__(k2Threads, 1)
       const int valid = sh_item[slot].valid, left0 = sh_item[slot].n_active;
       const int p0 = sh_item[slot].p0, np = sh_item[slot].np, hk = sh_item[slot].hk, kv_len = sh_item[slot].kv_len;
       const uint32_t *srow = p.summary + (size_t)sh_item[slot].srow * p.sw;
+      Band band{};
+      if (kBand) band = sh_item[slot].band;
       __syncwarp();
       if (lane == 0) mbar_arrive(&item_empty[slot]);
       if (!valid) break;
@@ -345,16 +355,18 @@ __global__ void __launch_bounds__(k2Threads, 1)
           ok = false;
           break;
         }
-        while (!tile_active(srow, j)) ++j;
+        while (!tile_active(srow, band, j)) ++j;
         const int pi = j * 8 + lane;
-        int page = (lane < 8 && pi < np) ? __ldg(a.kv_indices + p0 + pi) : a.num_pages;
-        if (lane < 8 && pi < np && (page < 0 || page >= a.num_pages)) {
+        const bool wanted = lane < 8 && pi < np && (!kBand || band_page(band, pi));
+        int page = wanted ? __ldg(a.kv_indices + p0 + pi) : a.num_pages;
+        if (wanted && (page < 0 || page >= a.num_pages)) {
           report_error(a.err, PIEKV_ERR_PAGE_ID, KID_PREFILL, p0 + pi, page);
           page = a.num_pages;  // outside the tensor map: zero fill
         }  // pages beyond the request's list are out of range too: their rows are zero-filled
         // The V tile that holds a partly filled last page lands on a barrier of its own, has its stale
         // rows zeroed, and only then is handed to the MMA warp (at most once per item).
-        const bool partial = is_v && (kv_len & (kPage - 1)) != 0 && j == (kv_len - 1) / kBN;
+        const bool partial = is_v && (kBand ? band_unseen_v_rows(band, kv_len, j, 0u, lane, false)
+                                            : (kv_len & (kPage - 1)) != 0 && j == (kv_len - 1) / kBN);
         uint64_t *land = partial ? &v_land : &full[st];
         if (lane == 0) mbar_arrive_expect_tx(land, kTileBytes);
         __syncwarp();
@@ -371,8 +383,12 @@ __global__ void __launch_bounds__(k2Threads, 1)
             break;
           }
           ++lands;
-          const int first = kv_len - j * kBN;
-          zero_v_rows(ring0 + st * kTileBytes, first, min(kBN, (first + kPage - 1) / kPage * kPage), lane);
+          if (kBand) {
+            band_unseen_v_rows(band, kv_len, j, ring0 + st * kTileBytes, lane, true);
+          } else {
+            const int first = kv_len - j * kBN;
+            zero_v_rows(ring0 + st * kTileBytes, first, min(kBN, (first + kPage - 1) / kPage * kPage), lane);
+          }
           fence_proxy_async_smem();  // generic-proxy stores before the tensor core's reads
           __syncwarp();
           if (lane == 0) mbar_arrive(&full[st]);
@@ -541,6 +557,7 @@ __global__ void __launch_bounds__(k2Threads, 1)
         continue;
       }
       const int kv_len = it.kv_len;
+      const int low = max(0, kv_len - it.qo_len + it.r0 + row - a.window_left);  // kBand: the row's window
       const int limit =
           row_valid ? ((a.causal && !has_mask) ? min(kv_len - 1, kv_len - it.qo_len + it.r0 + row) : kv_len - 1) : -1;
       const uint32_t *srow = p.summary + (size_t)it.srow * p.sw;
@@ -550,15 +567,16 @@ __global__ void __launch_bounds__(k2Threads, 1)
       int done = 0;  // tiles of this item consumed
 
       for (int j = 0; j < n_tiles; ++j) {
-        if (!tile_active(srow, j)) continue;
+        if (!tile_active(srow, it.band, j)) continue;
         uint4 mw = make_uint4(0, 0, 0, 0);
+        if (kBand) mw = band_bits(j * kBN, it.band.first, low, limit);
         if (has_mask && row_valid) mw = __ldg(mrow + j);  // in flight while we wait for S
         ok = wait_or_abort(&s_full[x], sc & 1, abort_flag);
         if (!ok) break;
         ++sc;
         tc::fence_after_sync();
         const int t0 = j * kBN;
-        const bool full_tile = has_mask ? (mw.x & mw.y & mw.z & mw.w) == 0xffffffffu : t0 + kBN - 1 <= limit;
+        const bool full_tile = kBand || has_mask ? (mw.x & mw.y & mw.z & mw.w) == 0xffffffffu : t0 + kBN - 1 <= limit;
 
         // ---- pass 1: running maximum, 64 columns at a time (rolled: the unrolled body of a whole row is
         // ~10 KB of code per softmax warp, which evicts the MMA thread's code from the instruction cache)
@@ -573,7 +591,7 @@ __global__ void __launch_bounds__(k2Threads, 1)
             const uint32_t w0 = h ? mw.z : mw.x, w1 = h ? mw.w : mw.y;
 #pragma unroll
             for (int i = 0; i < 64; ++i) {
-              const bool allow = has_mask ? (((i < 32 ? w0 : w1) >> (i & 31)) & 1u) != 0 : t0 + h * 64 + i <= limit;
+              const bool allow = kBand || has_mask ? (((i < 32 ? w0 : w1) >> (i & 31)) & 1u) != 0 : t0 + h * 64 + i <= limit;
               sr[i] = allow ? sr[i] : 0xff800000u;
             }
           }
@@ -619,7 +637,7 @@ __global__ void __launch_bounds__(k2Threads, 1)
             const uint32_t w0 = h ? mw.z : mw.x, w1 = h ? mw.w : mw.y;
 #pragma unroll
             for (int i = 0; i < 64; ++i) {
-              const bool allow = has_mask ? (((i < 32 ? w0 : w1) >> (i & 31)) & 1u) != 0 : t0 + h * 64 + i <= limit;
+              const bool allow = kBand || has_mask ? (((i < 32 ? w0 : w1) >> (i & 31)) & 1u) != 0 : t0 + h * 64 + i <= limit;
               sr[i] = allow ? sr[i] : 0xff800000u;
             }
           }
@@ -682,11 +700,11 @@ __global__ void __launch_bounds__(k2Threads, 1)
   }
 }
 
-template <typename T>
+template <typename T, bool kBand>
 int launch_t(const AttnArgs &a, const CUtensorMap &tq, const CUtensorMap &tkv, const PrefillParams &p, int max_tiles,
              cudaStream_t st) {
   static unsigned char configured[kMaxDevices] = {0};
-  if (int rc = opt_in_dynamic_smem(prefill_tc2_kernel<T>, k2SmemBytes, configured,
+  if (int rc = opt_in_dynamic_smem(prefill_tc2_kernel<T, kBand>, k2SmemBytes, configured,
                                    "prefill (two heads): cudaFuncSetAttribute"))
     return rc;
   const long long items = (long long)max_tiles * (a.hq / 2);
@@ -694,7 +712,7 @@ int launch_t(const AttnArgs &a, const CUtensorMap &tq, const CUtensorMap &tkv, c
   const int sms = sm_count();
   PIEKV_REQUIRE(sms > 0, "prefill: cannot read the multiprocessor count");
   const unsigned grid = (unsigned)(items < sms ? items : sms);
-  prefill_tc2_kernel<T><<<grid, k2Threads, k2SmemBytes, st>>>(tq, tkv, p);
+  prefill_tc2_kernel<T, kBand><<<grid, k2Threads, k2SmemBytes, st>>>(tq, tkv, p);
   PIEKV_LAUNCH_CHECK("prefill_tc2_kernel");
   return 0;
 }
@@ -708,8 +726,11 @@ int launch_prefill_tc2(const AttnArgs &a, int dtype, const PrefillParams &p, int
   CUtensorMap tq, tkv;
   if (int rc = make_q_tensor_map(&tq, a.q, a.nnz, a.hq, a.q_sn, a.q_sh, dtype, kBM, 1)) return rc;
   if (int rc = make_page_tensor_map(&tkv, a.pool, a.num_pages, a.hkv, dtype, 1, 1, 1)) return rc;
-  if (dtype == PIEKV_BF16) return launch_t<__nv_bfloat16>(a, tq, tkv, p, max_tiles, st);
-  return launch_t<__half>(a, tq, tkv, p, max_tiles, st);
+  if (a.first_tokens > 0)
+    return dtype == PIEKV_BF16 ? launch_t<__nv_bfloat16, true>(a, tq, tkv, p, max_tiles, st)
+                               : launch_t<__half, true>(a, tq, tkv, p, max_tiles, st);
+  if (dtype == PIEKV_BF16) return launch_t<__nv_bfloat16, false>(a, tq, tkv, p, max_tiles, st);
+  return launch_t<__half, false>(a, tq, tkv, p, max_tiles, st);
 }
 
 }  // namespace piekv
