@@ -1,6 +1,8 @@
 // Decode attention for groups of requests that share the leading pages of their contexts.
 #include "attn.cuh"
 #include "common.cuh"
+#include "decode_span.cuh"
+#include "prefix_tc.cuh"
 #include "shared_prefix.cuh"
 
 namespace piekv {
@@ -188,11 +190,17 @@ extern "C" int64_t piekv_shared_prefix_plan_bytes(int32_t batch, int32_t num_gro
   return plan_view(nullptr, batch, num_groups, num_qo_heads, num_kv_heads).bytes;
 }
 
+// Partials of the prefix: max_splits per (request, query head).
+static int64_t prefix_ml_bytes(int batch, int hq, int max_splits) {
+  return ((int64_t)max_splits * batch * hq * 8 + 255) / 256 * 256;
+}
+
 extern "C" int64_t piekv_shared_prefix_workspace_bytes(int32_t batch, int32_t num_qo_heads, int32_t num_kv_heads,
                                                        int32_t head_dim, int32_t max_splits) {
-  (void)head_dim;
   if (batch < 0 || num_qo_heads <= 0 || num_kv_heads <= 0 || max_splits < 1) return 0;
-  return kCounterBytes;
+  if (head_dim != 128) return kCounterBytes;
+  return kCounterBytes + (decode_span_scratch_bytes(num_qo_heads, num_kv_heads) + 255) / 256 * 256 +
+         prefix_ml_bytes(batch, num_qo_heads, max_splits) + (int64_t)max_splits * batch * num_qo_heads * 128 * 4;
 }
 
 extern "C" int piekv_shared_prefix_plan(const piekv_shared_prefix_args *args, void *stream) {
@@ -234,5 +242,44 @@ extern "C" int piekv_shared_prefix_run(const piekv_shared_prefix_args *args, voi
   a.sm_scale = args->sm_scale;
   a.err = args->err;
   a.sinks = args->sinks;
-  return launch_attn_generic(a, args->dtype, (cudaStream_t)stream);
+  cudaStream_t st = (cudaStream_t)stream;
+  // a thread of the prefix kernel brings a query row in by 16-byte loads
+  const bool rows16 = (reinterpret_cast<uintptr_t>(a.q) & 15) == 0 && (a.q_sn & 7) == 0 && (a.q_sh & 7) == 0;
+  if (!decode_span_supported(a, args->dtype) || !rows16) return launch_attn_generic(a, args->dtype, st);
+  const int64_t need = piekv_shared_prefix_workspace_bytes(a.batch, a.hq, a.hkv, a.dim, args->max_splits);
+  PIEKV_REQUIRE(args->workspace != nullptr && args->workspace_bytes >= need,
+                "shared_prefix_run: workspace too small (%lld < %lld bytes)", (long long)args->workspace_bytes,
+                (long long)need);
+  PIEKV_REQUIRE((reinterpret_cast<uintptr_t>(args->workspace) & 255) == 0,
+                "shared_prefix_run: workspace must be 256-byte aligned");
+  const PlanView v = plan_view(args->plan, a.batch, args->num_groups, a.hq, a.hkv);
+  uint8_t *ws = reinterpret_cast<uint8_t *>(args->workspace) + kCounterBytes +
+                (decode_span_scratch_bytes(a.hq, a.hkv) + 255) / 256 * 256;
+  PrefixTcParams px{};
+  px.q = a.q;
+  px.q_sn = a.q_sn;
+  px.q_sh = a.q_sh;
+  px.kv_indptr = a.kv_indptr;
+  px.kv_indices = a.kv_indices;
+  px.n_items = v.header;
+  px.groups = v.groups;
+  px.items = v.items;
+  px.part_ml = reinterpret_cast<float2 *>(ws);
+  px.part_o = reinterpret_cast<float *>(ws + prefix_ml_bytes(a.batch, a.hq, args->max_splits));
+  px.batch = a.batch;
+  px.hq = a.hq;
+  px.group = a.hq / a.hkv;
+  px.num_pages = a.num_pages;
+  px.max_splits = args->max_splits;
+  px.scale_log2 = a.sm_scale * 1.4426950408889634f;
+  px.err = a.err;
+  if (int rc = launch_prefix_tc(px, a.pool, a.hkv, args->dtype, st)) return rc;
+  SpanPrefix sp;
+  sp.requests = v.requests;
+  sp.groups = v.groups;
+  sp.part_o = px.part_o;
+  sp.part_ml = px.part_ml;
+  sp.max_splits = args->max_splits;
+  sp.overlap = 1;
+  return launch_decode_span(a, args->dtype, sp, args->workspace, args->workspace_bytes, st);
 }
