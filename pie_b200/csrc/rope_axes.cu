@@ -29,22 +29,21 @@ struct AxesParams {
   piekv_rope_axes_table t;
 };
 
-// cos / sin of pair `pr` of token `tok`; false when the position is outside the table
-__device__ __forceinline__ bool pair_cos_sin(const AxesParams &p, int tok, int pr, float &c, float &s) {
-  const int pos = __ldg(p.pos + (int64_t)p.t.axis[pr] * p.pos_stride + tok);
+// cos / sin of pair `pr` (frequency `turn`) of token `tok` at position `pos`
+__device__ __forceinline__ void pair_cos_sin(const AxesParams &p, int tok, int pos, int pr, uint64_t turn, float &c, float &s) {
   if (p.t.cos_sin_table != nullptr) {
     if (pos < 0 || pos >= p.t.table_len) {
       report_error(p.err, PIEKV_ERR_TABLE_RANGE, KID_ROPE_AXES, tok, pos);
       c = 1.f;
       s = 0.f;
-      return false;
+      return;
     }
     const float *row = p.t.cos_sin_table + (size_t)pos * (2 * p.t.half);
     c = __ldg(row + pr);
     s = __ldg(row + p.t.half + pr);
-    return true;
+    return;
   }
-  const uint64_t t = (uint64_t)(int64_t)pos * p.t.turn[pr];
+  const uint64_t t = (uint64_t)(int64_t)pos * turn;
   const uint32_t quarter = (uint32_t)((t + (1ull << 61)) >> 62);
   const int32_t rest = (int32_t)(uint32_t)((t - ((uint64_t)quarter << 62)) >> 32);  // in [-2^29, 2^29): turns * 2^32
   float s0, c0;
@@ -54,7 +53,9 @@ __device__ __forceinline__ bool pair_cos_sin(const AxesParams &p, int tok, int p
   s = swap ? c0 : s0;
   if (quarter == 1 || quarter == 2) c = -c;
   if (quarter & 2) s = -s;
-  return true;
+}
+__device__ __forceinline__ void pair_cos_sin(const AxesParams &p, int tok, int pr, float &c, float &s) {
+  pair_cos_sin(p, tok, __ldg(p.pos + (int64_t)p.t.axis[pr] * p.pos_stride + tok), pr, p.t.turn[pr], c, s);
 }
 
 // The K row of a token in the pool (V half_page elements behind it); nullptr with the error recorded when the
@@ -135,8 +136,254 @@ __global__ void __launch_bounds__(256) rope_axes_kernel(const __grid_constant__ 
   }
 }
 
+// Whole head rows in 16-byte pieces.  A thread owns VEC pairs of one token (two pieces of a row: its halves, or
+// neighbours when pairs are interleaved), forms their cos and sin once and keeps them in registers while it walks the
+// heads blockIdx.y gives it, q before k before v: no (cos, sin) is formed twice, nothing goes through shared memory.
+// kUnits rows are loaded before the first is stored.
+constexpr int kUnits = 2;
+constexpr int kThreads = 256;
+constexpr int kThreadsPerSm = 1024;
+
+template <typename T, bool kNeighbours>
+__global__ void __launch_bounds__(kThreads, 3) rope_axes_rows_kernel(const __grid_constant__ AxesParams p, int heads_per_slice) {
+  constexpr int VEC = 16 / sizeof(T);
+  const int tok = blockIdx.x * blockDim.y + threadIdx.y;
+  if (tok >= p.nnz) return;
+  const int half = p.t.half;
+  const int ch = threadIdx.x;
+  const int e0 = kNeighbours ? 2 * ch * VEC : ch * VEC, e1 = kNeighbours ? e0 + VEC : e0 + half;
+  const int q_heads = p.q != nullptr ? p.hq : 0, k_end = q_heads + p.hkv, heads = k_end + (p.pool != nullptr ? p.hkv : 0);
+  const int h0 = blockIdx.y * heads_per_slice, h1 = min(heads, h0 + heads_per_slice);
+  const T *q = reinterpret_cast<const T *>(p.q) + (int64_t)tok * p.q_sn;
+  const T *k = reinterpret_cast<const T *>(p.k) + (int64_t)tok * p.k_sn;
+  const T *v = reinterpret_cast<const T *>(p.v) + (int64_t)tok * p.v_sn;
+  float c[VEC], s[VEC];
+  T *krow = nullptr;
+  bool ready = false;
+  for (int h = h0; h < h1; h += kUnits) {
+    uint4 lo[kUnits], hi[kUnits];
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) {
+      const int hh = h + u;
+      if (hh < h1) {
+        const T *src = hh < q_heads ? q + (int64_t)hh * p.q_sh
+                                    : (hh < k_end ? k + (int64_t)(hh - q_heads) * p.k_sh : v + (int64_t)(hh - k_end) * p.v_sh);
+        lo[u] = *reinterpret_cast<const uint4 *>(src + e0);
+        hi[u] = *reinterpret_cast<const uint4 *>(src + e1);
+      }
+    }
+    if (!ready) {  // while the first rows are on their way
+      if (h0 < k_end) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) pair_cos_sin(p, tok, ch * VEC + j, c[j], s[j]);
+      }
+      if (p.pool != nullptr && h1 > q_heads) krow = pool_row<T>(p, tok);
+      ready = true;
+    }
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) {
+      const int hh = h + u;
+      if (hh >= h1) break;
+      if (hh < k_end) {
+        T *a = reinterpret_cast<T *>(&lo[u]), *b = reinterpret_cast<T *>(&hi[u]);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          // pair j: (a[j], b[j]) of the row's halves, or neighbours 2j, 2j + 1 of the two pieces in order
+          T &x = kNeighbours ? (2 * j < VEC ? a[2 * j] : b[2 * j - VEC]) : a[j];
+          T &y = kNeighbours ? (2 * j < VEC ? a[2 * j + 1] : b[2 * j + 1 - VEC]) : b[j];
+          float xo, yo;
+          rope_rotate(Elem<T>::to_f32(x), Elem<T>::to_f32(y), c[j], s[j], xo, yo);
+          x = Elem<T>::from_f32(xo);
+          y = Elem<T>::from_f32(yo);
+        }
+      }
+      T *d0 = nullptr, *d1 = nullptr;
+      if (hh < q_heads) {
+        d0 = reinterpret_cast<T *>(p.q_out) + (int64_t)tok * p.qo_sn + (int64_t)hh * p.qo_sh;
+      } else if (hh < k_end) {
+        const int hk = hh - q_heads;
+        if (krow != nullptr) d0 = krow + (size_t)hk * p.dim;
+        if (p.k_out != nullptr) d1 = reinterpret_cast<T *>(p.k_out) + (int64_t)tok * p.ko_sn + (int64_t)hk * p.ko_sh;
+      } else if (krow != nullptr) {
+        d0 = krow + ((size_t)p.page_size * p.hkv + (size_t)(hh - k_end)) * p.dim;
+      }
+      if (d0 != nullptr) {
+        *reinterpret_cast<uint4 *>(d0 + e0) = lo[u];
+        *reinterpret_cast<uint4 *>(d0 + e1) = hi[u];
+      }
+      if (d1 != nullptr) {
+        *reinterpret_cast<uint4 *>(d1 + e0) = lo[u];
+        *reinterpret_cast<uint4 *>(d1 + e1) = hi[u];
+      }
+    }
+  }
+}
+
+// The same for rows whose heads lie next to each other (a token's q, k and v rows are one run of bytes each), laid out
+// for bandwidth: rows move by bulk copies, global to shared memory and back, a ring of stages per block, and only the
+// rotation itself passes through registers - in place in the stage; v never does.  A block's positions and page rows
+// are looked up 128 tokens at a time, (cos, sin) of the next token are formed while the copies of this one fly.
+// Measured (20480 tokens, 32 q / 8 kv heads, bf16, 504 MB): see kBulkBlocks.
+constexpr int kBulkThreads = 128;
+constexpr int kBulkChunk = 128;
+constexpr int kMaxStages = 4;
+constexpr int kBulkBlocks = 4;       // per SM
+constexpr int kBulkSmem = 50 * 1024;  // per block: four blocks per SM
+
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint64_t *bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+__device__ __forceinline__ void bulk_store(void *dst, uint32_t src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(src), "r"(bytes) : "memory");
+}
+
+template <typename T, bool kNeighbours>
+__global__ void __launch_bounds__(kBulkThreads) rope_axes_bulk_kernel(const __grid_constant__ AxesParams p, int stages,
+                                                                      int stage_bytes) {
+  constexpr int VEC = 16 / sizeof(T);
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ __align__(8) uint64_t full[kMaxStages];
+  __shared__ __align__(16) float sh_c[2][kMaxHalfDim], sh_s[2][kMaxHalfDim];
+  __shared__ int sh_pos[PIEKV_MAX_ROPE_AXES][kBulkChunk];
+  __shared__ T *sh_row[kBulkChunk];
+  const int tid = threadIdx.y * blockDim.x + threadIdx.x, threads = blockDim.x * blockDim.y;
+  const int half = p.t.half;
+  const uint32_t q_bytes = p.q != nullptr ? (uint32_t)(p.hq * p.dim * sizeof(T)) : 0u;
+  const uint32_t k_bytes = (uint32_t)(p.hkv * p.dim * sizeof(T));
+  const uint32_t v_bytes = p.pool != nullptr ? k_bytes : 0u;
+  const int heads = (p.q != nullptr ? p.hq : 0) + p.hkv;  // rows to rotate, q then k
+  const int count = (p.nnz - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x;  // tokens of this block
+  auto token = [&](int i) { return (int)blockIdx.x + i * (int)gridDim.x; };
+  auto load = [&](int i) {  // thread 0
+    const int s = i % stages;
+    const int64_t tok = token(i);
+    const uint32_t dst = smem_u32(smem) + (uint32_t)(s * stage_bytes);
+    mbar_arrive_expect_tx(&full[s], q_bytes + k_bytes + v_bytes);
+    if (q_bytes) bulk_load(dst, reinterpret_cast<const T *>(p.q) + tok * p.q_sn, q_bytes, &full[s]);
+    bulk_load(dst + q_bytes, reinterpret_cast<const T *>(p.k) + tok * p.k_sn, k_bytes, &full[s]);
+    if (v_bytes) bulk_load(dst + q_bytes + k_bytes, reinterpret_cast<const T *>(p.v) + tok * p.v_sn, v_bytes, &full[s]);
+  };
+  if (tid == 0) {
+    for (int s = 0; s < stages; ++s) mbar_init(&full[s], 1);
+    mbar_fence_init();
+    for (int i = 0; i < stages && i < count; ++i) load(i);
+  }
+  // this thread's pair when (cos, sin) are formed
+  const uint64_t turn = tid < half ? p.t.turn[tid] : 0;
+  const int axis = tid < half ? p.t.axis[tid] : 0;
+  auto form = [&](int i) {
+    if (tid < half)
+      pair_cos_sin(p, token(i), sh_pos[axis][i % kBulkChunk], tid, turn, sh_c[i & 1][tid], sh_s[i & 1][tid]);
+  };
+  const int ch = threadIdx.x;
+  const int e0 = kNeighbours ? 2 * ch * VEC : ch * VEC, e1 = kNeighbours ? e0 + VEC : e0 + half;
+  bool ok = true;
+  for (int i = 0; i < count; ++i) {
+    if (i % kBulkChunk == 0) {
+      __syncthreads();  // nobody still reads the last chunk's (and, the first time, the barriers are ready)
+      for (int j = tid; j < kBulkChunk && i + j < count; j += threads) {
+        const int tok = token(i + j);
+        for (int a = 0; a < p.t.num_axes; ++a) sh_pos[a][j] = __ldg(p.pos + (int64_t)a * p.pos_stride + tok);
+        sh_row[j] = p.pool != nullptr ? pool_row<T>(p, tok) : nullptr;
+      }
+      __syncthreads();
+      form(i);
+      __syncthreads();
+    }
+    const int s = i % stages;
+    uint8_t *stage = smem + s * stage_bytes;
+    if (ok) ok = mbar_wait(&full[s], (i / stages) & 1);
+    float c[VEC], sn[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; j += 4) {
+      *reinterpret_cast<float4 *>(c + j) = *reinterpret_cast<const float4 *>(&sh_c[i & 1][ch * VEC + j]);
+      *reinterpret_cast<float4 *>(sn + j) = *reinterpret_cast<const float4 *>(&sh_s[i & 1][ch * VEC + j]);
+    }
+    for (int h = threadIdx.y; h < heads; h += blockDim.y) {
+      T *row = reinterpret_cast<T *>(stage) + h * p.dim;
+      uint4 lo = *reinterpret_cast<const uint4 *>(row + e0), hi = *reinterpret_cast<const uint4 *>(row + e1);
+      T *a = reinterpret_cast<T *>(&lo), *b = reinterpret_cast<T *>(&hi);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        T &x = kNeighbours ? (2 * j < VEC ? a[2 * j] : b[2 * j - VEC]) : a[j];
+        T &y = kNeighbours ? (2 * j < VEC ? a[2 * j + 1] : b[2 * j + 1 - VEC]) : b[j];
+        float xo, yo;
+        rope_rotate(Elem<T>::to_f32(x), Elem<T>::to_f32(y), c[j], sn[j], xo, yo);
+        x = Elem<T>::from_f32(xo);
+        y = Elem<T>::from_f32(yo);
+      }
+      *reinterpret_cast<uint4 *>(row + e0) = lo;
+      *reinterpret_cast<uint4 *>(row + e1) = hi;
+    }
+    if (i + 1 < count && (i + 1) % kBulkChunk != 0) form(i + 1);
+    fence_proxy_async_smem();  // the rotated rows before the bulk stores that read them
+    __syncthreads();
+    if (tid == 0) {
+      const int64_t tok = token(i);
+      const uint32_t src = smem_u32(stage);
+      if (ok) {
+        if (q_bytes) bulk_store(reinterpret_cast<T *>(p.q_out) + tok * p.qo_sn, src, q_bytes);
+        if (p.k_out != nullptr) bulk_store(reinterpret_cast<T *>(p.k_out) + tok * p.ko_sn, src + q_bytes, k_bytes);
+        T *krow = sh_row[i % kBulkChunk];
+        if (krow != nullptr) {
+          bulk_store(krow, src + q_bytes, k_bytes);
+          bulk_store(krow + (size_t)p.page_size * p.hkv * p.dim, src + q_bytes + k_bytes, v_bytes);
+        }
+      } else {
+        report_error(p.err, PIEKV_ERR_WAIT_TIMEOUT, KID_ROPE_AXES, blockIdx.x, i);
+      }
+      asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+      // the stage of the token before is free once its stores have read it
+      if (i >= 1 && i - 1 + stages < count) {
+        asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+        load(i - 1 + stages);
+      }
+    }
+  }
+  if (tid == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // shared memory outlives the copies
+}
+
 template <typename T>
 int launch_axes(const AxesParams &p, cudaStream_t st) {
+  constexpr int VEC = 16 / sizeof(T);
+  auto rows16 = [](const void *ptr, int64_t sn, int64_t sh) {
+    return (reinterpret_cast<uintptr_t>(ptr) & 15) == 0 && sn % VEC == 0 && sh % VEC == 0;  // (null counts as aligned)
+  };
+  const int pieces = p.t.half / VEC;
+  if (2 * p.t.half == p.dim && p.t.half % VEC == 0 && rows16(p.q, p.q_sn, p.q_sh) && rows16(p.q_out, p.qo_sn, p.qo_sh) &&
+      rows16(p.k, p.k_sn, p.k_sh) && rows16(p.k_out, p.ko_sn, p.ko_sh) && rows16(p.v, p.v_sn, p.v_sh) && rows16(p.pool, 0, 0)) {
+    const int heads = (p.q != nullptr ? p.hq : 0) + p.hkv + (p.pool != nullptr ? p.hkv : 0);
+    // rows that are one run of bytes, and enough tokens that a block works on several: bulk copies
+    const bool runs = (p.q == nullptr || (p.q_sh == p.dim && p.qo_sh == p.dim)) && p.k_sh == p.dim &&
+                      (p.k_out == nullptr || p.ko_sh == p.dim) && (p.pool == nullptr || p.v_sh == p.dim);
+    const int stage_bytes = (heads * p.dim * (int)sizeof(T) + 127) / 128 * 128;
+    const int stages = kBulkSmem / stage_bytes < kMaxStages ? kBulkSmem / stage_bytes : kMaxStages;
+    const int blocks = kBulkBlocks * sm_count();
+    const dim3 bulk_block(pieces, kBulkThreads / pieces);
+    if (runs && stages >= 2 && p.nnz >= 2 * blocks && (int)(bulk_block.x * bulk_block.y) >= p.t.half) {
+      static unsigned char configured[2][kMaxDevices] = {{0}};
+      auto kernel = p.t.interleave ? rope_axes_bulk_kernel<T, true> : rope_axes_bulk_kernel<T, false>;
+      if (int rc = opt_in_dynamic_smem(kernel, kBulkSmem, configured[p.t.interleave ? 1 : 0], "rope_axes: cudaFuncSetAttribute"))
+        return rc;
+      kernel<<<blocks, bulk_block, stages * stage_bytes, st>>>(p, stages, stage_bytes);
+      PIEKV_LAUNCH_CHECK("rope_axes_bulk_kernel");
+      return 0;
+    }
+    // a token's heads are divided among threads until every SM has kThreadsPerSm of them
+    const long long want = (long long)kThreadsPerSm * sm_count(), have = (long long)p.nnz * pieces;
+    const long long slices = have >= want ? 1 : (want + have - 1) / have;
+    const int per = slices >= heads ? 1 : (int)((heads + slices - 1) / slices);
+    const dim3 block(pieces, kThreads / pieces);
+    const dim3 grid((p.nnz + block.y - 1) / block.y, (heads + per - 1) / per);
+    if (p.t.interleave)
+      rope_axes_rows_kernel<T, true><<<grid, block, 0, st>>>(p, per);
+    else
+      rope_axes_rows_kernel<T, false><<<grid, block, 0, st>>>(p, per);
+    PIEKV_LAUNCH_CHECK("rope_axes_rows_kernel");
+    return 0;
+  }
   rope_axes_kernel<T><<<p.nnz, 256, 0, st>>>(p);
   PIEKV_LAUNCH_CHECK("rope_axes_kernel");
   return 0;
@@ -159,10 +406,6 @@ extern "C" int piekv_rope_axes_prepare(const piekv_rope_params *rope, const int3
     half += sections[i];
   }
   PIEKV_REQUIRE(half > 0 && half <= kMaxHalfDim, "%s: sections of %d pairs (1..%d)", who, half, kMaxHalfDim);
-  if (cyclic)
-    for (int i = 1; i < num_axes; ++i)
-      PIEKV_REQUIRE(sections[i] == 0 || i + num_axes * (sections[i] - 1) < half,
-                    "%s: %d pairs of axis %d dealt out in turn do not fit %d pairs", who, sections[i], i, half);
   PIEKV_REQUIRE(rope->mode == PIEKV_ROPE_PLAIN || rope->mode == PIEKV_ROPE_LLAMA31 || rope->mode == PIEKV_ROPE_TABLE,
                 "%s: rope mode %d (plain, llama31 or table)", who, rope->mode);
   if (int rc = check_rope(rope, 2 * half, who)) return rc;
@@ -174,7 +417,7 @@ extern "C" int piekv_rope_axes_prepare(const piekv_rope_params *rope, const int3
   for (int ax = 0; ax < num_axes; ++ax) {
     if (cyclic) {
       if (ax == 0) continue;  // axis 0 has what the others leave
-      for (int n = 0; n < sections[ax]; ++n) table->axis[ax + n * num_axes] = (uint8_t)ax;
+      for (int i = ax; i < half && i < num_axes * sections[ax]; i += num_axes) table->axis[i] = (uint8_t)ax;
     } else {
       for (int n = 0; n < sections[ax]; ++n) table->axis[first + n] = (uint8_t)ax;
       first += sections[ax];

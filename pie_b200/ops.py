@@ -94,6 +94,15 @@ def _stream(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+def _stream_of(index: int) -> int:
+    """`_stream` for a device ordinal, without a Stream object (a third of a short call's host time)."""
+    cur = torch.cuda.current_device()
+    if index != cur:
+        raise ValueError(f"tensors live on cuda:{index} but the current CUDA device is cuda:{cur}; "
+                         f"call torch.cuda.set_device({index}) (or use `with torch.cuda.device({index})`) first")
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
 def _rows(t: torch.Tensor, name: str) -> Tuple[int, int]:
     """(token stride, head stride) in elements of a [n, H, D] tensor whose last axis is contiguous."""
     if t.dim() != 3:
@@ -463,15 +472,17 @@ class AxisRopeConfig(RopeConfig):
     sections: Tuple[int, ...] = ()
     cyclic: bool = False
 
+    def __setattr__(self, name, value) -> None:
+        self.__dict__["_table"] = None  # laid out again at the next use
+        object.__setattr__(self, name, value)
+
     def prepared(self) -> "_lib.RopeAxesTable":
         """The host table the kernels take, laid out once per set of parameters."""
-        t = self.cos_sin_table if self.mode == "table" else None
-        key = (self.mode, self.theta, self.scale, self.low_freq_factor, self.high_freq_factor, self.old_context_len,
-               self.interleave, tuple(self.sections), self.cyclic,
-               None if t is None else (t.data_ptr(), tuple(t.shape), t.dtype, t.device, t.is_contiguous()))
-        have = self.__dict__.get("_prepared")
-        if have is not None and have[0] == key:
-            return have[1]
+        table = self.__dict__["_table"]
+        if table is not None:
+            if self.mode == "table":
+                table.cos_sin_table = self.cos_sin_table.data_ptr()
+            return table
         sections = [int(x) for x in self.sections]
         if not 1 <= len(sections) <= _lib.MAX_ROPE_AXES:
             raise ValueError(f"sections must name 1 to {_lib.MAX_ROPE_AXES} axes, got {len(sections)}")
@@ -481,8 +492,26 @@ class AxisRopeConfig(RopeConfig):
         table = _lib.RopeAxesTable()
         check(lib.piekv_rope_axes_prepare(C.byref(rp), (C.c_int32 * len(sections))(*sections), len(sections),
                                           1 if self.cyclic else 0, C.byref(table)), "AxisRopeConfig")
-        self.__dict__["_prepared"] = (key, table)
+        self.__dict__["_table"] = table
         return table
+
+
+def _device_rows(t: torch.Tensor, name: str, device: int) -> Tuple[int, int]:
+    """_rows() of a tensor that has to be on CUDA device `device` (-1 for a tensor elsewhere)."""
+    if t.get_device() != device or not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor on cuda:{device}, got {t.device}")
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 3:
+        raise ValueError(f"{name} must be [tokens, heads, head_dim], got shape {tuple(shape)}")
+    if shape[2] > 1 and stride[2] != 1:
+        raise ValueError(f"{name}: head_dim axis must be contiguous")
+    return stride[0], stride[1]
+
+
+def _device_i32(t: torch.Tensor, name: str, device: int) -> int:
+    if t.dtype != torch.int32 or t.get_device() != device or not t.is_cuda or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 CUDA tensor on cuda:{device}, got {t.dtype} on {t.device}")
+    return t.data_ptr()
 
 
 def _rope_axes(q, k, v, pos_ids, rope: AxisRopeConfig, q_out, k_out, who: str, append=None) -> None:
@@ -491,58 +520,62 @@ def _rope_axes(q, k, v, pos_ids, rope: AxisRopeConfig, q_out, k_out, who: str, a
     _require_cuda(k, "k")
     _require_cuda(pos_ids, "pos_ids")
     table = rope.prepared()
-    n, hkv, d = k.shape if k.dim() == 3 else (0, 0, 0)
-    a = _lib.RopeAxesArgs()
-    a.k_stride_n, a.k_stride_h = _rows(k, "k")
-    a.k = k.data_ptr()
+    device = k.get_device()
+    k_rows = _device_rows(k, "k", device)
+    n, hkv, d = shape = k.shape
+    dtype = k.dtype
     if pos_ids.dtype != torch.int32 or pos_ids.dim() != 2 or pos_ids.shape[0] != table.num_axes or \
             pos_ids.shape[1] < n or (n > 1 and pos_ids.stride(1) != 1):
         raise ValueError(f"{who}: pos_ids must be int32 [{table.num_axes} axes, {n} tokens] with contiguous rows, got "
                          f"{tuple(pos_ids.shape)} {pos_ids.dtype}")
-    a.pos, a.pos_stride = pos_ids.data_ptr(), pos_ids.stride(0)
+    if pos_ids.get_device() != device:
+        raise ValueError(f"{who}: pos_ids is on {pos_ids.device}, k on {k.device}")
     if 2 * table.half > d:
         raise ValueError(f"{who}: sections of {table.half} pairs do not fit head_dim {d}")
-    same = [k, pos_ids]
+    if rope.mode == "table" and rope.cos_sin_table.get_device() != device:
+        raise ValueError(f"{who}: cos_sin_table on {rope.cos_sin_table.device}, k on {k.device}")
+    q_ptr = qo_ptr = ko_ptr = None
+    q_rows = qo_rows = ko_rows = v_rows = (0, 0)
+    hq = 0
     if q is not None:
         _require_cuda(q, "q")
-        a.q_stride_n, a.q_stride_h = _rows(q, "q")
-        if q.shape[0] != n or q.shape[2] != d or q.dtype != k.dtype:
-            raise ValueError(f"{who}: q {tuple(q.shape)} {q.dtype} does not match k {tuple(k.shape)} {k.dtype}")
-        if q_out.shape != q.shape or q_out.dtype != q.dtype:
-            raise ValueError(f"{who}: q_out must be shaped and typed like q")
-        a.q_out_stride_n, a.q_out_stride_h = _rows(q_out, "q_out")
-        a.q, a.q_out, a.num_qo_heads = q.data_ptr(), q_out.data_ptr(), q.shape[1]
-        same += [q, q_out]
+        q_rows = _device_rows(q, "q", device)
+        if q.shape[0] != n or q.shape[2] != d or q.dtype != dtype:
+            raise ValueError(f"{who}: q {tuple(q.shape)} {q.dtype} does not match k {tuple(shape)} {dtype}")
+        hq, q_ptr = q.shape[1], q.data_ptr()
+        if q_out is q:
+            qo_rows, qo_ptr = q_rows, q_ptr
+        else:
+            if q_out.shape != q.shape or q_out.dtype != dtype:
+                raise ValueError(f"{who}: q_out must be shaped and typed like q")
+            qo_rows, qo_ptr = _device_rows(q_out, "q_out", device), q_out.data_ptr()
     if k_out is not None:
-        a.k_out, (a.k_out_stride_n, a.k_out_stride_h) = k_out.data_ptr(), _rows(k_out, "k_out")
+        ko_rows, ko_ptr = _device_rows(k_out, "k_out", device), k_out.data_ptr()
+    tail = (None, None, None, None, None)
+    v_ptr, batch, page_size, num_pages = None, 0, 0, 0
     if append is not None:
         batch_indices, positions, pool, kv_indices, kv_indptr = append
         _require_cuda(v, "v")
-        a.v_stride_n, a.v_stride_h = _rows(v, "v")
+        v_rows, v_ptr = _device_rows(v, "v", device), v.data_ptr()
         num_pages, page_size, pool_heads, pool_dim = _check_pool(pool)
-        if (hkv, d) != (pool_heads, pool_dim) or v.shape != k.shape:
-            raise ValueError(f"{who}: key {tuple(k.shape)} / value {tuple(v.shape)} do not match the cache "
+        if hkv != pool_heads or d != pool_dim or v.shape != shape:
+            raise ValueError(f"{who}: key {tuple(shape)} / value {tuple(v.shape)} do not match the cache "
                              f"[*, {pool_heads}, {pool_dim}]")
-        if k.dtype != pool.dtype or v.dtype != pool.dtype:
-            raise ValueError(f"{who}: key/value dtype {k.dtype}/{v.dtype} differs from the cache dtype {pool.dtype}")
-        for t, name in ((batch_indices, "batch_indices"), (positions, "positions"), (kv_indices, "kv_indices"),
-                        (kv_indptr, "kv_indptr")):
-            _require_i32(t, name)
+        if dtype != pool.dtype or v.dtype != dtype:
+            raise ValueError(f"{who}: key/value dtype {dtype}/{v.dtype} differs from the cache dtype {pool.dtype}")
+        if pool.get_device() != device:
+            raise ValueError(f"{who}: the cache is on {pool.device}, k on {k.device}")
+        tail = (_device_i32(batch_indices, "batch_indices", device), _device_i32(positions, "positions", device),
+                pool.data_ptr(), _device_i32(kv_indices, "kv_indices", device), _device_i32(kv_indptr, "kv_indptr", device))
         if batch_indices.shape[0] < n or positions.shape[0] < n:
             raise ValueError(f"{who}: batch_indices / positions shorter than the number of tokens")
-        a.v, a.pool = v.data_ptr(), pool.data_ptr()
-        a.batch_indices, a.positions = batch_indices.data_ptr(), positions.data_ptr()
-        a.kv_indices, a.kv_indptr, a.batch = kv_indices.data_ptr(), kv_indptr.data_ptr(), kv_indptr.shape[0] - 1
-        a.num_pages, a.page_size = num_pages, page_size
-        same += [v, pool, batch_indices, positions, kv_indices, kv_indptr]
-    for t in same:
-        if t.device != k.device:
-            raise ValueError(f"{who}: tensors on {t.device} and {k.device}")
-    if rope.mode == "table" and rope.cos_sin_table.device != k.device:
-        raise ValueError(f"{who}: cos_sin_table on {rope.cos_sin_table.device}, k on {k.device}")
-    a.nnz, a.num_kv_heads, a.head_dim, a.dtype = n, hkv, d, _dtype_code(k.dtype, who)
-    a.err = _err_word(k.device).data_ptr()
-    check(lib.piekv_rope_axes(C.byref(a), C.byref(table), _stream(k.device)), who)
+        batch = kv_indptr.shape[0] - 1
+    args = _lib.RopeAxesArgs(q_ptr, k.data_ptr(), v_ptr, qo_ptr, ko_ptr, *q_rows, *k_rows, *v_rows, *qo_rows, *ko_rows,
+                             pos_ids.data_ptr(), pos_ids.stride(0), *tail, _err_word(k.device).data_ptr(), n, batch, hq, hkv,
+                             d, page_size, num_pages, _dtype_code(dtype, who))
+    status = lib.piekv_rope_axes(args, table, _stream_of(device))
+    if status:
+        check(status, who)
 
 
 def apply_rope_axes_inplace(q: Optional[torch.Tensor], k: torch.Tensor, pos_ids: torch.Tensor, rope: AxisRopeConfig) -> None:
@@ -561,7 +594,7 @@ def rope_axes_append_paged_kv_cache(q: Optional[torch.Tensor], k: torch.Tensor, 
     append_paged_kv_cache; a token whose request, slot or page does not exist is skipped and reported
     (`device_error`), its q is still rotated."""
     if q is not None and q_out is None:
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
     _rope_axes(q, k, v, pos_ids, rope, q_out, None, "rope_axes_append_paged_kv_cache",
                (batch_indices, positions, paged_kv_cache, kv_indices, kv_indptr))
     return q_out
@@ -719,6 +752,18 @@ class BatchDecodeWithPagedKVCacheWrapper:
                           hq=int(num_qo_heads), hkv=int(num_kv_heads), d=int(head_dim), page_size=int(page_size),
                           dtype=q_data_type, window_left=int(window_left), first_tokens=first_tokens,
                           sm_scale=float(sm_scale) if sm_scale is not None else 1.0 / math.sqrt(head_dim))
+        if first_tokens > 0:
+            for t, name in ((indices, "indices"), (last_page_len, "last_page_len"),
+                            (self.workspace_buffer, "workspace_buffer")):
+                if t.device != indptr.device:
+                    raise ValueError(f"{name} is on {t.device}, indptr on {indptr.device}")
+            pl = self._plan
+            pl["shape"] = torch.Size((batch, pl["hq"], pl["d"]))
+            pl["first_options"] = _attn_options(pl["window_left"], None, pl["hq"], first_tokens)
+            pl["first_call"] = ((indptr.data_ptr(), indices.data_ptr(), last_page_len.data_ptr(), batch, pl["hq"],
+                                 pl["hkv"], pl["d"], pl["page_size"]),
+                                (self.workspace_buffer.data_ptr(), self.workspace_buffer.numel(),
+                                 _err_word(indptr.device).data_ptr()), indptr.get_device())
 
     def run(self, q: torch.Tensor, paged_kv_cache: torch.Tensor, out: Optional[torch.Tensor] = None,
             return_lse: bool = False, sinks: Optional[torch.Tensor] = None, sm_scale: Optional[float] = None):
@@ -727,6 +772,8 @@ class BatchDecodeWithPagedKVCacheWrapper:
         if self._plan is None:
             raise RuntimeError("Must call plan() before run()")
         pl = self._plan
+        if pl["first_tokens"] > 0:
+            return self._run_first_tokens(q, paged_kv_cache, out, return_lse, sinks, sm_scale)
         _require_cuda(q, "q")
         num_pages, page_size, hkv, d = _check_pool(paged_kv_cache)
         qs = _rows(q, "q")
@@ -743,7 +790,7 @@ class BatchDecodeWithPagedKVCacheWrapper:
             raise ValueError("out must be a contiguous tensor shaped and typed like q")
         lse = torch.empty((pl["batch"], pl["hq"]), dtype=torch.float32, device=q.device) if return_lse else None
         ws = self.workspace_buffer
-        opt = _attn_options(pl["window_left"], sinks, pl["hq"], pl["first_tokens"])
+        opt = _attn_options(pl["window_left"], sinks, pl["hq"])
         check(lib.piekv_decode_run_opt(q.data_ptr(), qs[0], qs[1], paged_kv_cache.data_ptr(), out.data_ptr(),
                                        lse.data_ptr() if lse is not None else None, pl["indptr"].data_ptr(),
                                        pl["indices"].data_ptr(), pl["last_page_len"].data_ptr(), pl["batch"],
@@ -755,6 +802,39 @@ class BatchDecodeWithPagedKVCacheWrapper:
         return (out, lse) if return_lse else out
 
     forward = run
+
+    def _run_first_tokens(self, q, paged_kv_cache, out, return_lse, sinks, sm_scale):
+        """run() of a plan with a window and first tokens: the same checks, what the plan fixes prepared once."""
+        pl = self._plan
+        head, tail, device = pl["first_call"]
+        if not isinstance(q, torch.Tensor):
+            _require_cuda(q, "q")
+        q_rows = _device_rows(q, "q", device)
+        num_pages, page_size, hkv, d = _check_pool(paged_kv_cache)
+        if q.shape != pl["shape"]:
+            raise ValueError(f"q shape {tuple(q.shape)} differs from the plan {tuple(pl['shape'])}")
+        if page_size != pl["page_size"] or hkv != pl["hkv"] or d != pl["d"]:
+            raise ValueError("paged_kv_cache shape differs from the plan")
+        if q.dtype != paged_kv_cache.dtype:
+            raise ValueError(f"q dtype {q.dtype} differs from the cache dtype {paged_kv_cache.dtype}")
+        if paged_kv_cache.get_device() != device:
+            raise ValueError(f"the cache is on {paged_kv_cache.device}, the plan on cuda:{device}")
+        if out is None:
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        elif out.shape != q.shape or out.dtype != q.dtype or out.get_device() != device or not out.is_contiguous():
+            raise ValueError("out must be a contiguous tensor shaped and typed like q")
+        lse = torch.empty((pl["batch"], pl["hq"]), dtype=torch.float32, device=q.device) if return_lse else None
+        opt = pl["first_options"]
+        if sinks is not None:
+            opt = _attn_options(pl["window_left"], sinks, pl["hq"], pl["first_tokens"])
+        status = lib.piekv_decode_run_opt(q.data_ptr(), *q_rows, paged_kv_cache.data_ptr(), out.data_ptr(),
+                                          lse.data_ptr() if return_lse else None, *head, num_pages,
+                                          _dtype_code(q.dtype, "decode run"),
+                                          pl["sm_scale"] if sm_scale is None else float(sm_scale), *tail,
+                                          _stream_of(device), opt)
+        if status:
+            check(status, "BatchDecode.run")
+        return (out, lse) if return_lse else out
 
     def _fused_inputs(self, q, k, v, pos_ids, paged_kv_cache):
         """Checks shared by the fused entry points; returns (plan, num_pages, d, batch, q / k / v row strides)."""
@@ -941,7 +1021,8 @@ class BatchSharedPrefixDecodeWrapper:
         a.max_splits = splits
         a.sm_scale = float(sm_scale) if sm_scale is not None else 1.0 / math.sqrt(head_dim)
         self._args = a
-        self._plan = dict(shape=(batch, int(num_qo_heads), int(head_dim)), dtype=q_data_type, device=dev,
+        self._plan = dict(shape=torch.Size((batch, int(num_qo_heads), int(head_dim))), dtype=q_data_type, device=dev,
+                          index=indptr.get_device(),
                           cache=(int(page_size), int(num_kv_heads), int(head_dim)), sm_scale=a.sm_scale,
                           keep=(indptr, indices, last_page_len, group_indptr))
         self.replan()
@@ -958,20 +1039,22 @@ class BatchSharedPrefixDecodeWrapper:
         if self._plan is None:
             raise RuntimeError("Must call plan() before run()")
         pl = self._plan
-        _require_cuda(q, "q")
+        device = pl["index"]
+        if not isinstance(q, torch.Tensor):
+            _require_cuda(q, "q")
+        qs = _device_rows(q, "q", device)
         num_pages, page_size, hkv, d = _check_pool(paged_kv_cache)
-        qs = _rows(q, "q")
-        if tuple(q.shape) != pl["shape"]:
-            raise ValueError(f"q shape {tuple(q.shape)} differs from the plan {pl['shape']}")
+        if q.shape != pl["shape"]:
+            raise ValueError(f"q shape {tuple(q.shape)} differs from the plan {tuple(pl['shape'])}")
         if (page_size, hkv, d) != pl["cache"]:
             raise ValueError("paged_kv_cache shape differs from the plan")
         if q.dtype != pl["dtype"] or q.dtype != paged_kv_cache.dtype:
             raise ValueError(f"q dtype {q.dtype}, cache dtype {paged_kv_cache.dtype}, planned {pl['dtype']}")
-        if q.device != pl["device"] or paged_kv_cache.device != pl["device"]:
-            raise ValueError(f"q is on {q.device}, the cache on {paged_kv_cache.device}, the plan on {pl['device']}")
+        if paged_kv_cache.get_device() != device:
+            raise ValueError(f"the cache is on {paged_kv_cache.device}, the plan on cuda:{device}")
         if out is None:
-            out = torch.empty(pl["shape"], dtype=q.dtype, device=q.device)
-        elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous():
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        elif out.shape != q.shape or out.dtype != q.dtype or out.get_device() != device or not out.is_contiguous():
             raise ValueError("out must be a contiguous tensor shaped and typed like q")
         lse = torch.empty(pl["shape"][:2], dtype=torch.float32, device=q.device) if return_lse else None
         a = _lib.SharedPrefixArgs.from_buffer_copy(self._args)  # host threads may run the same plan
@@ -983,7 +1066,9 @@ class BatchSharedPrefixDecodeWrapper:
         a.lse = lse.data_ptr() if return_lse else None
         a.sm_scale = float(sm_scale) if sm_scale is not None else pl["sm_scale"]
         a.sinks = _sink_ptr(sinks, pl["shape"][1])
-        check(lib.piekv_shared_prefix_run(C.byref(a), _stream(q.device)), "BatchSharedPrefixDecode.run")
+        status = lib.piekv_shared_prefix_run(a, _stream_of(device))
+        if status:
+            check(status, "BatchSharedPrefixDecode.run")
         return (out, lse) if return_lse else out
 
     forward = run
