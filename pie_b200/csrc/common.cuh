@@ -187,6 +187,24 @@ __device__ __forceinline__ int ld_global_relaxed_sys(const int *p) {
   return v;
 }
 
+// Loads that stay where they are written: the compiler may otherwise sink a load into the branch that uses it, and a
+// batch of loads meant to be in flight together becomes a chain.  Through L2 only (.cg): data of other CTAs.
+__device__ __forceinline__ float4 ld_batch_cg(const float4 *p) {
+  float4 v;
+  asm volatile("ld.global.cg.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ float2 ld_batch_cg(const float2 *p) {
+  float2 v;
+  asm volatile("ld.global.cg.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "l"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint4 ld_batch(const void *p) {
+  uint4 v;
+  asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
+  return v;
+}
+
 __device__ __forceinline__ void fence_proxy_async_smem() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }

@@ -57,6 +57,7 @@ struct SpanParams {
   SpanPrefix prefix;    // requests == nullptr: window with first tokens
   int b0, nb;           // the slice of the batch
   int n_hb, ctas;       // head blocks, CTAs per head block
+  int sms;
   int *counters;        // [n_hb][nb], zero between launches
   float *part_o;        // [n_hb * ctas][2][HB * group][128]
   float2 *part_ml;      // [n_hb * ctas][2][HB * group]
@@ -73,16 +74,18 @@ struct Row {
     l = 0.f;
     o = make_float4(0.f, 0.f, 0.f, 0.f);
   }
-  __device__ __forceinline__ void fold(float2 ml, float4 v) {
-    if (!(ml.y > 0.f)) return;
-    const float mn = fmaxf(m, ml.x);
-    const float a = fast_exp2(m - mn), w = fast_exp2(ml.x - mn);  // m = -inf at first: 0
+  // (without a branch: a batch of folds follows a batch of loads)
+  __device__ __forceinline__ void fold(float2 ml, float4 v, bool live = true) {
+    live = live && ml.y > 0.f;  // a partial that saw nothing has no meaning in v
+    const float mn = live ? fmaxf(m, ml.x) : m;
+    const float a = m == mn ? 1.f : fast_exp2(m - mn);  // m = -inf at first: 0
+    const float w = live ? fast_exp2(ml.x - mn) : 0.f;
     m = mn;
-    l = fmaf(l, a, ml.y * w);
-    o.x = fmaf(o.x, a, v.x * w);
-    o.y = fmaf(o.y, a, v.y * w);
-    o.z = fmaf(o.z, a, v.z * w);
-    o.w = fmaf(o.w, a, v.w * w);
+    l = fmaf(l, a, live ? ml.y * w : 0.f);
+    o.x = fmaf(o.x, a, live ? v.x * w : 0.f);
+    o.y = fmaf(o.y, a, live ? v.y * w : 0.f);
+    o.z = fmaf(o.z, a, live ? v.z * w : 0.f);
+    o.w = fmaf(o.w, a, live ? v.w * w : 0.f);
   }
 };
 
@@ -119,6 +122,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
   __shared__ int sh_warp[kThreads / 32];
   __shared__ float2 sh_ml[kWarps][16];
   __shared__ int sh_abort, sh_last;
+  __shared__ short sh_closed[kMaxSlice];  // requests whose own pages this CTA has finished, for the prefix's join
 
   const AttnArgs &a = p.a;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -166,7 +170,11 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
   }
   __syncthreads();
   const long long line = sh_cost[nb];
-  const long long shares = max(1ll, min((long long)p.ctas, line / kMinUnits));
+  // Beside the prefix kernel only the first CTAs find an SM: the line is divided among those.
+  const int ctas = p.prefix.requests != nullptr && p.prefix.overlap
+                       ? max(1, (int)((long long)p.ctas * __ldg(p.prefix.header + 3) / p.sms))
+                       : p.ctas;
+  const long long shares = max(1ll, min((long long)ctas, line / kMinUnits));
   // share c is [line * c / shares, line * (c + 1) / shares); unit x lies in share ((x + 1) * shares - 1) / line
   const int x0 = c < shares ? (int)(line * c / shares) : (int)line;
   const int x1 = c < shares ? (int)(line * (c + 1) / shares) : (int)line;
@@ -245,13 +253,12 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
   const float scale_log2 = a.sm_scale * 1.4426950408889634f;
   T *out = reinterpret_cast<T *>(a.out);
   int it = 0;             // stages consumed
-  bool waited = p.prefix.requests == nullptr;  // the prefix kernel's results are visible
+  int closed = 0;         // entries of sh_closed
 
-  auto slot_base = [&](int share, int b) -> size_t {
-    // A share's first request may have begun in an earlier share (slot 0); otherwise the piece that has to be joined
-    // is the share's last one (slot 1).
-    const int first_share = share_of(sh_cost[b] + kOpenCost);
-    return ((size_t)(share * p.n_hb + hb) * 2 + (share == first_share ? 1 : 0)) * rows;
+  // A share's first request may have begun in an earlier share (slot 0); otherwise the piece that has to be joined is
+  // the share's last one (slot 1).
+  auto slot_base = [&](int share, bool first_piece) -> size_t {
+    return ((size_t)(share * p.n_hb + hb) * 2 + (first_piece ? 1 : 0)) * rows;
   };
   auto store_row = [&](int b, int r, Row x) {
     const int head = head0 + r;
@@ -280,14 +287,14 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
 #pragma unroll
         for (int u = 0; u < HW; ++u) {
           const size_t at = part(max(min(i0 + j, count[u] - 1), 0), min(r + u * kWarps, rows - 1));
-          ml[j][u] = __ldcg(pml + at);
-          v[j][u] = __ldcg(reinterpret_cast<const float4 *>(po + at * kDim) + lane);
+          ml[j][u] = ld_batch_cg(pml + at);
+          v[j][u] = ld_batch_cg(reinterpret_cast<const float4 *>(po + at * kDim) + lane);
         }
 #pragma unroll
       for (int j = 0; j < PB; ++j)
 #pragma unroll
         for (int u = 0; u < HW; ++u)
-          if (i0 + j < count[u]) acc[u].fold(ml[j][u], v[j][u]);
+          acc[u].fold(ml[j][u], v[j][u], i0 + j < count[u]);
     }
   };
   auto for_rows = [&](auto fn) {  // warp w: rows w, w + 4, ..., four at a time
@@ -301,11 +308,26 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
         fn(std::integral_constant<int, 1>{}, r);
     }
   };
+  // rows r, r + 4, ... of request b are complete, but for a prefix: out, or put by until the prefix's results are there
+  auto finish_rows = [&](auto hw, const Row *acc, int r, int b, bool later) {
+    constexpr int HW = decltype(hw)::value;
+#pragma unroll
+    for (int u = 0; u < HW; ++u) {
+      const int row = r + u * kWarps;
+      if (row >= rows) continue;
+      if (!later) {
+        store_row(b, row, acc[u]);
+      } else {
+        const size_t at = (size_t)(p.b0 + b) * a.hq + head0 + row;
+        *(reinterpret_cast<float4 *>(p.prefix.own_o + at * kDim) + lane) = acc[u].o;
+        if (lane == 0) p.prefix.own_ml[at] = make_float2(acc[u].m, acc[u].l);
+      }
+    }
+  };
+  auto has_prefix = [&](int b) { return p.prefix.requests != nullptr && __ldg(&p.prefix.requests[p.b0 + b].x) > 0; };
   // the prefix partials of request b into acc
   auto fold_prefix = [&](auto hw, Row *acc, int r, int b) {
-    if (p.prefix.requests == nullptr) return;
     const int2 rq = __ldg(&p.prefix.requests[p.b0 + b]);
-    if (rq.x == 0) return;
     const sprefix::Group g = p.prefix.groups[rq.y];
     const int member = p.b0 + b - g.first;
     constexpr int HW = decltype(hw)::value;
@@ -500,23 +522,18 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
       return x;
     };
     const bool whole = lo == 0 && hi == pages;
+    const int s_first = whole ? c : share_of(sh_cost[b] + kOpenCost);
+    const bool later = has_prefix(b);
     if (whole) {
-      if (!waited) {
-        asm volatile("griddepcontrol.wait;" ::: "memory");
-        waited = true;
-      }
       for_rows([&](auto hw, int r) {
         constexpr int HW = decltype(hw)::value;
         Row acc[HW];
 #pragma unroll
         for (int u = 0; u < HW; ++u) acc[u] = own_row(min(r + u * kWarps, rows - 1));
-        fold_prefix(hw, acc, r, b);
-#pragma unroll
-        for (int u = 0; u < HW; ++u)
-          if (r + u * kWarps < rows) store_row(b, r + u * kWarps, acc[u]);
+        finish_rows(hw, acc, r, b, later);
       });
     } else {
-      const size_t base = slot_base(c, b);
+      const size_t base = slot_base(c, c == s_first);
       for (int r = warp; r < rows; r += kWarps) {
         const Row x = own_row(r);
         *(reinterpret_cast<float4 *>(p.part_o + (base + r) * kDim) + lane) = x.o;
@@ -526,44 +543,65 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
     fence_proxy_async_smem();  // these tiles are next written by bulk copies
     consumer_sync();
     if (any && lane == 0) mbar_arrive(&empty_bar[s]);
-    if (whole) return;
-
-    // ================= partials: the last share of the request to arrive folds them all
-    const int s_first = share_of(sh_cost[b] + kOpenCost), s_last = share_of(sh_cost[b + 1] - 1);
-    const int n = s_last - s_first + 1;
-    if (tid == 0) {
-      __threadfence();
-      int *counter = p.counters + hb * nb + b;
-      const int old = atomicAdd(counter, 1);
-      sh_last = old + 1 == n ? 1 : 0;
-      if (sh_last) {
-        *counter = 0;  // nobody else touches it in this launch
+    if (!whole) {
+      // ================= partials: the last share of the request to arrive folds them all
+      const int n = share_of(sh_cost[b + 1] - 1) - s_first + 1;
+      if (tid == 0) {
         __threadfence();
+        int *counter = p.counters + hb * nb + b;
+        const int old = atomicAdd(counter, 1);
+        sh_last = old + 1 == n ? 1 : 0;
+        if (sh_last) {
+          *counter = 0;  // nobody else touches it in this launch
+          __threadfence();
+        }
       }
+      consumer_sync();
+      if (sh_last == 0) return;
+      for_rows([&](auto hw, int r) {
+        constexpr int HW = decltype(hw)::value;
+        Row acc[HW];
+        int count[HW];
+#pragma unroll
+        for (int u = 0; u < HW; ++u) {
+          acc[u].clear();
+          count[u] = n;
+        }
+        fold_rows(hw, acc, r, count, p.part_o, p.part_ml, [&](int i, int row) { return slot_base(s_first + i, i == 0) + row; });
+        finish_rows(hw, acc, r, b, later);
+      });
     }
-    consumer_sync();
-    if (sh_last == 0) return;
-    if (!waited) {
-      asm volatile("griddepcontrol.wait;" ::: "memory");
-      waited = true;
+    if (later) {
+      if (tid == 0) sh_closed[closed] = (short)b;
+      ++closed;
     }
+  });
+  if (p.prefix.requests == nullptr) return;
+  // ================= the prefix's results, folded with the requests' own.  Waiting only now keeps the pages streaming
+  // while the prefix kernel works; the launch must not end before that kernel in any case.
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  consumer_sync();
+  for (int x = 0; x < closed; ++x) {
+    const int b = sh_closed[x];
     for_rows([&](auto hw, int r) {
       constexpr int HW = decltype(hw)::value;
       Row acc[HW];
+      float2 ml[HW];
 #pragma unroll
-      for (int u = 0; u < HW; ++u) acc[u].clear();
-      int count[HW];
+      for (int u = 0; u < HW; ++u) {  // written above by this very warp
+        const size_t at = (size_t)(p.b0 + b) * a.hq + head0 + min(r + u * kWarps, rows - 1);
+        ml[u] = ld_batch_cg(p.prefix.own_ml + at);
+        acc[u].o = ld_batch_cg(reinterpret_cast<const float4 *>(p.prefix.own_o + at * kDim) + lane);
+      }
 #pragma unroll
-      for (int u = 0; u < HW; ++u) count[u] = n;
-      fold_rows(hw, acc, r, count, p.part_o, p.part_ml, [&](int i, int row) { return slot_base(s_first + i, b) + row; });
+      for (int u = 0; u < HW; ++u) {
+        acc[u].m = ml[u].x;
+        acc[u].l = ml[u].y;
+      }
       fold_prefix(hw, acc, r, b);
-#pragma unroll
-      for (int u = 0; u < HW; ++u)
-        if (r + u * kWarps < rows) store_row(b, r + u * kWarps, acc[u]);
+      finish_rows(hw, acc, r, b, false);
     });
-  });
-  // the launch must not end before the one it was allowed to overtake
-  if (!waited) asm volatile("griddepcontrol.wait;" ::: "memory");
+  }
 }
 
 template <typename T, int HB, bool WIDE>
@@ -631,6 +669,7 @@ int launch_decode_span(const AttnArgs &a, int dtype, const SpanPrefix &prefix, v
   p.prefix = prefix;
   p.n_hb = a.hkv / heads;
   p.ctas = ctas_per_head_block(a.hkv);
+  p.sms = sm_count();
   uint8_t *ws = reinterpret_cast<uint8_t *>(workspace);
   p.counters = reinterpret_cast<int *>(ws);
   const int64_t rows = 2ll * p.ctas * a.hq;

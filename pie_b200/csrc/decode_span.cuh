@@ -9,8 +9,11 @@ namespace piekv {
 struct SpanPrefix {
   const int2 *requests = nullptr;  // [batch] (pages read with the group, group); nullptr: no prefix
   const sprefix::Group *groups = nullptr;
+  const int *header = nullptr;     // the plan's
   const float *part_o = nullptr;   // [split][batch][Hq][128]
   const float2 *part_ml = nullptr;
+  float *own_o = nullptr;          // [batch][Hq][128]: the requests' own pages, until the prefix's results are there
+  float2 *own_ml = nullptr;
   int max_splits = 0;
   int overlap = 0;  // the launch may start before the prefix kernel has ended
 };

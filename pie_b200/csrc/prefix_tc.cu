@@ -106,8 +106,8 @@ __global__ void __launch_bounds__(kPxThreads, 1)
 
   // The kernel behind this one reads its own pages first and waits for these results only then.
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int items = *p.n_items;
-  if ((int)blockIdx.x >= items) return;
+  const int items = __ldg(p.header), ctas = __ldg(p.header + 2);
+  if ((int)blockIdx.x >= ctas) return;
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -161,7 +161,7 @@ __global__ void __launch_bounds__(kPxThreads, 1)
       uint64_t *full = is_v ? v_full : k_full, *empty = is_v ? v_empty : k_empty;
       int armed = 0;
       bool ok = true;
-      for (int i = blockIdx.x; ok && i < items; i += gridDim.x) {
+      for (int i = blockIdx.x; ok && i < items; i += ctas) {
         const Work w = work_of(p, i);
         for (int t = 0; ok && t < w.n[0]; ++t)
           for (int x = 0; x < (w.pair ? 1 : 2); ++x) {
@@ -233,7 +233,7 @@ __global__ void __launch_bounds__(kPxThreads, 1)
         };
         bool ok = true;
         int qi = 0;
-        for (int i = blockIdx.x; ok && i < items; i += gridDim.x, ++qi) {
+        for (int i = blockIdx.x; ok && i < items; i += ctas, ++qi) {
           const Work w = work_of(p, i);
           const int na = w.n[0], nb = w.n[1];
           ok = wait(&q_full[0], qi) && wait_k();
@@ -290,7 +290,7 @@ __global__ void __launch_bounds__(kPxThreads, 1)
     int sc = 0, oc = 0;  // score tiles and items (with tiles) finished: phases of s_full and o_done
     bool ok = true;
 
-    for (int i = blockIdx.x; ok && i < items; i += gridDim.x) {
+    for (int i = blockIdx.x; ok && i < items; i += ctas) {
       const Work w = work_of(p, i);
       const int rows = w.rows[x], n = w.n[x];
       const bool row_valid = row < rows;

@@ -8,7 +8,7 @@ struct PrefixTcParams {
   const void *q;  // [batch, Hq, 128], rows 16-byte aligned
   int64_t q_sn, q_sh;
   const int32_t *kv_indptr, *kv_indices;
-  const int *n_items;
+  const int *header;  // the plan's
   const sprefix::Group *groups;
   const sprefix::Item *items;
   float *part_o;    // [split][batch][Hq][128], unnormalised

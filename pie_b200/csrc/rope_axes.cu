@@ -168,8 +168,8 @@ __global__ void __launch_bounds__(kThreads, 3) rope_axes_rows_kernel(const __gri
       if (hh < h1) {
         const T *src = hh < q_heads ? q + (int64_t)hh * p.q_sh
                                     : (hh < k_end ? k + (int64_t)(hh - q_heads) * p.k_sh : v + (int64_t)(hh - k_end) * p.v_sh);
-        lo[u] = *reinterpret_cast<const uint4 *>(src + e0);
-        hi[u] = *reinterpret_cast<const uint4 *>(src + e1);
+        lo[u] = ld_batch(src + e0);
+        hi[u] = ld_batch(src + e1);
       }
     }
     if (!ready) {  // while the first rows are on their way

@@ -14,7 +14,6 @@ namespace {
 constexpr int64_t kCounterBytes = 65536;
 // A prefix shorter than this is left to the requests: reading it once saves less than joining two parts costs.
 constexpr int kMinSharedPages = 4;
-constexpr int kMinTilesPerItem = 2;
 
 // Full pages of request b (the partly filled last page of a fork is a copy of its own).
 __device__ __forceinline__ int full_pages(const int32_t *kv_indptr, const int32_t *last, int b, int page_size) {
@@ -61,17 +60,31 @@ __global__ void __launch_bounds__(128) sp_match_kernel(const int32_t *__restrict
   if (threadIdx.x == 0) match[b] = sh_first;
 }
 
-// Checks the grouping, decides what every group reads once and lists the pieces of work.  One block.
-__global__ void __launch_bounds__(1024) sp_plan_kernel(const int32_t *__restrict__ group_indptr, int batch, int groups,
+// Times in units of one kv tile (64 KiB of K and V, the time an SM needs to stream them: 1.45 us), as measured on the
+// two attention kernels: starting a prefix CTA, an item's own costs (query rows in, partial rows out), a tile against
+// more than 128 rows (bound by the tensor and special-function pipes) or fewer (by the stream), starting the other
+// kernel, and one row of partial results written and folded.
+constexpr float kStartPrefix = 4.f, kStartItem = 4.f, kTilePair = 1.8f, kTileSingle = 1.f, kStartSpan = 3.f;
+constexpr float kFoldPerRow = 4 * 512.f / 65536.f;
+constexpr int kMaxSearchGroups = 256;
+
+// Checks the grouping, decides what every group reads once, how many SMs work on that while the others stream the
+// requests' own pages, and into how many pieces each prefix is cut.  One block.
+//
+// More pieces spread a prefix over more SMs but leave more partial results to fold; more CTAs on the prefix leave
+// fewer SMs to the other kernel, which runs at the same time.  Each thread costs one (CTAs, tiles per piece) pair with
+// the constants above; the cheapest is taken.
+__global__ void __launch_bounds__(1024) sp_plan_kernel(const int32_t *__restrict__ kv_indptr,
+                                                       const int32_t *__restrict__ group_indptr, int batch, int groups,
                                                        int page_size, int heads_per_kv, int hkv, int max_splits,
                                                        int sms, PlanView v, int32_t *err) {
-  __shared__ long long sh_tiles;
-  __shared__ int sh_base, sh_most, sh_per, sh_used, sh_count;
+  __shared__ unsigned long long sh_tiles, sh_own, sh_best;
+  __shared__ int sh_base, sh_most, sh_used, sh_count;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (tid == 0) {
-    sh_tiles = 0;
+    sh_tiles = sh_own = 0;
+    sh_best = ~0ull;
     sh_base = sh_most = sh_used = sh_count = 0;
-    sh_per = 1 << 30;
   }
   int bad = -1;
   for (int g = tid; g < groups; g += 1024) {
@@ -82,24 +95,36 @@ __global__ void __launch_bounds__(1024) sp_plan_kernel(const int32_t *__restrict
   const bool refused = __syncthreads_or(bad >= 0) != 0;
   if (refused) {  // every request on its own
     for (int b = tid; b < batch; b += 1024) v.requests[b] = make_int2(0, 0);
-    if (tid == 0) v.header[0] = v.header[1] = 0;
+    if (tid == 0) {
+      v.header[0] = v.header[1] = v.header[2] = 0;
+      v.header[3] = sms;
+    }
     return;
   }
-  // ---- a warp per group: pages common to all its requests
+  auto blocks_of = [&](int members) { return (int)(((long long)members * heads_per_kv + kRowsPerItem - 1) / kRowsPerItem); };
+  auto tiles_of = [&](int pages) { return (pages * page_size + kTileTokens - 1) / kTileTokens; };
+  // ---- a warp per group: pages common to all its requests, pages left to each
   for (int g = warp; g < groups; g += 32) {
     const int a = group_indptr[g], m = group_indptr[g + 1] - a;
     int pages = 1 << 30;
-    for (int i = lane; i < m; i += 32) pages = min(pages, v.match[a + i]);
+    long long own = 0;
+    for (int i = lane; i < m; i += 32) {
+      pages = min(pages, v.match[a + i]);
+      own += max(0, kv_indptr[a + i + 1] - kv_indptr[a + i]);
+    }
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) pages = min(pages, __shfl_xor_sync(0xffffffffu, pages, d));
+    for (int d = 16; d > 0; d >>= 1) {
+      pages = min(pages, __shfl_xor_sync(0xffffffffu, pages, d));
+      own += __shfl_xor_sync(0xffffffffu, own, d);
+    }
     if (m < 2 || pages < kMinSharedPages) pages = 0;
     for (int i = lane; i < m; i += 32) v.requests[a + i] = make_int2(pages, g);
     if (lane == 0) {
       v.groups[g] = Group{a, m, pages, 0};
+      atomicAdd(&sh_own, (unsigned long long)(own - (long long)m * pages));
       if (pages > 0) {
-        const int tiles = (pages * page_size + kTileTokens - 1) / kTileTokens;
-        const int blocks = (int)(((long long)m * heads_per_kv + kRowsPerItem - 1) / kRowsPerItem) * hkv;
-        atomicAdd(reinterpret_cast<unsigned long long *>(&sh_tiles), (unsigned long long)tiles * blocks);
+        const int tiles = tiles_of(pages), blocks = blocks_of(m) * hkv;
+        atomicAdd(&sh_tiles, (unsigned long long)tiles * blocks);
         atomicAdd(&sh_base, blocks);
         atomicMax(&sh_most, tiles);
         atomicAdd(&sh_used, 1);
@@ -107,38 +132,50 @@ __global__ void __launch_bounds__(1024) sp_plan_kernel(const int32_t *__restrict
     }
   }
   __syncthreads();
-  // ---- tiles per piece: one piece per SM where that is possible (each thread tries a length), four rounds of
-  // pieces where there are more (group, kv head, row block) triples than SMs
-  const long long total = sh_tiles;
-  const int base = sh_base, most = sh_most;
-  auto blocks_of = [&](const Group &g) {
-    return (int)(((long long)g.members * heads_per_kv + kRowsPerItem - 1) / kRowsPerItem) * hkv;
-  };
-  auto tiles_of = [&](const Group &g) { return (g.pages * page_size + kTileTokens - 1) / kTileTokens; };
-  if (base > sms) {
-    if (tid == 0) sh_per = max(kMinTilesPerItem, (int)((total + 4 * sms - 1) / (4 * sms)));
-  } else if (base > 0) {
-    const int least = max(kMinTilesPerItem, (int)((total + sms - 1) / sms));
-    for (int per = least + tid; per < most && per < sh_per; per += 1024) {
-      int n = 0;
-      for (int g = 0; g < groups && n <= sms; ++g) {
+  const float own_tiles = (float)((double)sh_own * page_size / kTileTokens * hkv);
+  const int most = max(sh_most, 1), max_chunks = max(1, max_splits / 2);
+  // thread = (CTAs: 32 steps up to all SMs, tiles per piece: the longest prefix in 1 .. 32 pieces)
+  int ctas = max(1, sms * (warp + 1) / 32);
+  int per = (most + lane) / (lane + 1);
+  if (sh_base > 0) {
+    if (groups <= kMaxSearchGroups) {
+      long long items = 0, folds = 0, pairs = 0;
+      int longest = 0;  // tiles of an item
+      for (int g = 0; g < groups; ++g) {
         const Group gr = v.groups[g];
-        if (gr.pages > 0) n += blocks_of(gr) * ((tiles_of(gr) + per - 1) / per);
+        if (gr.pages == 0) continue;
+        const int chunks = min((tiles_of(gr.pages) + per - 1) / per, max_chunks);
+        const int rows = gr.members * heads_per_kv;
+        longest = max(longest, (tiles_of(gr.pages) + chunks - 1) / chunks);
+        items += (long long)blocks_of(gr.members) * chunks;
+        if (rows > kRowsPerItem / 2) pairs += (long long)blocks_of(gr.members) * chunks;
+        folds += (long long)rows * chunks * (rows % kRowsPerItem <= kRowsPerItem / 2 && rows < kRowsPerItem ? 2 : 1);
       }
-      if (n <= sms) {
-        atomicMin(&sh_per, per);
-        break;
+      items *= hkv;
+      if (items <= sh_base + kSpareItems) {
+        const long long rounds = (items + ctas - 1) / ctas;
+        const float tile = kTileSingle + (kTilePair - kTileSingle) * (float)(pairs * hkv) / (float)items;
+        const float prefix = kStartPrefix + (float)rounds * (kStartItem + tile * (float)longest);
+        const float fold = (float)folds * hkv * kFoldPerRow / (float)sms;
+        const float own = kStartSpan + own_tiles / (float)(ctas < sms ? sms - ctas : sms);
+        const float cost = (ctas < sms ? fmaxf(prefix, own) : prefix + own) + fold;
+        atomicMin(&sh_best, ((unsigned long long)__float_as_uint(cost) << 32) | (unsigned)tid);
       }
+    } else if (tid == 0) {  // hundreds of groups: enough pieces without cutting
+      sh_best = 31 * 32;    // all SMs, whole prefixes
     }
   }
   __syncthreads();
-  const int per = min(sh_per, max(most, 1));
-  const int max_chunks = max(1, max_splits / 2);
+  if (sh_base > 0) {
+    const int best = sh_best == ~0ull ? 31 * 32 : (int)(sh_best & 1023);
+    ctas = max(1, sms * (best / 32 + 1) / 32);
+    per = (most + best % 32) / (best % 32 + 1);
+  }
   for (int g = warp; g < groups; g += 32) {
-    Group gr = v.groups[g];
+    const Group gr = v.groups[g];
     if (gr.pages == 0) continue;
-    const int blocks = blocks_of(gr) / hkv;
-    int chunks = min((tiles_of(gr) + per - 1) / per, max_chunks);
+    const int blocks = blocks_of(gr.members);
+    int chunks = min((tiles_of(gr.pages) + per - 1) / per, max_chunks);
     int at = 0;
     if (lane == 0) {
       at = atomicAdd(&sh_count, blocks * hkv * chunks);
@@ -155,8 +192,11 @@ __global__ void __launch_bounds__(1024) sp_plan_kernel(const int32_t *__restrict
   }
   __syncthreads();
   if (tid == 0) {
-    v.header[0] = min(sh_count, v.max_items);
+    const int items = min(sh_count, v.max_items);
+    v.header[0] = items;
     v.header[1] = sh_used;
+    v.header[2] = min(ctas, items);
+    v.header[3] = items > 0 && ctas < sms ? sms - ctas : sms;
   }
 }
 
@@ -190,9 +230,9 @@ extern "C" int64_t piekv_shared_prefix_plan_bytes(int32_t batch, int32_t num_gro
   return plan_view(nullptr, batch, num_groups, num_qo_heads, num_kv_heads).bytes;
 }
 
-// Partials of the prefix: max_splits per (request, query head).
+// Partials: max_splits of the prefix and one of the request's own pages per (request, query head).
 static int64_t prefix_ml_bytes(int batch, int hq, int max_splits) {
-  return ((int64_t)max_splits * batch * hq * 8 + 255) / 256 * 256;
+  return (((int64_t)max_splits + 1) * batch * hq * 8 + 255) / 256 * 256;
 }
 
 extern "C" int64_t piekv_shared_prefix_workspace_bytes(int32_t batch, int32_t num_qo_heads, int32_t num_kv_heads,
@@ -200,7 +240,7 @@ extern "C" int64_t piekv_shared_prefix_workspace_bytes(int32_t batch, int32_t nu
   if (batch < 0 || num_qo_heads <= 0 || num_kv_heads <= 0 || max_splits < 1) return 0;
   if (head_dim != 128) return kCounterBytes;
   return kCounterBytes + (decode_span_scratch_bytes(num_qo_heads, num_kv_heads) + 255) / 256 * 256 +
-         prefix_ml_bytes(batch, num_qo_heads, max_splits) + (int64_t)max_splits * batch * num_qo_heads * 128 * 4;
+         prefix_ml_bytes(batch, num_qo_heads, max_splits) + ((int64_t)max_splits + 1) * batch * num_qo_heads * 128 * 4;
 }
 
 extern "C" int piekv_shared_prefix_plan(const piekv_shared_prefix_args *args, void *stream) {
@@ -212,8 +252,8 @@ extern "C" int piekv_shared_prefix_plan(const piekv_shared_prefix_args *args, vo
   sp_match_kernel<<<a.batch, 128, 0, st>>>(a.kv_indptr, a.kv_indices, a.kv_last_page_len, a.group_indptr, a.batch,
                                            a.num_groups, a.page_size, v.match);
   PIEKV_LAUNCH_CHECK("sp_match_kernel");
-  sp_plan_kernel<<<1, 1024, 0, st>>>(a.group_indptr, a.batch, a.num_groups, a.page_size, a.num_qo_heads / a.num_kv_heads,
-                                     a.num_kv_heads, a.max_splits, sm_count(), v, a.err);
+  sp_plan_kernel<<<1, 1024, 0, st>>>(a.kv_indptr, a.group_indptr, a.batch, a.num_groups, a.page_size,
+                                     a.num_qo_heads / a.num_kv_heads, a.num_kv_heads, a.max_splits, sm_count(), v, a.err);
   PIEKV_LAUNCH_CHECK("sp_plan_kernel");
   return 0;
 }
@@ -261,7 +301,7 @@ extern "C" int piekv_shared_prefix_run(const piekv_shared_prefix_args *args, voi
   px.q_sh = a.q_sh;
   px.kv_indptr = a.kv_indptr;
   px.kv_indices = a.kv_indices;
-  px.n_items = v.header;
+  px.header = v.header;
   px.groups = v.groups;
   px.items = v.items;
   px.part_ml = reinterpret_cast<float2 *>(ws);
@@ -276,9 +316,12 @@ extern "C" int piekv_shared_prefix_run(const piekv_shared_prefix_args *args, voi
   if (int rc = launch_prefix_tc(px, a.pool, a.hkv, args->dtype, st)) return rc;
   SpanPrefix sp;
   sp.requests = v.requests;
+  sp.header = v.header;
   sp.groups = v.groups;
   sp.part_o = px.part_o;
   sp.part_ml = px.part_ml;
+  sp.own_o = px.part_o + (int64_t)args->max_splits * a.batch * a.hq * 128;
+  sp.own_ml = px.part_ml + (int64_t)args->max_splits * a.batch * a.hq;
   sp.max_splits = args->max_splits;
   sp.overlap = 1;
   return launch_decode_span(a, args->dtype, sp, args->workspace, args->workspace_bytes, st);

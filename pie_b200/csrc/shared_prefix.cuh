@@ -22,7 +22,8 @@ struct Item {
 };
 
 struct PlanView {
-  int *header;       // [0] items  [1] prefixes in use
+  int *header;       // [0] items  [1] prefixes in use  [2] CTAs that work on them  [3] SMs left for the requests' own
+                     // pages meanwhile (all of them when the two kernels follow each other)
   Group *groups;     // [num_groups]
   int2 *requests;    // [batch] (pages read with the group, group)
   int *match;        // [batch] scratch: leading full pages equal to the group's first request's
