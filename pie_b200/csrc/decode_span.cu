@@ -13,14 +13,19 @@
 // Work partition (in the kernel, no plan, so a captured graph follows its tables): every CTA reads the page counts
 // of the whole batch, scans them, and takes an equal share [X_c, X_{c+1}) of the line on which each request occupies
 // its visible pages plus kOpenCost (opening and closing a request costs about as much as streaming that many pages).
-// A request cut by a share's end leaves partials in the two slots a CTA owns; CTAs of a request are consecutive, so
-// who holds a partial, and how many there are, follows from the line - there is no slot allocator, and results are
-// reproducible bit for bit.  The last CTA to arrive (one counter per request and head block, left zero) folds them.
+// A request cut by a share's end leaves partials in the two slots a share owns; the shares of a request are
+// consecutive, so who holds a partial, and how many there are, follows from the line - there is no slot allocator, and
+// results are reproducible bit for bit.  The last share to arrive (a counter per request and kv head, left zero) folds.
 //
-// Data path: a CTA takes HB kv heads of a page (HB = 4, 2 or 1, whichever divides), 4/HB pages per stage: 32 KiB by
-// TMA into three stages, two CTAs per SM (192 KiB in flight per SM).  The producer warp and the consumers walk the
-// same sequence independently; only barriers pass between them.  Consumer warp w owns tile (page w / HB, head
-// w % HB): K and V [16 tokens x 128], 128-byte swizzled, as the m16n8k16 tensor-core fragments want them.
+// Data path: a CTA takes HB kv heads of a page (HB = 2, or 1 where the head count is odd): HB * 8 KiB by TMA into a ring
+// of stages, 192 KiB in flight per SM.  The producer warp and the consumer warps walk the same sequence independently;
+// only the ring's barriers pass between them.  Consumer warp w owns head w: K and V [16 tokens x 128], 128-byte swizzled,
+// as the m16n8k16 tensor-core fragments want them.  No step waits for the whole CTA: a warp opens, closes and folds the
+// rows of its own head, and arrives only when its stream has ended.  (With block-wide closes through shared memory and
+// arrivals on the way, a third of a CTA's time on short requests went into them.)
+//
+// Partial rows are kept in the order the MMA fragments hold them: element nt * 8 + 2 * q + e of a row at
+// q * 32 + nt * 2 + e, so that a lane's 32 values of a row are one run of 128 bytes.
 //
 // Precision: a GQA group of up to 8 heads fills rows 0-7 of the 16-row MMA.  Rows 8-15 then carry the part of each
 // probability that its 16-bit rounding drops, so P V is formed with 16 bits of P (bf16) at no extra MMA.
@@ -39,18 +44,21 @@ namespace {
 
 constexpr int kDim = 128;
 constexpr int kPage = 16;
-constexpr int kWarps = 4;  // consumer warps
-constexpr int kConsumers = kWarps * 32;
-constexpr int kThreads = kConsumers + 32;
-constexpr int kStages = 3;
 constexpr int kTileBytes = 8192;  // one (page, head): K 4 KiB + V 4 KiB
-constexpr int kStageBytes = kWarps * kTileBytes;
-constexpr int kSmemBytes = kStages * kStageBytes + 1024;
-constexpr int kCtasPerSm = 2;
 constexpr int kCounterBytes = 65536;
-constexpr int kMaxSlice = 512;  // requests per launch: their page counts are kept in shared memory
-constexpr int kOpenCost = 2;    // pages
-constexpr int kMinUnits = 4;    // a share is not made smaller than this
+constexpr int kMaxSlice = 512;   // requests per launch: the line is kept in shared memory
+constexpr int kOpenCost = 2;     // pages
+constexpr int kMinUnits = 4;     // a share is not made smaller than this
+
+// Launch shape for HB heads per CTA: 12 warps per SM (168 registers each) and 24 tiles in flight.
+template <int HB>
+struct Shape {
+  static constexpr int kThreads = (HB + 1) * 32;
+  static constexpr int kCtasPerSm = HB == 1 ? 6 : 4;
+  static constexpr int kStages = HB == 1 ? 4 : 3;
+  static constexpr int kStageBytes = HB * kTileBytes;
+  static constexpr int kSmemBytes = kStages * kStageBytes + 1024;
+};
 
 struct SpanParams {
   AttnArgs a;           // pointers of the whole batch
@@ -58,34 +66,37 @@ struct SpanParams {
   int b0, nb;           // the slice of the batch
   int n_hb, ctas;       // head blocks, CTAs per head block
   int sms;
-  int *counters;        // [n_hb][nb], zero between launches
-  float *part_o;        // [n_hb * ctas][2][HB * group][128]
-  float2 *part_ml;      // [n_hb * ctas][2][HB * group]
+  int *counters;        // [Hkv][nb], zero between launches
+  float *part_o;        // [share][2][Hq][128]
+  float2 *part_ml;      // [share][2][Hq]
 };
 
-__device__ __forceinline__ void consumer_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kConsumers) : "memory"); }
-
-// (maximum, sum, 4 columns of the accumulator) of one row, and the fold of another partial into it
-struct Row {
+// Four rows per warp, eight lanes a row: maximum, sum and 16 columns of the accumulator, column groups k * 8 + (lane & 7)
+// of four.
+struct Rows {
   float m, l;
-  float4 o;
+  float4 o[4];
   __device__ __forceinline__ void clear() {
     m = -INFINITY;
     l = 0.f;
-    o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
   }
   // (without a branch: a batch of folds follows a batch of loads)
-  __device__ __forceinline__ void fold(float2 ml, float4 v, bool live = true) {
+  __device__ __forceinline__ void fold(float2 ml, const float4 *v, bool live) {
     live = live && ml.y > 0.f;  // a partial that saw nothing has no meaning in v
     const float mn = live ? fmaxf(m, ml.x) : m;
     const float a = m == mn ? 1.f : fast_exp2(m - mn);  // m = -inf at first: 0
     const float w = live ? fast_exp2(ml.x - mn) : 0.f;
     m = mn;
     l = fmaf(l, a, live ? ml.y * w : 0.f);
-    o.x = fmaf(o.x, a, live ? v.x * w : 0.f);
-    o.y = fmaf(o.y, a, live ? v.y * w : 0.f);
-    o.z = fmaf(o.z, a, live ? v.z * w : 0.f);
-    o.w = fmaf(o.w, a, live ? v.w * w : 0.f);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      o[k].x = fmaf(o[k].x, a, live ? v[k].x * w : 0.f);
+      o[k].y = fmaf(o[k].y, a, live ? v[k].y * w : 0.f);
+      o[k].z = fmaf(o[k].z, a, live ? v[k].z * w : 0.f);
+      o[k].w = fmaf(o[k].w, a, live ? v[k].w * w : 0.f);
+    }
   }
 };
 
@@ -112,17 +123,15 @@ __device__ __forceinline__ Visible visible_part(const SpanParams &p, int b) {
 }
 
 template <typename T, int HB, bool WIDE>
-__global__ void __launch_bounds__(kThreads, kCtasPerSm)
+__global__ void __launch_bounds__(Shape<HB>::kThreads, Shape<HB>::kCtasPerSm)
     decode_span_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ SpanParams p) {
-  constexpr int PG = kWarps / HB;  // pages per stage
+  constexpr int kThreads = Shape<HB>::kThreads, kStages = Shape<HB>::kStages, kStageBytes = Shape<HB>::kStageBytes;
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t full_bar[kStages], empty_bar[kStages];
-  __shared__ int sh_cost[kMaxSlice + 1];       // prefix sums of pages + kOpenCost
-  __shared__ __align__(16) int4 sh_req[kMaxSlice];  // first list entry, length, front, second
+  __shared__ int sh_cost[kMaxSlice + 1];  // prefix sums of pages + kOpenCost
   __shared__ int sh_warp[kThreads / 32];
-  __shared__ float2 sh_ml[kWarps][16];
-  __shared__ int sh_abort, sh_last;
-  __shared__ short sh_closed[kMaxSlice];  // requests whose own pages this CTA has finished, for the prefix's join
+  __shared__ short sh_closed[HB][kMaxSlice];  // requests whose own pages a warp has finished, for the prefix's join
+  __shared__ int sh_abort;
 
   const AttnArgs &a = p.a;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -134,7 +143,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
   if (tid == 0) {
     for (int s = 0; s < kStages; ++s) {
       mbar_init(&full_bar[s], 1);
-      mbar_init(&empty_bar[s], kWarps);
+      mbar_init(&empty_bar[s], HB);
     }
     sh_abort = 0;
     mbar_fence_init();
@@ -146,9 +155,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
     for (int i = 0; i < per; ++i) {
       const int b = tid * per + i;
       if (b < nb) {
-        const Visible v = visible_part(p, p.b0 + b);
-        sh_req[b] = make_int4(__ldg(a.kv_indptr + p.b0 + b), v.len, v.front, v.second);
-        sum += v.pages + kOpenCost;
+        sum += visible_part(p, p.b0 + b).pages + kOpenCost;
         sh_cost[b + 1] = sum;  // relative to this thread's first
       }
     }
@@ -202,23 +209,23 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
     }
   };
 
-  if (warp == kWarps) {
+  if (warp == HB) {
     // ------------------------------------------------------------------ producer
     int armed = 0;
     bool ok = true;
     for_pieces([&](int b, int lo, int hi, int) {
-      const int4 r = sh_req[b];
+      const Visible r = visible_part(p, p.b0 + b);
+      const int32_t *list = a.kv_indices + __ldg(a.kv_indptr + p.b0 + b);
       int base = lo - 32, id = 0;
-      for (int v = lo; v < hi && ok; v += PG) {
-        const int npg = min(PG, hi - v);
-        if (v + npg > base + 32) {  // the next 32 page ids in one load
+      for (int v = lo; v < hi && ok; ++v) {
+        if (v >= base + 32) {  // the next 32 page ids in one load
           base = v;
           const int vi = v + lane;
-          id = vi < hi ? __ldg(a.kv_indices + r.x + (vi < r.z ? vi : vi - r.z + r.w)) : 0;
+          id = vi < hi ? __ldg(list + (vi < r.front ? vi : vi - r.front + r.second)) : 0;
         }
-        int page = __shfl_sync(0xffffffffu, id, (v - base + lane) & 31);
-        if (lane < npg && (page < 0 || page >= a.num_pages)) {
-          if (hb == 0) report_error(a.err, PIEKV_ERR_PAGE_ID, KID_DECODE, p.b0 + b, page);
+        int page = __shfl_sync(0xffffffffu, id, v - base);
+        if (page < 0 || page >= a.num_pages) {
+          if (hb == 0 && lane == 0) report_error(a.err, PIEKV_ERR_PAGE_ID, KID_DECODE, p.b0 + b, page);
           page = a.num_pages;  // outside the tensor map: zeros
         }
         const int s = armed % kStages;
@@ -228,10 +235,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
           ok = false;
           break;
         }
-        if (lane == 0) mbar_arrive_expect_tx(&full_bar[s], (uint32_t)(npg * HB * kTileBytes));
-        __syncwarp();
-        if (lane < npg)
-          tma_load_5d(stage0 + s * kStageBytes + lane * (HB * kTileBytes), &tmap, 0, 0, 0, hb * HB, page * 2, &full_bar[s]);
+        if (lane == 0) {
+          mbar_arrive_expect_tx(&full_bar[s], (uint32_t)kStageBytes);
+          tma_load_5d(stage0 + s * kStageBytes, &tmap, 0, 0, 0, hb * HB, page * 2, &full_bar[s]);
+        }
         ++armed;
       }
     });
@@ -244,115 +251,43 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
     return;
   }
 
-  // -------------------------------------------------------------------- consumers
-  const int pslot = warp / HB, h = warp % HB;
+  // -------------------------------------------------------------------- consumers: warp = kv head
   const int quad = lane >> 2, qlane = lane & 3;
   const int group = a.hq / a.hkv;
-  const int rows = HB * group;                // query heads of this head block: head0 .. head0 + rows
-  const int head0 = hb * HB * group;
+  const int hk = hb * HB + warp;
+  const int head0 = hk * group;  // query heads head0 .. head0 + group - 1 are the MMA's rows
   const float scale_log2 = a.sm_scale * 1.4426950408889634f;
   T *out = reinterpret_cast<T *>(a.out);
-  int it = 0;             // stages consumed
-  int closed = 0;         // entries of sh_closed
+  const bool prefixed = p.prefix.requests != nullptr;
+  int it = 0;      // stages consumed
+  int closed = 0;  // entries of sh_closed
+  int pend_b[2] = {-1, -1};  // requests with a partial in this share's slots
 
   // A share's first request may have begun in an earlier share (slot 0); otherwise the piece that has to be joined is
   // the share's last one (slot 1).
   auto slot_base = [&](int share, bool first_piece) -> size_t {
-    return ((size_t)(share * p.n_hb + hb) * 2 + (first_piece ? 1 : 0)) * rows;
+    return ((size_t)share * 2 + (first_piece ? 1 : 0)) * a.hq + head0;
   };
-  auto store_row = [&](int b, int r, Row x) {
-    const int head = head0 + r;
-    const float l = add_sink(x.l, x.m, a.sinks, head);
-    const float inv = l > 0.f ? 1.f / l : 0.f;
-    uint2 pk;
-    pk.x = pack2<T>(x.o.x * inv, x.o.y * inv);
-    pk.y = pack2<T>(x.o.z * inv, x.o.w * inv);
-    const size_t at = (size_t)(p.b0 + b) * a.hq + head;
-    *reinterpret_cast<uint2 *>(out + at * kDim + lane * 4) = pk;
-    if (a.lse != nullptr && lane == 0) a.lse[at] = l > 0.f ? (x.m + log2f(l)) * 0.6931471805599453f : -INFINITY;
+  auto first_share = [&](int b) { return share_of(sh_cost[b] + kOpenCost); };
+  auto last_share = [&](int b) { return share_of(sh_cost[b + 1] - 1); };
+  auto has_prefix = [&](int b) { return prefixed && __ldg(&p.prefix.requests[p.b0 + b].x) > 0; };
+  auto store_lse = [&](int b, int head, float m, float l) {
+    if (a.lse != nullptr)
+      a.lse[(size_t)(p.b0 + b) * a.hq + head] = l > 0.f ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
   };
-  // Fold stored partials of rows r, r + 4, ... (HW of them, count[u] of each) into acc: partial i of row x is at
-  // part(i, x).
-  auto fold_rows = [&](auto hw, Row *acc, int r, const int *count, const float *po, const float2 *pml, auto part) {
-    constexpr int HW = decltype(hw)::value;
-    constexpr int PB = 16 / HW;  // loads of 16 partials are in flight before one is used
-    int most = 0;
-#pragma unroll
-    for (int u = 0; u < HW; ++u) most = max(most, count[u]);
-    for (int i0 = 0; i0 < most; i0 += PB) {
-      float2 ml[PB][HW];
-      float4 v[PB][HW];
-#pragma unroll
-      for (int j = 0; j < PB; ++j)
-#pragma unroll
-        for (int u = 0; u < HW; ++u) {
-          const size_t at = part(max(min(i0 + j, count[u] - 1), 0), min(r + u * kWarps, rows - 1));
-          ml[j][u] = ld_batch_cg(pml + at);
-          v[j][u] = ld_batch_cg(reinterpret_cast<const float4 *>(po + at * kDim) + lane);
-        }
-#pragma unroll
-      for (int j = 0; j < PB; ++j)
-#pragma unroll
-        for (int u = 0; u < HW; ++u)
-          acc[u].fold(ml[j][u], v[j][u], i0 + j < count[u]);
-    }
-  };
-  auto for_rows = [&](auto fn) {  // warp w: rows w, w + 4, ..., four at a time
-    for (int r = warp; r < rows; r += 4 * kWarps) {
-      const int left = (rows - r + kWarps - 1) / kWarps;
-      if (left >= 3)
-        fn(std::integral_constant<int, 4>{}, r);
-      else if (left == 2)
-        fn(std::integral_constant<int, 2>{}, r);
-      else
-        fn(std::integral_constant<int, 1>{}, r);
-    }
-  };
-  // rows r, r + 4, ... of request b are complete, but for a prefix: out, or put by until the prefix's results are there
-  auto finish_rows = [&](auto hw, const Row *acc, int r, int b, bool later) {
-    constexpr int HW = decltype(hw)::value;
-#pragma unroll
-    for (int u = 0; u < HW; ++u) {
-      const int row = r + u * kWarps;
-      if (row >= rows) continue;
-      if (!later) {
-        store_row(b, row, acc[u]);
-      } else {
-        const size_t at = (size_t)(p.b0 + b) * a.hq + head0 + row;
-        *(reinterpret_cast<float4 *>(p.prefix.own_o + at * kDim) + lane) = acc[u].o;
-        if (lane == 0) p.prefix.own_ml[at] = make_float2(acc[u].m, acc[u].l);
-      }
-    }
-  };
-  auto has_prefix = [&](int b) { return p.prefix.requests != nullptr && __ldg(&p.prefix.requests[p.b0 + b].x) > 0; };
-  // the prefix partials of request b into acc
-  auto fold_prefix = [&](auto hw, Row *acc, int r, int b) {
-    const int2 rq = __ldg(&p.prefix.requests[p.b0 + b]);
-    const sprefix::Group g = p.prefix.groups[rq.y];
-    const int member = p.b0 + b - g.first;
-    constexpr int HW = decltype(hw)::value;
-    int count[HW];
-#pragma unroll
-    for (int u = 0; u < HW; ++u)
-      count[u] = sprefix::partials_of(g, member * group + min(r + u * kWarps, rows - 1) % group, group, p.prefix.max_splits);
-    fold_rows(hw, acc, r, count, p.prefix.part_o, p.prefix.part_ml,
-              [&](int i, int row) { return ((size_t)i * a.batch + p.b0 + b) * a.hq + head0 + row; });
-  };
-
   for_pieces([&](int b, int lo, int hi, int pages) {
-    const int4 rq = sh_req[b];
-    const int len = rq.y, front = rq.z, second = rq.w;
-    const bool prefix = p.prefix.requests != nullptr;
-    const int low = prefix ? 0 : max(0, len - 1 - a.window_left);
-    const int first = prefix ? 0 : a.first_tokens;
-    if (warp == 0 && lane == 0 && len > 0) {
+    const Visible seen_part = visible_part(p, p.b0 + b);
+    const int len = seen_part.len, front = seen_part.front, second = seen_part.second;
+    const int low = prefixed ? 0 : max(0, len - 1 - a.window_left);
+    const int first = prefixed ? 0 : a.first_tokens;
+    if (hk == 0 && lane == 0 && len > 0) {
       const int last = __ldg(a.kv_last_page_len + p.b0 + b);
       if (last < 1 || last > kPage) report_error(a.err, PIEKV_ERR_LAST_PAGE_LEN, KID_DECODE, p.b0 + b, last);
     }
     // query fragments of this warp's kv head (rows beyond the group are zero)
     uint32_t qa[8][4];
     {
-      const T *qb = reinterpret_cast<const T *>(a.q) + (int64_t)(p.b0 + b) * a.q_sn + (int64_t)(head0 + h * group) * a.q_sh;
+      const T *qb = reinterpret_cast<const T *>(a.q) + (int64_t)(p.b0 + b) * a.q_sn + (int64_t)head0 * a.q_sh;
 #pragma unroll
       for (int ks = 0; ks < 8; ++ks) {
         const int col = ks * 16 + qlane * 2;
@@ -368,9 +303,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
 #pragma unroll
     for (int nt = 0; nt < 16; ++nt) o[nt][0] = o[nt][1] = o[nt][2] = o[nt][3] = 0.f;
     float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
-    int s = 0;
-    for (int v0 = lo; v0 < hi; v0 += PG) {
-      s = it % kStages;
+    for (int vi = lo; vi < hi; ++vi) {
+      const int s = it % kStages;
       bool ok = *(volatile int *)&sh_abort == 0;
       if (ok && !mbar_wait(&full_bar[s], (it / kStages) & 1)) {
         if (lane == 0 && atomicExch(&sh_abort, 1) == 0)
@@ -378,11 +312,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
         ok = false;
       }
       ++it;
-      const int vi = v0 + pslot;
-      if (ok && vi < hi) {
+      if (ok) {
         const int t0 = (vi < front ? vi : vi - front + second) * kPage;
-        const uint32_t page_base = stage0 + s * kStageBytes + pslot * (HB * kTileBytes);
-        const uint32_t ktile = page_base + h * 4096, vtile = page_base + HB * 4096 + h * 4096;
+        const uint32_t ktile = stage0 + s * kStageBytes + warp * 4096, vtile = ktile + HB * 4096;
         // tokens of the page that are seen: below `first` or from `low` on, and inside the context
         uint32_t seen = 0xffffu >> (kPage - min(kPage, len - t0));
         seen &= ((1u << min(max(first - t0, 0), kPage)) - 1u) | (0xffffu << min(max(low - t0, 0), kPage));
@@ -394,7 +326,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
             if (!((seen >> row) & 1u))
               *reinterpret_cast<uint4 *>(vptr + ((x >> 3) & 1) * 2048 + row * 128 + (x & 7) * 16) = make_uint4(0, 0, 0, 0);
           }
-          fence_proxy_async_smem();
+          fence_proxy_async_smem();  // the stage is next written by a bulk copy
           __syncwarp();
         }
         // ---- S = Q K^T
@@ -478,141 +410,177 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
         }
       }
       __syncwarp();
-      // the piece's last stage is kept a little longer: its tiles carry the warps' results below
-      if (lane == 0 && v0 + PG < hi) mbar_arrive(&empty_bar[s]);
+      if (lane == 0) mbar_arrive(&empty_bar[s]);
     }
 
-    // ================= the piece is done: every warp puts its rows over its own tile of the last stage
-    const bool any = lo < hi;
-    if (any) {
-      l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
-      l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
-      l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
-      l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
-      // float2 index within a 512-byte row, XORed with the row so that the eight rows of a store hit different banks
-      uint8_t *kt = stage0_ptr + s * kStageBytes + pslot * (HB * kTileBytes) + h * 4096;
+    // ================= the piece is done: its rows straight from the fragments
+    l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
+    l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
+    l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
+    l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
+    if (!WIDE) {
 #pragma unroll
       for (int nt = 0; nt < 16; ++nt) {
-        const int at = ((nt * 4 + qlane) ^ (quad << 2)) * 8 + quad * 512;
-        if (WIDE) {
-          *reinterpret_cast<float2 *>(kt + at) = make_float2(o[nt][0], o[nt][1]);
-          *reinterpret_cast<float2 *>(kt + HB * 4096 + at) = make_float2(o[nt][2], o[nt][3]);
+        o[nt][0] += o[nt][2];
+        o[nt][1] += o[nt][3];
+      }
+    }
+    const bool whole = lo == 0 && hi == pages;
+    const bool later = has_prefix(b);
+    const int s_first = whole ? c : first_share(b);
+    float *po;  // where partial rows go
+    float2 *pml;
+    if (whole) {
+      const size_t at = (size_t)(p.b0 + b) * a.hq + head0;
+      po = p.prefix.own_o + at * kDim;
+      pml = p.prefix.own_ml + at;
+    } else {
+      const size_t at = slot_base(c, c == s_first);
+      po = p.part_o + at * kDim;
+      pml = p.part_ml + at;
+    }
+#pragma unroll
+    for (int half = 0; half < (WIDE ? 2 : 1); ++half) {
+      const int row = quad + half * 8;
+      if (row < group) {
+        const float m = half ? m1 : m0;
+        float l = half ? l1 : l0;
+        if (whole && !later) {
+          l = add_sink(l, m, a.sinks, head0 + row);
+          const float inv = l > 0.f ? 1.f / l : 0.f;
+          uint32_t *orow = reinterpret_cast<uint32_t *>(out + ((size_t)(p.b0 + b) * a.hq + head0 + row) * kDim);
+#pragma unroll
+          for (int nt = 0; nt < 16; ++nt)
+            orow[nt * 4 + qlane] = pack2<T>(o[nt][half * 2] * inv, o[nt][half * 2 + 1] * inv);
+          if (qlane == 0) store_lse(b, head0 + row, m, l);
         } else {
-          *reinterpret_cast<float2 *>(kt + at) = make_float2(o[nt][0] + o[nt][2], o[nt][1] + o[nt][3]);
+          float4 *prow = reinterpret_cast<float4 *>(po + (size_t)row * kDim) + qlane * 8;
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            prow[i] = make_float4(o[2 * i][half * 2], o[2 * i][half * 2 + 1], o[2 * i + 1][half * 2], o[2 * i + 1][half * 2 + 1]);
+          if (qlane == 0) pml[row] = make_float2(m, l);
         }
       }
-      if (qlane == 0) {
-        sh_ml[warp][quad] = make_float2(m0, l0);
-        if (WIDE) sh_ml[warp][quad + 8] = make_float2(m1, l1);
-      }
     }
-    consumer_sync();
-    const uint8_t *stage = stage0_ptr + s * kStageBytes;
-    auto own_row = [&](int r) {  // this piece's row r: the warps of its head folded
-      Row x;
-      x.clear();
-      if (any) {
-        const int hh = r / group, q = r - hh * group;
-#pragma unroll
-        for (int ps = 0; ps < PG; ++ps)
-          x.fold(sh_ml[ps * HB + hh][q],
-                 *reinterpret_cast<const float4 *>(stage + ps * (HB * kTileBytes) + hh * 4096 + (q >> 3) * (HB * 4096) +
-                                                   (q & 7) * 512 + ((lane * 2) ^ ((q & 7) << 2)) * 8));
-      }
-      return x;
-    };
-    const bool whole = lo == 0 && hi == pages;
-    const int s_first = whole ? c : share_of(sh_cost[b] + kOpenCost);
-    const bool later = has_prefix(b);
-    if (whole) {
-      for_rows([&](auto hw, int r) {
-        constexpr int HW = decltype(hw)::value;
-        Row acc[HW];
-#pragma unroll
-        for (int u = 0; u < HW; ++u) acc[u] = own_row(min(r + u * kWarps, rows - 1));
-        finish_rows(hw, acc, r, b, later);
-      });
-    } else {
-      const size_t base = slot_base(c, c == s_first);
-      for (int r = warp; r < rows; r += kWarps) {
-        const Row x = own_row(r);
-        *(reinterpret_cast<float4 *>(p.part_o + (base + r) * kDim) + lane) = x.o;
-        if (lane == 0) p.part_ml[base + r] = make_float2(x.m, x.l);
-      }
-    }
-    fence_proxy_async_smem();  // these tiles are next written by bulk copies
-    consumer_sync();
-    if (any && lane == 0) mbar_arrive(&empty_bar[s]);
     if (!whole) {
-      // ================= partials: the last share of the request to arrive folds them all
-      const int n = share_of(sh_cost[b + 1] - 1) - s_first + 1;
-      if (tid == 0) {
+      pend_b[c == s_first ? 1 : 0] = b;
+    } else if (later) {
+      if (lane == 0) sh_closed[warp][closed] = (short)b;
+      ++closed;
+    }
+  });
+
+  // ================= joins.  Steps 0 and 1: the requests with a partial in this share's slots, folded by the share that
+  // arrives last.  Then, for what is behind a prefix, the prefix's results with the requests' own: waiting for them only
+  // now keeps the pages streaming while the prefix kernel works.  One loop, so that this code exists once: on a short
+  // call fetching instructions is most of its time.
+#pragma unroll 1
+  for (int x = 0;; ++x) {
+    int b;
+    bool later = false;
+    if (x < 2) {
+      b = x == 0 ? pend_b[0] : pend_b[1];
+      if (b < 0) continue;
+      int is_last = 0;
+      __syncwarp();
+      if (lane == 0) {
         __threadfence();
-        int *counter = p.counters + hb * nb + b;
-        const int old = atomicAdd(counter, 1);
-        sh_last = old + 1 == n ? 1 : 0;
-        if (sh_last) {
+        int *counter = p.counters + hk * nb + b;
+        is_last = atomicAdd(counter, 1) == last_share(b) - first_share(b);
+        if (is_last) {
           *counter = 0;  // nobody else touches it in this launch
           __threadfence();
         }
       }
-      consumer_sync();
-      if (sh_last == 0) return;
-      for_rows([&](auto hw, int r) {
-        constexpr int HW = decltype(hw)::value;
-        Row acc[HW];
-        int count[HW];
+      if (!__shfl_sync(0xffffffffu, is_last, 0)) continue;
+      later = has_prefix(b);
+    } else {
+      if (!prefixed) break;
+      if (x == 2) {  // (also without work: the launch must not end before the one it was allowed to overtake)
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        __syncwarp();
+      }
+      if (x - 2 >= closed) break;
+      b = sh_closed[warp][x - 2];
+    }
+    const size_t request = (size_t)(p.b0 + b) * a.hq + head0;
+    sprefix::Group g{};
+    int n = 0;
+    if (x < 2)
+      n = last_share(b) - first_share(b) + 1;
+    else
+      g = p.prefix.groups[__ldg(&p.prefix.requests[p.b0 + b].y)];
+    // partial i of row r: at + (x < 2 ? max(2 i - 1, 0) : i) * step + r
+    const size_t at = x < 2 ? slot_base(first_share(b), true) : request;
+    const size_t step = x < 2 ? (size_t)a.hq : (size_t)a.batch * a.hq;
+    const float *po = x < 2 ? p.part_o : p.prefix.part_o;
+    const float2 *pml = x < 2 ? p.part_ml : p.prefix.part_ml;
+#pragma unroll 1
+    for (int r0 = 0; r0 < group; r0 += 4) {
+      const int r = min(r0 + (lane >> 3), group - 1), sub = lane & 7;
+      Rows acc;
+      acc.clear();
+      if (x >= 2) {
+        n = sprefix::partials_of(g, (p.b0 + b - g.first) * group + r, group, p.prefix.max_splits);
+        const float2 ml = ld_batch_cg(p.prefix.own_ml + request + r);  // written above by this warp
+        float4 v[4];
 #pragma unroll
-        for (int u = 0; u < HW; ++u) {
-          acc[u].clear();
-          count[u] = n;
+        for (int k = 0; k < 4; ++k)
+          v[k] = ld_batch_cg(reinterpret_cast<const float4 *>(p.prefix.own_o + (request + r) * kDim) + k * 8 + sub);
+        acc.fold(ml, v, true);
+      }
+      const int most = __reduce_max_sync(0xffffffffu, n);
+#pragma unroll 1
+      for (int i0 = 0; i0 < most; i0 += 4) {
+        float2 ml[4];
+        float4 v[4][4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int i = max(min(i0 + j, n - 1), 0);
+          const size_t row = at + (size_t)(x < 2 ? max(2 * i - 1, 0) : i) * step + r;
+          ml[j] = ld_batch_cg(pml + row);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) v[j][k] = ld_batch_cg(reinterpret_cast<const float4 *>(po + row * kDim) + k * 8 + sub);
         }
-        fold_rows(hw, acc, r, count, p.part_o, p.part_ml, [&](int i, int row) { return slot_base(s_first + i, i == 0) + row; });
-        finish_rows(hw, acc, r, b, later);
-      });
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc.fold(ml[j], v[j], i0 + j < n);
+      }
+      if (r0 + (lane >> 3) < group) {
+        if (later) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) *(reinterpret_cast<float4 *>(p.prefix.own_o + (request + r) * kDim) + k * 8 + sub) = acc.o[k];
+          if (sub == 0) p.prefix.own_ml[request + r] = make_float2(acc.m, acc.l);
+        } else {
+          const float l = add_sink(acc.l, acc.m, a.sinks, head0 + r);
+          const float inv = l > 0.f ? 1.f / l : 0.f;
+          // fragment order: o[k] holds columns 16 sub + 2 k + {0, 1} and 16 sub + 8 + 2 k + {0, 1}
+          uint32_t *row = reinterpret_cast<uint32_t *>(out + (request + r) * kDim) + sub * 8;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            row[k] = pack2<T>(acc.o[k].x * inv, acc.o[k].y * inv);
+            row[4 + k] = pack2<T>(acc.o[k].z * inv, acc.o[k].w * inv);
+          }
+          if (sub == 0) store_lse(b, head0 + r, acc.m, l);
+        }
+      }
     }
     if (later) {
-      if (tid == 0) sh_closed[closed] = (short)b;
+      if (lane == 0) sh_closed[warp][closed] = (short)b;
       ++closed;
     }
-  });
-  if (p.prefix.requests == nullptr) return;
-  // ================= the prefix's results, folded with the requests' own.  Waiting only now keeps the pages streaming
-  // while the prefix kernel works; the launch must not end before that kernel in any case.
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  consumer_sync();
-  for (int x = 0; x < closed; ++x) {
-    const int b = sh_closed[x];
-    for_rows([&](auto hw, int r) {
-      constexpr int HW = decltype(hw)::value;
-      Row acc[HW];
-      float2 ml[HW];
-#pragma unroll
-      for (int u = 0; u < HW; ++u) {  // written above by this very warp
-        const size_t at = (size_t)(p.b0 + b) * a.hq + head0 + min(r + u * kWarps, rows - 1);
-        ml[u] = ld_batch_cg(p.prefix.own_ml + at);
-        acc[u].o = ld_batch_cg(reinterpret_cast<const float4 *>(p.prefix.own_o + at * kDim) + lane);
-      }
-#pragma unroll
-      for (int u = 0; u < HW; ++u) {
-        acc[u].m = ml[u].x;
-        acc[u].l = ml[u].y;
-      }
-      fold_prefix(hw, acc, r, b);
-      finish_rows(hw, acc, r, b, false);
-    });
   }
 }
 
 template <typename T, int HB, bool WIDE>
 int launch_t(const CUtensorMap &tm, const SpanParams &p, cudaStream_t st) {
   static unsigned char configured[kMaxDevices] = {0};
-  if (int rc = opt_in_dynamic_smem(decode_span_kernel<T, HB, WIDE>, kSmemBytes, configured, "decode span: cudaFuncSetAttribute"))
+  if (int rc = opt_in_dynamic_smem(decode_span_kernel<T, HB, WIDE>, Shape<HB>::kSmemBytes, configured,
+                                   "decode span: cudaFuncSetAttribute"))
     return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(p.n_hb * p.ctas));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = kSmemBytes;
+  cfg.blockDim = dim3(Shape<HB>::kThreads);
+  cfg.dynamicSmemBytes = Shape<HB>::kSmemBytes;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -627,14 +595,15 @@ int launch_t(const CUtensorMap &tm, const SpanParams &p, cudaStream_t st) {
 
 template <typename T>
 int launch_h(int heads, bool wide, const CUtensorMap &tm, const SpanParams &p, cudaStream_t st) {
-  if (heads == 4) return wide ? launch_t<T, 4, true>(tm, p, st) : launch_t<T, 4, false>(tm, p, st);
   if (heads == 2) return wide ? launch_t<T, 2, true>(tm, p, st) : launch_t<T, 2, false>(tm, p, st);
   return wide ? launch_t<T, 1, true>(tm, p, st) : launch_t<T, 1, false>(tm, p, st);
 }
 
-int heads_per_cta(int hkv) { return hkv % 4 == 0 ? 4 : (hkv % 2 == 0 ? 2 : 1); }
-int ctas_per_head_block(int hkv) {
-  const int n = kCtasPerSm * sm_count() / (hkv / heads_per_cta(hkv));
+int heads_per_cta(int hkv) { return hkv % 2 == 0 ? 2 : 1; }
+// shares of the line: CTAs of one head block
+int shares_of(int hkv) {
+  const int heads = heads_per_cta(hkv);
+  const int n = (heads == 2 ? Shape<2>::kCtasPerSm : Shape<1>::kCtasPerSm) * sm_count() / (hkv / heads);
   return n > 1 ? n : 1;
 }
 
@@ -644,16 +613,16 @@ bool decode_span_supported(const AttnArgs &a, int dtype) {
   if (dtype != PIEKV_BF16 && dtype != PIEKV_F16) return false;
   if (a.dim != kDim || a.page_size != kPage) return false;
   if (a.hq % a.hkv != 0 || a.hq / a.hkv > 16) return false;
-  if (a.hkv / heads_per_cta(a.hkv) > kCounterBytes / 4) return false;
+  if (a.hkv > kCounterBytes / 4) return false;
   if ((reinterpret_cast<uintptr_t>(a.pool) & 15) || (reinterpret_cast<uintptr_t>(a.q) & 3) ||
-      (reinterpret_cast<uintptr_t>(a.out) & 7))
+      (reinterpret_cast<uintptr_t>(a.out) & 3))
     return false;
   return !((a.q_sn & 1) || (a.q_sh & 1));
 }
 
-// Partials of a launch: two slots per CTA, one row per query head of its head block.
+// Partials of a launch: two slots per share of the line, one row per query head.
 int64_t decode_span_scratch_bytes(int hq, int hkv) {
-  const int64_t rows = 2ll * ctas_per_head_block(hkv) * hq;
+  const int64_t rows = 2ll * shares_of(hkv) * hq;
   return (rows * 8 + 255) / 256 * 256 + rows * kDim * 4;
 }
 
@@ -668,7 +637,7 @@ int launch_decode_span(const AttnArgs &a, int dtype, const SpanPrefix &prefix, v
   p.a = a;
   p.prefix = prefix;
   p.n_hb = a.hkv / heads;
-  p.ctas = ctas_per_head_block(a.hkv);
+  p.ctas = shares_of(a.hkv);
   p.sms = sm_count();
   uint8_t *ws = reinterpret_cast<uint8_t *>(workspace);
   p.counters = reinterpret_cast<int *>(ws);
@@ -679,7 +648,7 @@ int launch_decode_span(const AttnArgs &a, int dtype, const SpanPrefix &prefix, v
   if (int rc = make_page_tensor_map(&tm, a.pool, a.num_pages, a.hkv, dtype, /*box_halves=*/2, /*box_heads=*/heads,
                                     /*box_kv=*/2))
     return rc;
-  const int most = kCounterBytes / 4 / p.n_hb;
+  const int most = kCounterBytes / 4 / a.hkv;
   const int slice = most < kMaxSlice ? most : kMaxSlice;
   for (int b0 = 0; b0 < a.batch; b0 += slice) {
     p.b0 = b0;

@@ -419,8 +419,14 @@ __global__ void __launch_bounds__(kPxThreads, 1)
         tc::tmem_ld32(o_addr + ch * 32, oreg);
         tc::tmem_wait_ld();
         if (row_valid) {
+          // fragment order (decode_span.cu): element nt * 8 + 2 * q + e at q * 32 + nt * 2 + e, a sector per q
 #pragma unroll
-          for (int e = 0; e < 4; ++e) store_v8(p.part_o + at * kDim + ch * 32 + e * 8, oreg + e * 8);
+          for (int q = 0; q < 4; ++q) {
+            uint32_t v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = oreg[(e >> 1) * 8 + q * 2 + (e & 1)];
+            store_v8(p.part_o + at * kDim + q * 32 + ch * 8, v);
+          }
         }
       }
       if (row_valid) p.part_ml[at] = make_float2(m_ref, l);
