@@ -497,81 +497,98 @@ class AxisRopeConfig(RopeConfig):
 
 
 def _device_rows(t: torch.Tensor, name: str, device: int) -> Tuple[int, int]:
-    """_rows() of a tensor that has to be on CUDA device `device` (-1 for a tensor elsewhere)."""
-    if t.get_device() != device or not t.is_cuda:
+    """_rows() of a tensor that has to be on CUDA device `device`."""
+    if t.get_device() != device:
         raise ValueError(f"{name} must be a CUDA tensor on cuda:{device}, got {t.device}")
-    shape, stride = t.shape, t.stride()
-    if len(shape) != 3:
-        raise ValueError(f"{name} must be [tokens, heads, head_dim], got shape {tuple(shape)}")
-    if shape[2] > 1 and stride[2] != 1:
+    stride = t.stride()
+    if len(stride) != 3:
+        raise ValueError(f"{name} must be [tokens, heads, head_dim], got shape {tuple(t.shape)}")
+    if stride[2] != 1 and t.shape[2] > 1:
         raise ValueError(f"{name}: head_dim axis must be contiguous")
     return stride[0], stride[1]
 
 
 def _device_i32(t: torch.Tensor, name: str, device: int) -> int:
-    if t.dtype != torch.int32 or t.get_device() != device or not t.is_cuda or not t.is_contiguous():
+    if t.dtype is not torch.int32 or t.get_device() != device or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int32 CUDA tensor on cuda:{device}, got {t.dtype} on {t.device}")
     return t.data_ptr()
 
 
+_ERR_PTRS: dict = {}
+
+
+def _err_ptr(index: int) -> int:
+    """Address of the error word of a device."""
+    ptr = _ERR_PTRS.get(index)
+    if ptr is None:
+        ptr = _ERR_PTRS[index] = _err_word(torch.device("cuda", index)).data_ptr()
+    return ptr
+
+
 def _rope_axes(q, k, v, pos_ids, rope: AxisRopeConfig, q_out, k_out, who: str, append=None) -> None:
+    # (a decode step's call is as short as its checks: each tensor is asked for each property once)
     if not isinstance(rope, AxisRopeConfig):
         raise ValueError(f"{who}: rope must be an AxisRopeConfig")
-    _require_cuda(k, "k")
-    _require_cuda(pos_ids, "pos_ids")
+    for t, name in ((k, "k"), (pos_ids, "pos_ids")):
+        if not isinstance(t, torch.Tensor) or not t.is_cuda:
+            _require_cuda(t, name)
     table = rope.prepared()
     device = k.get_device()
     k_rows = _device_rows(k, "k", device)
     n, hkv, d = shape = k.shape
     dtype = k.dtype
-    if pos_ids.dtype != torch.int32 or pos_ids.dim() != 2 or pos_ids.shape[0] != table.num_axes or \
-            pos_ids.shape[1] < n or (n > 1 and pos_ids.stride(1) != 1):
+    pos_shape, pos_stride = pos_ids.shape, pos_ids.stride()
+    if pos_ids.dtype is not torch.int32 or len(pos_shape) != 2 or pos_shape[0] != table.num_axes or pos_shape[1] < n or \
+            (n > 1 and pos_stride[1] != 1):
         raise ValueError(f"{who}: pos_ids must be int32 [{table.num_axes} axes, {n} tokens] with contiguous rows, got "
-                         f"{tuple(pos_ids.shape)} {pos_ids.dtype}")
+                         f"{tuple(pos_shape)} {pos_ids.dtype}")
     if pos_ids.get_device() != device:
         raise ValueError(f"{who}: pos_ids is on {pos_ids.device}, k on {k.device}")
     if 2 * table.half > d:
         raise ValueError(f"{who}: sections of {table.half} pairs do not fit head_dim {d}")
     if rope.mode == "table" and rope.cos_sin_table.get_device() != device:
         raise ValueError(f"{who}: cos_sin_table on {rope.cos_sin_table.device}, k on {k.device}")
-    q_ptr = qo_ptr = ko_ptr = None
+    q_ptr = qo_ptr = ko_ptr = v_ptr = None
     q_rows = qo_rows = ko_rows = v_rows = (0, 0)
     hq = 0
     if q is not None:
-        _require_cuda(q, "q")
         q_rows = _device_rows(q, "q", device)
-        if q.shape[0] != n or q.shape[2] != d or q.dtype != dtype:
-            raise ValueError(f"{who}: q {tuple(q.shape)} {q.dtype} does not match k {tuple(shape)} {dtype}")
-        hq, q_ptr = q.shape[1], q.data_ptr()
+        q_shape = q.shape
+        if q_shape[0] != n or q_shape[2] != d or q.dtype is not dtype:
+            raise ValueError(f"{who}: q {tuple(q_shape)} {q.dtype} does not match k {tuple(shape)} {dtype}")
+        hq, q_ptr = q_shape[1], q.data_ptr()
         if q_out is q:
             qo_rows, qo_ptr = q_rows, q_ptr
         else:
-            if q_out.shape != q.shape or q_out.dtype != dtype:
+            if q_out.shape != q_shape or q_out.dtype is not dtype:
                 raise ValueError(f"{who}: q_out must be shaped and typed like q")
             qo_rows, qo_ptr = _device_rows(q_out, "q_out", device), q_out.data_ptr()
     if k_out is not None:
         ko_rows, ko_ptr = _device_rows(k_out, "k_out", device), k_out.data_ptr()
     tail = (None, None, None, None, None)
-    v_ptr, batch, page_size, num_pages = None, 0, 0, 0
+    batch = page_size = num_pages = 0
     if append is not None:
         batch_indices, positions, pool, kv_indices, kv_indptr = append
-        _require_cuda(v, "v")
+        if not isinstance(v, torch.Tensor):
+            _require_cuda(v, "v")
         v_rows, v_ptr = _device_rows(v, "v", device), v.data_ptr()
-        num_pages, page_size, pool_heads, pool_dim = _check_pool(pool)
+        if isinstance(pool, (tuple, list)) or pool.get_device() != device or len(pool.shape) != 5 or pool.shape[1] != 2 or \
+                not pool.is_contiguous():
+            _check_pool(pool)
+            raise ValueError(f"{who}: the cache is on {pool.device}, k on {k.device}")
+        num_pages, _, page_size, pool_heads, pool_dim = pool.shape
         if hkv != pool_heads or d != pool_dim or v.shape != shape:
             raise ValueError(f"{who}: key {tuple(shape)} / value {tuple(v.shape)} do not match the cache "
                              f"[*, {pool_heads}, {pool_dim}]")
-        if dtype != pool.dtype or v.dtype != dtype:
+        if dtype is not pool.dtype or v.dtype is not dtype:
             raise ValueError(f"{who}: key/value dtype {dtype}/{v.dtype} differs from the cache dtype {pool.dtype}")
-        if pool.get_device() != device:
-            raise ValueError(f"{who}: the cache is on {pool.device}, k on {k.device}")
         tail = (_device_i32(batch_indices, "batch_indices", device), _device_i32(positions, "positions", device),
                 pool.data_ptr(), _device_i32(kv_indices, "kv_indices", device), _device_i32(kv_indptr, "kv_indptr", device))
-        if batch_indices.shape[0] < n or positions.shape[0] < n:
+        if batch_indices.numel() < n or positions.numel() < n:
             raise ValueError(f"{who}: batch_indices / positions shorter than the number of tokens")
-        batch = kv_indptr.shape[0] - 1
+        batch = kv_indptr.numel() - 1
     args = _lib.RopeAxesArgs(q_ptr, k.data_ptr(), v_ptr, qo_ptr, ko_ptr, *q_rows, *k_rows, *v_rows, *qo_rows, *ko_rows,
-                             pos_ids.data_ptr(), pos_ids.stride(0), *tail, _err_word(k.device).data_ptr(), n, batch, hq, hkv,
+                             pos_ids.data_ptr(), pos_stride[0], *tail, _err_ptr(device), n, batch, hq, hkv,
                              d, page_size, num_pages, _dtype_code(dtype, who))
     status = lib.piekv_rope_axes(args, table, _stream_of(device))
     if status:
