@@ -52,6 +52,7 @@ struct PrefillParams {
   const uint4 *packed;
   int sw;
   int has_mask;
+  int tokens;              // two-problem kernel with a band: query tokens per 128-row tile (all heads of a kv head)
 };
 
 // bounded wait that also gives up when another role has already aborted
@@ -124,6 +125,51 @@ __device__ __forceinline__ bool band_unseen_v_rows(const Band &w, int kv_len, in
     } else {
       a = kv_len;
       e = (kv_len + kPage - 1) / kPage * kPage;
+    }
+    a = max(a - t0, 0);
+    e = min(e - t0, kBN);
+    if (a < e) {
+      any = true;
+      if (zero) zero_v_rows(v_tile_smem, a, e, lane);
+    }
+  }
+  return any;
+}
+
+// The keys an item of the two-problem kernel streams, as a list of pages without the ones nobody sees: pages
+// [0, front) and [low_page, ...) of the request, `pages` in all.  Slot s of the list is key s, behind the first
+// tokens' pages key s + shift.
+struct VisibleKeys {
+  int first, low;       // keys [0, first) and [low, ...) are seen by some row
+  int front, low_page, pages, shift;
+};
+__device__ __forceinline__ VisibleKeys visible_keys(const AttnArgs &a, int kv_len, int pos_first, int hi) {
+  VisibleKeys w;
+  w.first = max(0, min(a.first_tokens, hi));
+  w.low = max(0, pos_first - a.window_left);
+  w.front = (w.first + kPage - 1) / kPage;
+  w.low_page = max(w.front, w.low / kPage);
+  w.pages = hi > 0 ? w.front + max(0, (hi + kPage - 1) / kPage - w.low_page) : 0;
+  w.shift = (w.low_page - w.front) * kPage;
+  return w;
+}
+// Slots of loaded pages that no row sees, as up to three ranges: behind the first tokens, before the window, behind the
+// context.  Tells whether tile j has any; with `zero` it clears their V rows.
+__device__ __forceinline__ bool unseen_v_rows(const VisibleKeys &w, int kv_len, int j, uint32_t v_tile_smem, int lane, bool zero) {
+  const int t0 = j * kBN, low = w.low - w.shift, len = kv_len - w.shift;
+  bool any = false;
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+    int a, e;
+    if (i == 0) {
+      a = w.first;
+      e = min(w.front * kPage, low);
+    } else if (i == 1) {
+      a = max(low / kPage * kPage, w.first);
+      e = low;
+    } else {
+      a = len;
+      e = (len + kPage - 1) / kPage * kPage;
     }
     a = max(a - t0, 0);
     e = min(e - t0, kBN);

@@ -12,9 +12,9 @@ namespace piekv {
 int make_page_tensor_map(CUtensorMap *tm, const void *pool, int num_pages, int hkv, int dtype, int box_halves,
                          int box_heads, int box_kv);
 
-// q [n, Hq, 128] (strides in elements) seen as {64 d, n tokens, 2 d-halves, Hq}; box {64, rows, 2, heads}.
+// q [n, Hq, 128] (strides in elements) seen as {64 d, n tokens, 2 d-halves, Hq}; box {64, rows, halves, heads}.
 int make_q_tensor_map(CUtensorMap *tm, const void *q, int64_t nnz, int hq, int64_t q_sn, int64_t q_sh, int dtype,
-                      int box_rows, int box_heads = 1);
+                      int box_rows, int box_heads = 1, int box_halves = 2);
 
 // Row-major matrix [rows, cols] of 16-bit elements (row stride in elements) seen as {cols, rows}; box
 // {box_cols (64: one 128-byte swizzled row), box_rows}: shared memory receives [box_rows][64], K-major.

@@ -219,7 +219,7 @@ def test_decode_bad_pages_are_reported():
 # ---- prefill
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
-@pytest.mark.parametrize("hq, hkv", [(8, 2), (4, 4), (6, 2), (2, 1), (5, 1)])
+@pytest.mark.parametrize("hq, hkv", [(8, 2), (4, 4), (6, 2), (2, 1), (5, 1), (6, 1), (16, 2), (10, 1), (16, 1), (20, 1)])
 @pytest.mark.parametrize("window, first", [(63, 4), (0, 1), (200, 130), (15, 300)])
 def test_prefill(dtype, hq, hkv, window, first):
     sc = make_scenario(hq, hkv, 128, dtype, [(0, 1), (0, 17), (5, 128), (700, 129), (300, 1), (511, 256), (40, 0), (1000, 3)],
