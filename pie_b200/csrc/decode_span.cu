@@ -47,7 +47,7 @@ constexpr int kPage = 16;
 constexpr int kTileBytes = 8192;  // one (page, head): K 4 KiB + V 4 KiB
 constexpr int kCounterBytes = 65536;
 constexpr int kMaxSlice = 512;   // requests per launch: the line is kept in shared memory
-constexpr int kOpenCost = 2;     // pages
+constexpr int kOpenCost = 4;     // pages
 constexpr int kMinUnits = 4;     // a share is not made smaller than this
 
 // Launch shape for HB heads per CTA: 12 warps per SM (168 registers each) and 24 tiles in flight.
@@ -521,7 +521,8 @@ __global__ void __launch_bounds__(Shape<HB>::kThreads, Shape<HB>::kCtasPerSm)
       Rows acc;
       acc.clear();
       if (x >= 2) {
-        n = sprefix::partials_of(g, (p.b0 + b - g.first) * group + r, group, p.prefix.max_splits);
+        const int block = ((p.b0 + b - g.first) * group + r) / sprefix::kRowsPerBlock;
+        n = sprefix::partials_of(p.prefix.segments[g.segment + block * a.hkv + hk], p.prefix.max_splits);
         const float2 ml = ld_batch_cg(p.prefix.own_ml + request + r);  // written above by this warp
         float4 v[4];
 #pragma unroll

@@ -9,6 +9,7 @@ namespace piekv {
 struct SpanPrefix {
   const int2 *requests = nullptr;  // [batch] (pages read with the group, group); nullptr: no prefix
   const sprefix::Group *groups = nullptr;
+  const sprefix::Segment *segments = nullptr;
   const int *header = nullptr;     // the plan's
   const float *part_o = nullptr;   // [split][batch][Hq][128]
   const float2 *part_ml = nullptr;

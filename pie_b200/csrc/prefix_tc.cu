@@ -1,11 +1,11 @@
 // Attention of many requests to the pages they share, on the sm_100a tensor cores (tcgen05 / TMEM).
 //
 // The query rows of a group and kv head are packed, row = request * (heads per kv head) + head, so a prefix is read
-// once for all of them: an item is (group, kv head, block of 256 rows, chunk of the prefix).  Two 128-row problems "A"
-// and "B" run against each other on one SM - while the softmax warps of one work on its scores, the tensor pipe runs
+// once for all of them.  A segment is (group, kv head, block of 256 rows); CTAs have equal shares of all segments' tiles
+// (the plan, shared_prefix.cu) and work through the pieces of segments in theirs.  Two 128-row problems "A" and "B" run against each other on one SM - while the softmax warps of one work on its scores, the tensor pipe runs
 // the other's MMAs:
 //   more than 128 rows    A and B are the two halves of the block and share every K and V tile
-//   at most 128 rows      A and B are the same rows over the two halves of the chunk
+//   at most 128 rows      A and B are the same rows over the two halves of the piece
 // Every problem leaves a partial result (m, l, O) per row, unnormalised and in fp32, for the kernel that folds it with
 // the request's own pages (decode_span.cu): M = max m_i, L = sum l_i 2^(m_i - M), O = sum O_i 2^(m_i - M).
 //
@@ -46,47 +46,59 @@ constexpr int kPxRegsLaunch = 168, kPxRegsSoftmax = 200, kPxRegsOther = 96;
 static_assert(256 * kPxRegsSoftmax + 128 * kPxRegsOther <= kPxThreads * kPxRegsLaunch, "registers the CTA owns");
 constexpr int kPxSmemBytes = kTileBytes * (2 + kKStages + kVStages) + 1024;
 constexpr int kPxVWarp = kMmaWarp + 1;
-static_assert(kTileTokens == kBN && kRowsPerItem == 2 * kBM, "plan and kernel cut the work alike");
+static_assert(kTileTokens == kBN && kRowsPerBlock == 2 * kBM, "plan and kernel cut the work alike");
+static_assert(sizeof(Segment) == 32, "a segment is read as two vectors");
 
-// An item as every role reads it off the plan.
+// A piece of a segment as every role reads it off the plan.
 struct Work {
-  int first, p0, pages;        // the group's first request, its page list, pages of the prefix
+  int request, list, pages;    // the group's first request, its page list, pages of the prefix
   int kv_head, row0;
   int rows[2];                 // rows of A and B
   int n[2], t0[2], split[2];   // tiles, first tile and partial index of A and B
   bool pair;                   // A and B share their tiles
 };
-__device__ __forceinline__ Work work_of(const PrefixTcParams &p, int i) {
-  const Item it = p.items[i];
-  const Group g = p.groups[it.group];
+__device__ __forceinline__ int4 ld_int4(const void *p) { return __ldg(reinterpret_cast<const int4 *>(p)); }
+// tiles [t0, t1) of segment `seg`, by CTA `cta`; t1 < 0: to its end
+__device__ __forceinline__ Work work_of(const PrefixTcParams &p, int cta, int seg, int t0, int t1) {
+  const int4 a = ld_int4(p.segments + seg), b = ld_int4(reinterpret_cast<const int4 *>(p.segments + seg) + 1);
+  Segment s;
+  s.request = a.x, s.list = a.y, s.pages = a.z, s.kv_head = a.w;
+  s.row0 = b.x, s.rows = b.y, s.first_cta = b.z, s.pieces = b.w;
   Work w;
-  w.first = g.first;
-  w.p0 = __ldg(p.kv_indptr + g.first);
-  w.pages = min(g.pages, __ldg(p.kv_indptr + g.first + 1) - w.p0);
-  w.kv_head = it.kv_head;
-  w.row0 = it.row_block * kRowsPerItem;
-  const int left = g.members * p.group - w.row0;
-  const int tiles = (g.pages * kPage + kBN - 1) / kBN;
-  const int t0 = (int)((long long)tiles * it.chunk / g.chunks), t1 = (int)((long long)tiles * (it.chunk + 1) / g.chunks);
-  w.pair = left > kBM;
+  w.request = s.request;
+  w.list = s.list;
+  w.pages = s.pages;
+  w.kv_head = s.kv_head;
+  w.row0 = s.row0;
+  if (t1 < 0) t1 = (s.pages * kPage + kBN - 1) / kBN;
+  const int piece = s.pieces > 1 ? cta - s.first_cta : 0;
+  w.pair = s.rows > kBM;
   w.t0[0] = t0;
   if (w.pair) {
     w.rows[0] = kBM;
-    w.rows[1] = min(kBM, left - kBM);
+    w.rows[1] = min(kBM, s.rows - kBM);
     w.n[0] = w.n[1] = t1 - t0;
     w.t0[1] = t0;
-    w.split[0] = w.split[1] = it.chunk;
+    w.split[0] = w.split[1] = piece;
   } else {
     const bool two = p.max_splits >= 2;
-    w.rows[0] = w.rows[1] = left;
+    w.rows[0] = w.rows[1] = s.rows;
     w.n[0] = two ? (t1 - t0 + 1) / 2 : t1 - t0;
     w.n[1] = t1 - t0 - w.n[0];
     w.t0[1] = t0 + w.n[0];
-    w.split[0] = two ? 2 * it.chunk : it.chunk;
-    w.split[1] = 2 * it.chunk + 1;
+    w.split[0] = two ? 2 * piece : piece;
+    w.split[1] = 2 * piece + 1;
     if (!two) w.rows[1] = 0;
   }
   return w;
+}
+// the pieces of a CTA's share in order: fn(piece) until it returns false
+template <typename F>
+__device__ __forceinline__ void for_pieces(const PrefixTcParams &p, int cta, F fn) {
+  const int2 from = __ldg(p.starts + cta), to = __ldg(p.starts + cta + 1);
+#pragma unroll 1
+  for (int seg = from.x; seg < to.x || (seg == to.x && to.y > 0); ++seg)
+    if (!fn(work_of(p, cta, seg, seg == from.x ? from.y : 0, seg == to.x ? to.y : -1))) return;
 }
 
 __device__ __forceinline__ void store_v8(float *dst, const uint32_t *r) {
@@ -106,8 +118,7 @@ __global__ void __launch_bounds__(kPxThreads, 1)
 
   // The kernel behind this one reads its own pages first and waits for these results only then.
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int items = __ldg(p.header), ctas = __ldg(p.header + 2);
-  if ((int)blockIdx.x >= ctas) return;
+  if ((int)blockIdx.x >= __ldg(p.header)) return;
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -161,8 +172,7 @@ __global__ void __launch_bounds__(kPxThreads, 1)
       uint64_t *full = is_v ? v_full : k_full, *empty = is_v ? v_empty : k_empty;
       int armed = 0;
       bool ok = true;
-      for (int i = blockIdx.x; ok && i < items; i += ctas) {
-        const Work w = work_of(p, i);
+      for_pieces(p, blockIdx.x, [&](const Work &w) {
         for (int t = 0; ok && t < w.n[0]; ++t)
           for (int x = 0; x < (w.pair ? 1 : 2); ++x) {
             if (t >= w.n[x]) continue;
@@ -174,9 +184,9 @@ __global__ void __launch_bounds__(kPxThreads, 1)
             }
             const int pi = (w.t0[x] + t) * 8 + lane;
             const bool wanted = lane < 8 && pi < w.pages;
-            int page = wanted ? __ldg(p.kv_indices + w.p0 + pi) : p.num_pages;
+            int page = wanted ? __ldg(p.kv_indices + w.list + pi) : p.num_pages;
             if (wanted && (page < 0 || page >= p.num_pages)) {
-              report_error(p.err, PIEKV_ERR_PAGE_ID, KID_SHARED_PREFIX, w.p0 + pi, page);
+              report_error(p.err, PIEKV_ERR_PAGE_ID, KID_SHARED_PREFIX, w.list + pi, page);
               page = p.num_pages;  // outside the tensor map: zeros, as behind the prefix
             }
             if (lane == 0) mbar_arrive_expect_tx(&full[st], kTileBytes);
@@ -188,7 +198,8 @@ __global__ void __launch_bounds__(kPxThreads, 1)
             }
             ++armed;
           }
-      }
+        return ok;
+      });
       // drain: the CTA must not retire while a bulk copy may still be landing
       __syncwarp();
       if (lane == 0)
@@ -232,29 +243,27 @@ __global__ void __launch_bounds__(kPxThreads, 1)
           return true;
         };
         bool ok = true;
-        int qi = 0;
-        for (int i = blockIdx.x; ok && i < items; i += ctas, ++qi) {
-          const Work w = work_of(p, i);
+        int qi[2] = {0, 0};  // query tiles of A and B taken so far: phases of q_full
+        for_pieces(p, blockIdx.x, [&](const Work &w) {
           const int na = w.n[0], nb = w.n[1];
-          ok = wait(&q_full[0], qi) && wait_k();
-          if (!ok) break;
+          ok = wait(&q_full[0], qi[0]++) && wait_k();
+          if (!ok) return false;
           scores(0);
           if (!w.pair) release_k();
-          ok = wait(&q_full[1], qi);  // (also without tiles of B: its phase has to be passed)
-          if (!ok) break;
           if (nb > 0) {
-            ok = wait_k();
-            if (!ok) break;
+            ok = wait(&q_full[1], qi[1]++) && wait_k();
+            if (!ok) return false;
             scores(1);
             release_k();
           }
-          for (int t = 0; ok && t < na; ++t) {
+#pragma unroll 1
+          for (int t = 0; t < na; ++t) {
             ok = wait_v() && pv(0, t > 0);
-            if (!ok) break;
+            if (!ok) return false;
             if (!w.pair) release_v();
             if (t + 1 < na) {
               ok = wait_k();
-              if (!ok) break;
+              if (!ok) return false;
               scores(0);
               if (!w.pair) release_k();
             } else {
@@ -262,18 +271,19 @@ __global__ void __launch_bounds__(kPxThreads, 1)
             }
             if (t >= nb) continue;
             ok = wait_v() && pv(1, t > 0);
-            if (!ok) break;
+            if (!ok) return false;
             release_v();
             if (t + 1 < nb) {
               ok = wait_k();
-              if (!ok) break;
+              if (!ok) return false;
               scores(1);
               release_k();
             } else {
               tc::commit(&o_done[1]);
             }
           }
-        }
+          return true;
+        });
         if (!ok) give_up(200);
       }
     }
@@ -290,14 +300,17 @@ __global__ void __launch_bounds__(kPxThreads, 1)
     int sc = 0, oc = 0;  // score tiles and items (with tiles) finished: phases of s_full and o_done
     bool ok = true;
 
-    for (int i = blockIdx.x; ok && i < items; i += ctas) {
-      const Work w = work_of(p, i);
+    for_pieces(p, blockIdx.x, [&](const Work &w) {
       const int rows = w.rows[x], n = w.n[x];
       const bool row_valid = row < rows;
       const bool warp_valid = q4 * 32 < rows;
       const int r = w.row0 + (w.pair ? x * kBM : 0) + row;  // row of the group
       const int member = r / p.group, g = r - member * p.group;
-      const int request = w.first + member, head = w.kv_head * p.group + g;
+      const int request = w.request + member, head = w.kv_head * p.group + g;
+      if (n == 0) {  // (nothing is announced for it: the barriers' phases count pieces with tiles)
+        if (row_valid) p.part_ml[((size_t)w.split[x] * p.batch + request) * p.hq + head] = make_float2(-INFINITY, 0.f);
+        return true;
+      }
       // ---- the query row into shared memory: K-major, 128-byte swizzle.  Every MMA that read the last item's is done:
       // this warp has seen the scores of all its tiles.
       if (warp_valid) {
@@ -314,13 +327,6 @@ __global__ void __launch_bounds__(kPxThreads, 1)
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&q_full[x]);
-      if (n == 0) {
-        if (row_valid && rows > 0) {
-          const size_t at = ((size_t)w.split[x] * p.batch + request) * p.hq + head;
-          p.part_ml[at] = make_float2(-INFINITY, 0.f);
-        }
-        continue;
-      }
       const int limit = w.pages * kPage - 1;
       float m_ref = -INFINITY, l = 0.f;
       for (int t = 0; t < n; ++t) {
@@ -408,9 +414,9 @@ __global__ void __launch_bounds__(kPxThreads, 1)
       // ---- the partial result.  The next item's O_x is not written before this warp has delivered that item's first
       // probabilities.
       if (ok) ok = wait_or_abort(&o_done[x], oc & 1, abort_flag);
-      if (!ok) break;
+      if (!ok) return false;
       ++oc;
-      if (!warp_valid) continue;
+      if (!warp_valid) return true;
       tc::fence_after_sync();
       const size_t at = ((size_t)w.split[x] * p.batch + request) * p.hq + head;
 #pragma unroll 1
@@ -430,7 +436,8 @@ __global__ void __launch_bounds__(kPxThreads, 1)
         }
       }
       if (row_valid) p.part_ml[at] = make_float2(m_ref, l);
-    }
+      return true;
+    });
     if (!ok) give_up(300 + warp);
   }
 

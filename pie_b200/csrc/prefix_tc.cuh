@@ -7,10 +7,10 @@ namespace piekv {
 struct PrefixTcParams {
   const void *q;  // [batch, Hq, 128], rows 16-byte aligned
   int64_t q_sn, q_sh;
-  const int32_t *kv_indptr, *kv_indices;
+  const int32_t *kv_indices;
   const int *header;  // the plan's
-  const sprefix::Group *groups;
-  const sprefix::Item *items;
+  const int2 *starts;
+  const sprefix::Segment *segments;
   float *part_o;    // [split][batch][Hq][128], unnormalised
   float2 *part_ml;  // [split][batch][Hq]: reference maximum (log2 units), sum
   int batch, hq, group, num_pages, max_splits;

@@ -60,31 +60,32 @@ __global__ void __launch_bounds__(128) sp_match_kernel(const int32_t *__restrict
   if (threadIdx.x == 0) match[b] = sh_first;
 }
 
-// Times in units of one kv tile (64 KiB of K and V, the time an SM needs to stream them: 1.45 us), as measured on the
-// two attention kernels: starting a prefix CTA, an item's own costs (query rows in, partial rows out), a tile against
-// more than 128 rows (bound by the tensor and special-function pipes) or fewer (by the stream), starting the other
-// kernel, and one row of partial results written and folded.
-constexpr float kStartPrefix = 4.f, kStartItem = 4.f, kTilePair = 1.8f, kTileSingle = 1.f, kStartSpan = 3.f;
-constexpr float kFoldPerRow = 4 * 512.f / 65536.f;
-constexpr int kMaxSearchGroups = 256;
+// The line that the CTAs' shares divide, in units of 0.3 us as measured on the prefix kernel: a tile against at most 128
+// rows (bound by its stream) or more (by the tensor and special-function pipes), and opening and closing a segment.
+constexpr int kTileSingle = 5, kTilePair = 8, kOpen = 14;
+// The same units for the choice of how many SMs work on prefixes: starting that kernel, starting the other one, a tile's
+// worth of own pages there, and one row of partial results written and folded, times SMs.
+constexpr float kStartPrefix = 16.f, kStartSpan = 24.f, kOwnTile = 6.f, kFoldRow = 0.12f;
 
 // Checks the grouping, decides what every group reads once, how many SMs work on that while the others stream the
-// requests' own pages, and into how many pieces each prefix is cut.  One block.
+// requests' own pages, and where each CTA's share of the prefixes starts.  One block.
 //
-// More pieces spread a prefix over more SMs but leave more partial results to fold; more CTAs on the prefix leave
-// fewer SMs to the other kernel, which runs at the same time.  Each thread costs one (CTAs, tiles per piece) pair with
-// the constants above; the cheapest is taken.
+// More CTAs on the prefixes leave fewer SMs to the other kernel, which runs at the same time, and cut them into more
+// pieces, whose partial results have to be folded.  Thread x costs x + 1 CTAs with the constants above; the cheapest
+// is taken.  Shares are equal parts of the line, so no CTA has more than its part whatever the prefixes' lengths.
 __global__ void __launch_bounds__(1024) sp_plan_kernel(const int32_t *__restrict__ kv_indptr,
                                                        const int32_t *__restrict__ group_indptr, int batch, int groups,
                                                        int page_size, int heads_per_kv, int hkv, int max_splits,
                                                        int sms, PlanView v, int32_t *err) {
-  __shared__ unsigned long long sh_tiles, sh_own, sh_best;
-  __shared__ int sh_base, sh_most, sh_used, sh_count;
+  __shared__ unsigned long long sh_own, sh_best, sh_longest, sh_rows, sh_row_len;
+  __shared__ long long sh_scan[32][2], sh_carry[2];
+  __shared__ int sh_used;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (tid == 0) {
-    sh_tiles = sh_own = 0;
+    sh_own = sh_longest = sh_rows = sh_row_len = 0;
     sh_best = ~0ull;
-    sh_base = sh_most = sh_used = sh_count = 0;
+    sh_used = 0;
+    sh_carry[0] = sh_carry[1] = 0;
   }
   int bad = -1;
   for (int g = tid; g < groups; g += 1024) {
@@ -101,8 +102,14 @@ __global__ void __launch_bounds__(1024) sp_plan_kernel(const int32_t *__restrict
     }
     return;
   }
-  auto blocks_of = [&](int members) { return (int)(((long long)members * heads_per_kv + kRowsPerItem - 1) / kRowsPerItem); };
-  auto tiles_of = [&](int pages) { return (pages * page_size + kTileTokens - 1) / kTileTokens; };
+  auto tiles_of = [&](int pages) { return (int)(((long long)pages * page_size + kTileTokens - 1) / kTileTokens); };
+  // blocks of more than 128 rows, and whether a smaller one is left
+  auto pair_blocks = [&](int members) { return (int)(((long long)members * heads_per_kv + kRowsPerBlock / 2 - 1) / kRowsPerBlock); };
+  auto single_blocks = [&](int members) {
+    const int left = (int)((long long)members * heads_per_kv % kRowsPerBlock);
+    return left > 0 && left <= kRowsPerBlock / 2 ? 1 : 0;
+  };
+  auto length = [&](int tiles, bool pair) { return (long long)tiles * (pair ? kTilePair : kTileSingle) + kOpen; };
   // ---- a warp per group: pages common to all its requests, pages left to each
   for (int g = warp; g < groups; g += 32) {
     const int a = group_indptr[g], m = group_indptr[g + 1] - a;
@@ -123,80 +130,134 @@ __global__ void __launch_bounds__(1024) sp_plan_kernel(const int32_t *__restrict
       v.groups[g] = Group{a, m, pages, 0};
       atomicAdd(&sh_own, (unsigned long long)(own - (long long)m * pages));
       if (pages > 0) {
-        const int tiles = tiles_of(pages), blocks = blocks_of(m) * hkv;
-        atomicAdd(&sh_tiles, (unsigned long long)tiles * blocks);
-        atomicAdd(&sh_base, blocks);
-        atomicMax(&sh_most, tiles);
+        const int tiles = tiles_of(pages), pb = pair_blocks(m), sb = single_blocks(m);
+        const long long rows_single = sb ? (long long)m * heads_per_kv - (long long)pb * kRowsPerBlock : 0;
+        const long long rows_pair = (long long)m * heads_per_kv - rows_single;
+        atomicMax(&sh_longest, (unsigned long long)length(tiles, pb > 0));
+        atomicAdd(&sh_rows, (unsigned long long)(rows_pair + 2 * rows_single));
+        atomicAdd(&sh_row_len, (unsigned long long)(rows_pair * length(tiles, true) + 2 * rows_single * length(tiles, false)));
         atomicAdd(&sh_used, 1);
       }
     }
   }
   __syncthreads();
-  const float own_tiles = (float)((double)sh_own * page_size / kTileTokens * hkv);
-  const int most = max(sh_most, 1), max_chunks = max(1, max_splits / 2);
-  // thread = (CTAs: 32 steps up to all SMs, tiles per piece: the longest prefix in 1 .. 32 pieces)
-  int ctas = max(1, sms * (warp + 1) / 32);
-  int per = (most + lane) / (lane + 1);
-  if (sh_base > 0) {
-    if (groups <= kMaxSearchGroups) {
-      long long items = 0, folds = 0, pairs = 0;
-      int longest = 0;  // tiles of an item
-      for (int g = 0; g < groups; ++g) {
-        const Group gr = v.groups[g];
-        if (gr.pages == 0) continue;
-        const int chunks = min((tiles_of(gr.pages) + per - 1) / per, max_chunks);
-        const int rows = gr.members * heads_per_kv;
-        longest = max(longest, (tiles_of(gr.pages) + chunks - 1) / chunks);
-        items += (long long)blocks_of(gr.members) * chunks;
-        if (rows > kRowsPerItem / 2) pairs += (long long)blocks_of(gr.members) * chunks;
-        folds += (long long)rows * chunks * (rows % kRowsPerItem <= kRowsPerItem / 2 && rows < kRowsPerItem ? 2 : 1);
-      }
-      items *= hkv;
-      if (items <= sh_base + kSpareItems) {
-        const long long rounds = (items + ctas - 1) / ctas;
-        const float tile = kTileSingle + (kTilePair - kTileSingle) * (float)(pairs * hkv) / (float)items;
-        const float prefix = kStartPrefix + (float)rounds * (kStartItem + tile * (float)longest);
-        const float fold = (float)folds * hkv * kFoldPerRow / (float)sms;
-        const float own = kStartSpan + own_tiles / (float)(ctas < sms ? sms - ctas : sms);
-        const float cost = (ctas < sms ? fmaxf(prefix, own) : prefix + own) + fold;
-        atomicMin(&sh_best, ((unsigned long long)__float_as_uint(cost) << 32) | (unsigned)tid);
-      }
-    } else if (tid == 0) {  // hundreds of groups: enough pieces without cutting
-      sh_best = 31 * 32;    // all SMs, whole prefixes
+  // ---- the line: segments and lengths of the groups, scanned in order
+  for (int g0 = 0; g0 < groups; g0 += 1024) {
+    const int g = g0 + tid;
+    long long x[2] = {0, 0};
+    if (g < groups && v.groups[g].pages > 0) {
+      const Group gr = v.groups[g];
+      const int tiles = tiles_of(gr.pages), pb = pair_blocks(gr.members), sb = single_blocks(gr.members);
+      x[0] = (long long)(pb + sb) * hkv;
+      x[1] = hkv * (pb * length(tiles, true) + sb * length(tiles, false));
     }
+    const long long own[2] = {x[0], x[1]};
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const long long y = __shfl_up_sync(0xffffffffu, x[k], d);
+        if (lane >= d) x[k] += y;
+      }
+      if (lane == 31) sh_scan[warp][k] = x[k];
+    }
+    __syncthreads();
+    for (int k = 0; k < 2; ++k) {
+      for (int w = 0; w < warp; ++w) x[k] += sh_scan[w][k];
+      x[k] += sh_carry[k];
+    }
+    if (g < groups) {
+      v.groups[g].segment = (int)(x[0] - own[0]);
+      v.line[g] = x[1] - own[1];
+    }
+    __syncthreads();
+    if (tid == 1023) {
+      sh_carry[0] = x[0];
+      sh_carry[1] = x[1];
+    }
+    __syncthreads();
+  }
+  const long long line = sh_carry[1];
+  const int segments = (int)sh_carry[0];
+  if (line == 0) {
+    if (tid == 0) {
+      v.header[0] = v.header[1] = v.header[2] = 0;
+      v.header[3] = sms;
+    }
+    return;
+  }
+  // ---- how many CTAs.  A share holds a tile at least; no segment is cut into more pieces than there is room for.
+  const int max_pieces = max(1, max_splits / 2);
+  const bool cut = max_pieces >= 3;
+  long long most = min((long long)sms, max(1ll, line / (kOpen + kTilePair)));
+  if (cut) most = max(1ll, min(most, (max_pieces - 2) * line / (long long)sh_longest));
+  if (tid < (int)most) {
+    const int n = tid + 1;
+    const float own = kStartSpan + (float)((double)sh_own * page_size / kTileTokens * hkv) * kOwnTile / (float)(n < sms ? sms - n : sms);
+    const float prefix = kStartPrefix + fmaxf((float)line / (float)n, cut ? 0.f : (float)sh_longest);
+    const float fold = kFoldRow * (float)hkv / (float)sms * ((float)sh_rows + (cut ? (float)sh_row_len * (float)n / (float)line : 0.f));
+    // beside each other, or (on all SMs) one after the other
+    const float cost = (n < sms ? fmaxf(prefix, own) : prefix + own) + fold;
+    atomicMin(&sh_best, ((unsigned long long)__float_as_uint(cost) << 32) | (unsigned)tid);
   }
   __syncthreads();
-  if (sh_base > 0) {
-    const int best = sh_best == ~0ull ? 31 * 32 : (int)(sh_best & 1023);
-    ctas = max(1, sms * (best / 32 + 1) / 32);
-    per = (most + best % 32) / (best % 32 + 1);
-  }
+  const int ctas = (int)(sh_best & 0xffffffffu) + 1;
+  auto share_of = [&](long long x) { return (int)(((x + 1) * ctas - 1) / line); };
   for (int g = warp; g < groups; g += 32) {
     const Group gr = v.groups[g];
     if (gr.pages == 0) continue;
-    const int blocks = blocks_of(gr.members);
-    int chunks = min((tiles_of(gr.pages) + per - 1) / per, max_chunks);
-    int at = 0;
-    if (lane == 0) {
-      at = atomicAdd(&sh_count, blocks * hkv * chunks);
-      if (at + blocks * hkv * chunks > v.max_items) {  // (cannot happen: kept so that nothing is written out of range)
-        report_error(err, PIEKV_ERR_PAGE_CAPACITY, KID_SHARED_PREFIX, g, chunks);
-        chunks = 0;
-      }
-      v.groups[g].chunks = chunks;
+    const int pb = pair_blocks(gr.members), blocks = pb + single_blocks(gr.members), tiles = tiles_of(gr.pages);
+    for (int i = lane; i < blocks * hkv; i += 32) {
+      const int block = i / hkv;
+      const bool pair = block < pb;
+      const long long at = v.line[g] + min(i, pb * hkv) * length(tiles, true) + max(0, i - pb * hkv) * length(tiles, false);
+      const int first = cut ? share_of(at + kOpen) : 0;
+      const int last = cut ? share_of(at + kOpen + (long long)(tiles - 1) * (pair ? kTilePair : kTileSingle)) : 0;
+      v.segments[gr.segment + i] = Segment{gr.first, kv_indptr[gr.first], gr.pages, i % hkv, block * kRowsPerBlock,
+                                           gr.members * heads_per_kv - block * kRowsPerBlock, first, last - first + 1};
     }
-    at = __shfl_sync(0xffffffffu, at, 0);
-    chunks = __shfl_sync(0xffffffffu, chunks, 0);
-    for (int i = lane; i < blocks * hkv * chunks; i += 32)
-      v.items[at + i] = Item{g, i % hkv, (i / hkv) % blocks, i / (hkv * blocks)};
   }
-  __syncthreads();
+  for (int c = tid; c <= ctas; c += 1024) {
+    const long long x = line * c / ctas;
+    int lo = 0, hi = groups - 1;  // last group whose start is <= x (of equal starts the one with a prefix: the last)
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (v.line[mid] <= x)
+        lo = mid;
+      else
+        hi = mid - 1;
+    }
+    int2 start = make_int2(segments, 0);
+    if (c < ctas) {
+      const Group gr = v.groups[lo];
+      const int tiles = tiles_of(gr.pages);
+      const long long in_pairs = (long long)pair_blocks(gr.members) * hkv * length(tiles, true);
+      long long y = x - v.line[lo];
+      int seg = gr.segment;
+      const bool pair = y < in_pairs;
+      if (!pair) {
+        seg += pair_blocks(gr.members) * hkv;
+        y -= in_pairs;
+      }
+      seg += (int)(y / length(tiles, pair));
+      y %= length(tiles, pair);
+      const int step = pair ? kTilePair : kTileSingle;
+      // tiles whose first unit lies before x belong to the share before
+      int tile = y <= kOpen ? 0 : (int)((y - kOpen + step - 1) / step);
+      if (!cut) tile = y > 0 ? tiles : 0;
+      if (tile >= tiles) {
+        ++seg;
+        tile = 0;
+      }
+      start = make_int2(seg, tile);
+    }
+    v.starts[c] = start;
+  }
   if (tid == 0) {
-    const int items = min(sh_count, v.max_items);
-    v.header[0] = items;
+    v.header[0] = ctas;
     v.header[1] = sh_used;
-    v.header[2] = min(ctas, items);
-    v.header[3] = items > 0 && ctas < sms ? sms - ctas : sms;
+    v.header[2] = segments;
+    v.header[3] = ctas < sms ? sms - ctas : sms;
   }
 }
 
@@ -299,11 +360,10 @@ extern "C" int piekv_shared_prefix_run(const piekv_shared_prefix_args *args, voi
   px.q = a.q;
   px.q_sn = a.q_sn;
   px.q_sh = a.q_sh;
-  px.kv_indptr = a.kv_indptr;
   px.kv_indices = a.kv_indices;
   px.header = v.header;
-  px.groups = v.groups;
-  px.items = v.items;
+  px.starts = v.starts;
+  px.segments = v.segments;
   px.part_ml = reinterpret_cast<float2 *>(ws);
   px.part_o = reinterpret_cast<float *>(ws + prefix_ml_bytes(a.batch, a.hq, args->max_splits));
   px.batch = a.batch;
@@ -318,6 +378,7 @@ extern "C" int piekv_shared_prefix_run(const piekv_shared_prefix_args *args, voi
   sp.requests = v.requests;
   sp.header = v.header;
   sp.groups = v.groups;
+  sp.segments = v.segments;
   sp.part_o = px.part_o;
   sp.part_ml = px.part_ml;
   sp.own_o = px.part_o + (int64_t)args->max_splits * a.batch * a.hq * 128;
