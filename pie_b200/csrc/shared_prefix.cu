@@ -61,11 +61,13 @@ __global__ void __launch_bounds__(128) sp_match_kernel(const int32_t *__restrict
 }
 
 // The line that the CTAs' shares divide, in units of 0.3 us as measured on the prefix kernel: a tile against at most 128
-// rows (bound by its stream) or more (by the tensor and special-function pipes), and opening and closing a segment.
-constexpr int kTileSingle = 5, kTilePair = 8, kOpen = 14;
-// The same units for the choice of how many SMs work on prefixes: starting that kernel, starting the other one, a tile's
-// worth of own pages there, and one row of partial results written and folded, times SMs.
-constexpr float kStartPrefix = 16.f, kStartSpan = 24.f, kOwnTile = 6.f, kFoldRow = 0.12f;
+// rows (bound by its stream) or more (by the tensor and special-function pipes), and opening and closing a piece.
+constexpr int kTileSingle = 5, kTilePair = 8, kOpen = 22;
+// The same units for the choice of how many SMs work on prefixes: starting that kernel, starting the other one beside it
+// or behind it, a tile's worth of own pages there, and one row of partial results folded by an SM.  Two kernels that
+// stream at the same time slow each other down by up to kContention.
+constexpr float kStartPrefix = 16.f, kStartBeside = 24.f, kStartBehind = 90.f, kOwnTile = 6.f, kFoldRow = 0.03f;
+constexpr float kContention = 0.3f;
 
 // Checks the grouping, decides what every group reads once, how many SMs work on that while the others stream the
 // requests' own pages, and where each CTA's share of the prefixes starts.  One block.
@@ -192,11 +194,16 @@ __global__ void __launch_bounds__(1024) sp_plan_kernel(const int32_t *__restrict
   long long most = min((long long)sms, max(1ll, line / (kOpen + kTilePair)));
   if (cut) most = max(1ll, min(most, (max_pieces - 2) * line / (long long)sh_longest));
   if (tid < (int)most) {
-    const int n = tid + 1;
-    const float own = kStartSpan + (float)((double)sh_own * page_size / kTileTokens * hkv) * kOwnTile / (float)(n < sms ? sms - n : sms);
-    const float prefix = kStartPrefix + fmaxf((float)line / (float)n, cut ? 0.f : (float)sh_longest);
-    const float fold = kFoldRow * (float)hkv / (float)sms * ((float)sh_rows + (cut ? (float)sh_row_len * (float)n / (float)line : 0.f));
-    // beside each other, or (on all SMs) one after the other
+    const int n = tid + 1, left = n < sms ? sms - n : sms;
+    const float own = (n < sms ? kStartBeside : kStartBehind) +
+                      (float)((double)sh_own * page_size / kTileTokens * hkv) * kOwnTile / (float)left;
+    // a share that starts inside a segment opens one piece more than the line counts, one that is not an even part of
+    // the segments (or a whole number of them) two
+    const bool even = n % segments == 0 || segments % n == 0;
+    float prefix = fmaxf((float)line / (float)n, cut ? 0.f : (float)sh_longest) + (even ? kOpen : 2 * kOpen);
+    if (n < sms) prefix *= 1.f + kContention * fminf(1.f, own / prefix);
+    prefix += kStartPrefix;
+    const float fold = kFoldRow * (float)hkv / (float)left * ((float)sh_rows + (cut ? (float)sh_row_len * (float)n / (float)line : 0.f));
     const float cost = (n < sms ? fmaxf(prefix, own) : prefix + own) + fold;
     atomicMin(&sh_best, ((unsigned long long)__float_as_uint(cost) << 32) | (unsigned)tid);
   }
