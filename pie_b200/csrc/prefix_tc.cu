@@ -94,8 +94,7 @@ __device__ __forceinline__ Work work_of(const PrefixTcParams &p, int cta, int se
 }
 // the pieces of a CTA's share in order: fn(piece) until it returns false
 template <typename F>
-__device__ __forceinline__ void for_pieces(const PrefixTcParams &p, int cta, F fn) {
-  const int2 from = __ldg(p.starts + cta), to = __ldg(p.starts + cta + 1);
+__device__ __forceinline__ void for_pieces(const PrefixTcParams &p, int cta, int2 from, int2 to, F fn) {
 #pragma unroll 1
   for (int seg = from.x; seg < to.x || (seg == to.x && to.y > 0); ++seg)
     if (!fn(work_of(p, cta, seg, seg == from.x ? from.y : 0, seg == to.x ? to.y : -1))) return;
@@ -118,7 +117,8 @@ __global__ void __launch_bounds__(kPxThreads, 1)
 
   // The kernel behind this one reads its own pages first and waits for these results only then.
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  if ((int)blockIdx.x >= __ldg(p.header)) return;
+  const int2 share_from = __ldg(p.starts + blockIdx.x), share_to = __ldg(p.starts + blockIdx.x + 1);
+  if (share_from.x == share_to.x && share_from.y == share_to.y) return;
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -172,7 +172,7 @@ __global__ void __launch_bounds__(kPxThreads, 1)
       uint64_t *full = is_v ? v_full : k_full, *empty = is_v ? v_empty : k_empty;
       int armed = 0;
       bool ok = true;
-      for_pieces(p, blockIdx.x, [&](const Work &w) {
+      for_pieces(p, blockIdx.x, share_from, share_to, [&](const Work &w) {
         for (int t = 0; ok && t < w.n[0]; ++t)
           for (int x = 0; x < (w.pair ? 1 : 2); ++x) {
             if (t >= w.n[x]) continue;
@@ -244,7 +244,7 @@ __global__ void __launch_bounds__(kPxThreads, 1)
         };
         bool ok = true;
         int qi[2] = {0, 0};  // query tiles of A and B taken so far: phases of q_full
-        for_pieces(p, blockIdx.x, [&](const Work &w) {
+        for_pieces(p, blockIdx.x, share_from, share_to, [&](const Work &w) {
           const int na = w.n[0], nb = w.n[1];
           ok = wait(&q_full[0], qi[0]++) && wait_k();
           if (!ok) return false;
@@ -300,7 +300,7 @@ __global__ void __launch_bounds__(kPxThreads, 1)
     int sc = 0, oc = 0;  // score tiles and items (with tiles) finished: phases of s_full and o_done
     bool ok = true;
 
-    for_pieces(p, blockIdx.x, [&](const Work &w) {
+    for_pieces(p, blockIdx.x, share_from, share_to, [&](const Work &w) {
       const int rows = w.rows[x], n = w.n[x];
       const bool row_valid = row < rows;
       const bool warp_valid = q4 * 32 < rows;

@@ -8,8 +8,7 @@ struct PrefixTcParams {
   const void *q;  // [batch, Hq, 128], rows 16-byte aligned
   int64_t q_sn, q_sh;
   const int32_t *kv_indices;
-  const int *header;  // the plan's
-  const int2 *starts;
+  const int2 *starts;  // the plan's
   const sprefix::Segment *segments;
   float *part_o;    // [split][batch][Hq][128], unnormalised
   float2 *part_ml;  // [split][batch][Hq]: reference maximum (log2 units), sum

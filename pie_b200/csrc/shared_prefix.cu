@@ -98,6 +98,7 @@ __global__ void __launch_bounds__(1024) sp_plan_kernel(const int32_t *__restrict
   const bool refused = __syncthreads_or(bad >= 0) != 0;
   if (refused) {  // every request on its own
     for (int b = tid; b < batch; b += 1024) v.requests[b] = make_int2(0, 0);
+    for (int c = tid; c <= sms; c += 1024) v.starts[c] = make_int2(0, 0);
     if (tid == 0) {
       v.header[0] = v.header[1] = v.header[2] = 0;
       v.header[3] = sms;
@@ -182,6 +183,7 @@ __global__ void __launch_bounds__(1024) sp_plan_kernel(const int32_t *__restrict
   const long long line = sh_carry[1];
   const int segments = (int)sh_carry[0];
   if (line == 0) {
+    for (int c = tid; c <= sms; c += 1024) v.starts[c] = make_int2(0, 0);
     if (tid == 0) {
       v.header[0] = v.header[1] = v.header[2] = 0;
       v.header[3] = sms;
@@ -224,8 +226,8 @@ __global__ void __launch_bounds__(1024) sp_plan_kernel(const int32_t *__restrict
                                            gr.members * heads_per_kv - block * kRowsPerBlock, first, last - first + 1};
     }
   }
-  for (int c = tid; c <= ctas; c += 1024) {
-    const long long x = line * c / ctas;
+  for (int c = tid; c <= sms; c += 1024) {  // (CTAs behind the last share start where they end)
+    const long long x = c < ctas ? line * c / ctas : 0;
     int lo = 0, hi = groups - 1;  // last group whose start is <= x (of equal starts the one with a prefix: the last)
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
@@ -315,6 +317,7 @@ extern "C" int piekv_shared_prefix_plan(const piekv_shared_prefix_args *args, vo
   if (int rc = check_args(args, "shared_prefix_plan")) return rc;
   const piekv_shared_prefix_args &a = *args;
   if (a.batch == 0) return 0;
+  PIEKV_REQUIRE(sm_count() <= kMaxCtas, "shared_prefix_plan: %d SMs, the plan holds %d shares", sm_count(), kMaxCtas);
   const PlanView v = plan_view(a.plan, a.batch, a.num_groups, a.num_qo_heads, a.num_kv_heads);
   cudaStream_t st = (cudaStream_t)stream;
   sp_match_kernel<<<a.batch, 128, 0, st>>>(a.kv_indptr, a.kv_indices, a.kv_last_page_len, a.group_indptr, a.batch,
@@ -368,7 +371,6 @@ extern "C" int piekv_shared_prefix_run(const piekv_shared_prefix_args *args, voi
   px.q_sn = a.q_sn;
   px.q_sh = a.q_sh;
   px.kv_indices = a.kv_indices;
-  px.header = v.header;
   px.starts = v.starts;
   px.segments = v.segments;
   px.part_ml = reinterpret_cast<float2 *>(ws);
