@@ -572,7 +572,8 @@ __global__ void __launch_bounds__(k2Threads, 1)
         ++sc;
         tc::fence_after_sync();
         const int t0 = j * kBN;
-        const bool full_tile = kBand || has_mask ? (mw.x & mw.y & mw.z & mw.w) == 0xffffffffu : t0 + kBN - 1 <= limit;
+        bool full_tile = kBand || has_mask ? (mw.x & mw.y & mw.z & mw.w) == 0xffffffffu : t0 + kBN - 1 <= limit;
+        if (kBand) full_tile = __all_sync(0xffffffffu, full_tile);  // the whole warp masks, and stores, together
 
         // ---- pass 1: running maximum, 64 columns at a time (rolled: the unrolled body of a whole row is
         // ~10 KB of code per softmax warp, which evicts the MMA thread's code from the instruction cache)
@@ -590,11 +591,16 @@ __global__ void __launch_bounds__(k2Threads, 1)
               const bool allow = kBand || has_mask ? (((i < 32 ? w0 : w1) >> (i & 31)) & 1u) != 0 : t0 + h * 64 + i <= limit;
               sr[i] = allow ? sr[i] : 0xff800000u;
             }
+            if (kBand) {  // back where they came from: pass 2 then reads them masked
+              tc::tmem_st32(s_addr + h * 64, sr);
+              tc::tmem_st32(s_addr + h * 64 + 32, sr + 32);
+            }
           }
 #pragma unroll
           for (int i = 0; i < 32; ++i)
             mxa[i & 3] = max3(mxa[i & 3], __uint_as_float(sr[2 * i]), __uint_as_float(sr[2 * i + 1]));
         }
+        if (kBand && !full_tile) tc::tmem_wait_st();
         float mx = fmaxf(fmaxf(mxa[0], mxa[1]), fmaxf(mxa[2], mxa[3])) * c;  // c > 0
         float alpha = 1.f;
         bool rescale = false;
@@ -629,7 +635,7 @@ __global__ void __launch_bounds__(k2Threads, 1)
           tc::tmem_ld32(s_addr + h * 64, sr);
           tc::tmem_ld32(s_addr + h * 64 + 32, sr + 32);
           tc::tmem_wait_ld();
-          if (!full_tile) {
+          if (!kBand && !full_tile) {
             const uint32_t w0 = h ? mw.z : mw.x, w1 = h ? mw.w : mw.y;
 #pragma unroll
             for (int i = 0; i < 64; ++i) {
