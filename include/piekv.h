@@ -354,7 +354,8 @@ int piekv_prefill_export_mask(const int32_t *qo_indptr, const int32_t *kv_indptr
  *                pages that hold such keys.
  *   first_tokens 0: none.  n > 0 together with a window: keys 0 .. n - 1 stay visible to every query at or
  *                behind them however far the window has moved on.  Pages between the first tokens and the
- *                window are never read (their entries in kv_indices may be stale or -1).  Not taken together
+ *                window are never read (their entries in kv_indices may be stale or -1), and rows of other pages
+ *                that no query token sees may hold anything, NaN included.  Not taken together
  *                with a mask (bytes or run lengths), nor by the fused step.  A decode call needs
  *                piekv_decode_first_tokens_workspace_bytes; a prefill call is planned without a mask and
  *                without a window (piekv_prefill_plan), the run applies both.

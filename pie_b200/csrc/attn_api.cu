@@ -67,6 +67,8 @@ static int apply_options(AttnArgs &a, const piekv_attn_options *opt, const char 
   a.window_left = opt->window_left;
   // without a window nothing is hidden that the first tokens could keep visible
   a.first_tokens = opt->window_left >= 0 ? opt->first_tokens : 0;
+  // (positions minus the window stay inside 32 bits, also of queries before the context)
+  if (a.first_tokens > 0 && a.window_left > (1 << 30)) a.window_left = 1 << 30;
   a.sinks = opt->sinks;
   return 0;
 }

@@ -84,7 +84,7 @@ struct Rows {
   }
   // (without a branch: a batch of folds follows a batch of loads)
   __device__ __forceinline__ void fold(float2 ml, const float4 *v, bool live) {
-    live = live && ml.y > 0.f;  // a partial that saw nothing has no meaning in v
+    live = live && ml.y != 0.f;  // a partial that saw nothing has no meaning in v; one that saw NaN keeps it
     const float mn = live ? fmaxf(m, ml.x) : m;
     const float a = m == mn ? 1.f : fast_exp2(m - mn);  // m = -inf at first: 0
     const float w = live ? fast_exp2(ml.x - mn) : 0.f;

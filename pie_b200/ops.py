@@ -476,6 +476,9 @@ class AxisRopeConfig(RopeConfig):
         self.__dict__["_table"] = None  # laid out again at the next use
         object.__setattr__(self, name, value)
 
+    def to_c(self, head_dim: int) -> RopeParams:
+        raise ValueError("an AxisRopeConfig is taken by rope_axes_append_paged_kv_cache and apply_rope_axes_inplace only")
+
     def prepared(self) -> "_lib.RopeAxesTable":
         """The host table the kernels take, laid out once per set of parameters."""
         table = self.__dict__["_table"]
@@ -488,7 +491,7 @@ class AxisRopeConfig(RopeConfig):
             raise ValueError(f"sections must name 1 to {_lib.MAX_ROPE_AXES} axes, got {len(sections)}")
         if self.mode == "none":
             raise ValueError("rope mode 'none' has no angles; use append_paged_kv_cache")
-        rp = self.to_c(2 * sum(sections))
+        rp = RopeConfig.to_c(self, 2 * sum(sections))
         table = _lib.RopeAxesTable()
         check(lib.piekv_rope_axes_prepare(C.byref(rp), (C.c_int32 * len(sections))(*sections), len(sections),
                                           1 if self.cyclic else 0, C.byref(table)), "AxisRopeConfig")
@@ -687,7 +690,7 @@ def _check_first_tokens(first_tokens: int, window_left: int) -> int:
     n = int(first_tokens)
     if n < 0:
         raise ValueError(f"first_tokens must be >= 0, got {n}")
-    return n if window_left >= 0 else 0
+    return min(n, 2 ** 31 - 1) if window_left >= 0 else 0
 
 
 class BatchDecodeWithPagedKVCacheWrapper:
@@ -989,8 +992,10 @@ class BatchSharedPrefixDecodeWrapper:
             raise ValueError("logits_soft_cap is not supported")
         if window_left != -1:
             raise ValueError("a sliding window is not supported here; use BatchDecodeWithPagedKVCacheWrapper")
-        if num_qo_heads % num_kv_heads != 0:
+        if num_kv_heads <= 0 or num_qo_heads <= 0 or num_qo_heads % num_kv_heads != 0:
             raise ValueError(f"num_qo_heads {num_qo_heads} is not a multiple of num_kv_heads {num_kv_heads}")
+        if head_dim <= 0 or page_size <= 0:
+            raise ValueError(f"bad head_dim {head_dim} / page_size {page_size}")
         if kv_data_type is not None and kv_data_type != q_data_type:
             raise ValueError("kv_data_type must equal q_data_type")
         batch = indptr.shape[0] - 1

@@ -81,6 +81,7 @@ def test_the_library_refuses_on_the_host():
 
 def test_first_tokens_are_checked():
     assert ops._check_first_tokens(4, 10) == 4
+    assert ops._check_first_tokens(2 ** 40, 10) == 2 ** 31 - 1
     assert ops._check_first_tokens(4, -1) == 0  # nothing is hidden without a window
     with pytest.raises(ValueError, match="first_tokens"):
         ops._check_first_tokens(-1, 10)
@@ -144,6 +145,28 @@ def test_decode_empty_requests_sinks_strides_and_scale():
                    first_tokens=3, sinks=sinks)
     P.check_attention(got[0], got[1], sc.q, sc.pool, ref, scale=0.3)
     assert (got[0][0] == 0).all() and torch.isinf(got[1][0]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("window, first", [(2 ** 31 - 1, 3), (5, 2 ** 31 - 1), (2 ** 31 - 1, 2 ** 31 - 1)])
+def test_the_largest_numbers(window, first):
+    sc = make_scenario(8, 2, 128, torch.bfloat16, [(c, 1) for c in (3, 50, 300)])
+    _check(sc, _decode(sc, window, first), -1, 0)
+    sc = make_scenario(8, 2, 128, torch.bfloat16, [(3, 40), (200, 70)])
+    _check(sc, _prefill(sc, window, first), -1, 0)
+    sc = make_scenario(9, 3, 128, torch.bfloat16, [(0, 40)])
+    sc.meta.kv_indptr[1], sc.meta.kv_last_page_len[0] = 1, 9  # more query tokens than keys
+    _check(sc, _prefill(sc, window, first), -1, 0)
+
+
+@pytest.mark.gpu
+def test_decode_nan_in_sight_comes_out():
+    sc = make_scenario(8, 2, 128, torch.bfloat16, [(2000, 1), (300, 1)])
+    clean = _decode(sc, 1500, 4)[0]
+    sc.pool[sc.meta.kv_indices[100], 0, 3, 1] = math.nan  # inside the first request's window, kv head 1
+    out = _decode(sc, 1500, 4)[0]
+    assert torch.isnan(out[0, 4:]).all()
+    assert torch.equal(out[0, :4], clean[0, :4]) and torch.equal(out[1], clean[1])
 
 
 @pytest.mark.gpu

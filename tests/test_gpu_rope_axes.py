@@ -41,6 +41,11 @@ def test_bad_modes_are_refused():
         _config((8,), theta=0.0).prepared()
 
 
+def test_the_one_axis_calls_refuse_an_axis_config():
+    with pytest.raises(ValueError, match="AxisRopeConfig"):
+        _config((16, 24, 24)).to_c(128)
+
+
 def test_the_prepared_table_follows_the_parameters():
     c = _config((4, 2, 2))
     first = c.prepared()

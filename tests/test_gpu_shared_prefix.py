@@ -306,6 +306,49 @@ def test_small_workspaces():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("splits", [1, 2, 4, 6, 9])
+def test_workspaces_with_room_for_few_pieces(splits):
+    b = Batch([(260, [10] * 70), (150, [5, 6]), (90, [33] * 40), (0, [40, 2])], 8, 2, seed=13)
+    n = len(b.lens)
+    need = _lib.lib.piekv_shared_prefix_workspace_bytes(n, 8, 2, 128, splits)
+    w = b.plan(ops.BatchSharedPrefixDecodeWrapper(torch.empty(need, dtype=torch.uint8, device="cuda")))
+    b.check(w.run(b.q.cuda(), b.pool.cuda(), return_lse=True))
+    assert ops.device_error("cuda") is None
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("seed", range(24))
+def test_random_batches(seed):
+    """Group counts, lengths and head counts at random: wherever the shares of the prefixes' tiles happen to be cut."""
+    rng = np.random.default_rng(seed)
+    hkv = int(rng.choice([1, 2, 3, 4, 8]))
+    hq = hkv * int(rng.choice([1, 2, 3, 4, 7, 8, 12]))
+    groups = []
+    for _ in range(int(rng.integers(1, 12))):
+        members = int(rng.integers(1, 40 if rng.random() < 0.3 else 6))
+        groups.append((int(rng.integers(0, 220)), [int(x) for x in rng.integers(0, 90, members)]))
+    b = Batch(groups, hq, hkv, dtype=torch.float16 if seed % 2 else torch.bfloat16, seed=seed)
+    b.check(_run(b))
+    assert ops.device_error("cuda") is None
+
+
+@pytest.mark.gpu
+def test_no_requests_and_nan_in_sight():
+    b = Batch([(0, [])], 8, 2)
+    w = b.plan(ops.BatchSharedPrefixDecodeWrapper(_workspace()))
+    out, lse = w.run(b.q.cuda(), b.pool.cuda(), return_lse=True)
+    assert out.shape == (0, 8, 128) and lse.shape == (0, 8)
+    # NaN that a request does see comes out, whichever part it is in and however the parts are cut, and only there
+    b = Batch([(300, [700, 20, 30]), (300, [3, 4])], 8, 2, seed=14)
+    clean = _run(b)[0]
+    b.pool[b.lists[1][-1], 0, 1] = math.nan       # own page of request 1
+    b.pool[b.lists[3][200], 0, 2, 1] = math.nan   # shared page of requests 3 and 4, kv head 1
+    out = _run(b)[0]
+    assert torch.isnan(out[1]).all() and torch.isnan(out[3:, 4:]).all()
+    assert torch.equal(out[0], clean[0]) and torch.equal(out[2], clean[2]) and torch.equal(out[3:, :4], clean[3:, :4])
+
+
+@pytest.mark.gpu
 def test_bad_page_ids_are_reported():
     b = Batch([(30, [10, 20])], 8, 2, seed=12)
     for x in b.lists:
@@ -327,6 +370,10 @@ def test_refusals_on_the_device():
     w = ops.BatchSharedPrefixDecodeWrapper(_workspace())
     with pytest.raises(ValueError, match="window"):
         b.plan(w, window_left=4)
+    b.hkv = 0
+    with pytest.raises(ValueError, match="multiple"):
+        b.plan(w)
+    b.hkv = 2
     with pytest.raises(ValueError, match="group_indptr"):
         b.plan(w, groups=torch.zeros(1, dtype=torch.int32, device="cuda"))
     with pytest.raises(ValueError, match="int32"):
