@@ -334,7 +334,17 @@ __global__ void __launch_bounds__(k2Threads, 1)
       if (lane == 0) mbar_arrive(&item_empty[slot]);
       if (!valid) break;
       int j = 0;
+      // kBand: a tile's page ids are loaded while the ring still waits for room
+      auto band_page_id = [&](int tile) -> int {
+        int pi = tile * 8 + lane;
+        if (lane >= 8 || pi >= keys.pages) return a.num_pages;
+        if (pi >= keys.front) pi += keys.low_page - keys.front;
+        return __ldg(a.kv_indices + p0 + pi);
+      };
+      int next_page = kBand ? band_page_id(0) : 0;
       for (int left = left0; left > 0; --left) {
+        int page = next_page;
+        if (kBand) next_page = band_page_id(j + 1);
         const int st = armed % stages;
         if (!wait_or_abort(&empty[st], ((armed / stages) & 1) ^ 1, abort_flag)) {
           give_up(is_v ? 121 : 101);
@@ -342,13 +352,9 @@ __global__ void __launch_bounds__(k2Threads, 1)
           break;
         }
         while (!tile_active(srow, j)) ++j;
-        int pi = j * 8 + lane;
-        bool wanted = lane < 8 && pi < np;
-        if (kBand) {
-          wanted = lane < 8 && pi < keys.pages;
-          if (pi >= keys.front) pi += keys.low_page - keys.front;
-        }
-        int page = wanted ? __ldg(a.kv_indices + p0 + pi) : a.num_pages;
+        const int pi = j * 8 + lane;
+        if (!kBand) page = (lane < 8 && pi < np) ? __ldg(a.kv_indices + p0 + pi) : a.num_pages;
+        const bool wanted = lane < 8 && pi < (kBand ? keys.pages : np);
         if (wanted && (page < 0 || page >= a.num_pages)) {
           report_error(a.err, PIEKV_ERR_PAGE_ID, KID_PREFILL, p0 + pi, page);
           page = a.num_pages;  // outside the tensor map: zero fill

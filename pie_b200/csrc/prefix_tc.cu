@@ -173,31 +173,38 @@ __global__ void __launch_bounds__(kPxThreads, 1)
       int armed = 0;
       bool ok = true;
       for_pieces(p, blockIdx.x, share_from, share_to, [&](const Work &w) {
-        for (int t = 0; ok && t < w.n[0]; ++t)
-          for (int x = 0; x < (w.pair ? 1 : 2); ++x) {
-            if (t >= w.n[x]) continue;
-            const int st = armed % stages;
-            if (!wait_or_abort(&empty[st], ((armed / stages) & 1) ^ 1, abort_flag)) {
-              give_up(is_v ? 121 : 101);
-              ok = false;
-              break;
-            }
-            const int pi = (w.t0[x] + t) * 8 + lane;
-            const bool wanted = lane < 8 && pi < w.pages;
-            int page = wanted ? __ldg(p.kv_indices + w.list + pi) : p.num_pages;
-            if (wanted && (page < 0 || page >= p.num_pages)) {
-              report_error(p.err, PIEKV_ERR_PAGE_ID, KID_SHARED_PREFIX, w.list + pi, page);
-              page = p.num_pages;  // outside the tensor map: zeros, as behind the prefix
-            }
-            if (lane == 0) mbar_arrive_expect_tx(&full[st], kTileBytes);
-            __syncwarp();
-            if (lane < 8) {
-              const uint32_t dst = ring0 + st * kTileBytes + lane * 2048;
-              tma_load_5d(dst, &tmap_kv, 0, 0, 0, w.kv_head, page * 2 + (is_v ? 1 : 0), &full[st]);
-              tma_load_5d(dst + kHalfBytes, &tmap_kv, 0, 0, 1, w.kv_head, page * 2 + (is_v ? 1 : 0), &full[st]);
-            }
-            ++armed;
+        // tiles in the order they are used: shared ones, or A's and B's in turn.  A tile's page ids are loaded while the
+        // ring still waits for room.
+        const int total = w.pair ? w.n[0] : w.n[0] + w.n[1];
+        const bool turns = !w.pair && w.n[1] > 0;
+        auto entry_of = [&](int u) { return (!turns ? w.t0[0] + u : (u & 1 ? w.t0[1] : w.t0[0]) + (u >> 1)) * 8 + lane; };
+        auto page_of = [&](int u) -> int {
+          if (u >= total || lane >= 8 || entry_of(u) >= w.pages) return p.num_pages;  // outside the tensor map: zeros
+          return __ldg(p.kv_indices + w.list + entry_of(u));
+        };
+        int next = page_of(0);
+        for (int u = 0; u < total; ++u) {
+          int page = next;
+          next = page_of(u + 1);
+          const int st = armed % stages;
+          if (!wait_or_abort(&empty[st], ((armed / stages) & 1) ^ 1, abort_flag)) {
+            give_up(is_v ? 121 : 101);
+            ok = false;
+            break;
           }
+          if (lane < 8 && entry_of(u) < w.pages && (page < 0 || page >= p.num_pages)) {
+            report_error(p.err, PIEKV_ERR_PAGE_ID, KID_SHARED_PREFIX, w.list + entry_of(u), page);
+            page = p.num_pages;
+          }
+          if (lane == 0) mbar_arrive_expect_tx(&full[st], kTileBytes);
+          __syncwarp();
+          if (lane < 8) {
+            const uint32_t dst = ring0 + st * kTileBytes + lane * 2048;
+            tma_load_5d(dst, &tmap_kv, 0, 0, 0, w.kv_head, page * 2 + (is_v ? 1 : 0), &full[st]);
+            tma_load_5d(dst + kHalfBytes, &tmap_kv, 0, 0, 1, w.kv_head, page * 2 + (is_v ? 1 : 0), &full[st]);
+          }
+          ++armed;
+        }
         return ok;
       });
       // drain: the CTA must not retire while a bulk copy may still be landing

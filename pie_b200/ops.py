@@ -783,7 +783,7 @@ class BatchDecodeWithPagedKVCacheWrapper:
             pl["first_call"] = ((indptr.data_ptr(), indices.data_ptr(), last_page_len.data_ptr(), batch, pl["hq"],
                                  pl["hkv"], pl["d"], pl["page_size"]),
                                 (self.workspace_buffer.data_ptr(), self.workspace_buffer.numel(),
-                                 _err_word(indptr.device).data_ptr()), indptr.get_device())
+                                 _err_ptr(indptr.get_device())), indptr.get_device())
 
     def run(self, q: torch.Tensor, paged_kv_cache: torch.Tensor, out: Optional[torch.Tensor] = None,
             return_lse: bool = False, sinks: Optional[torch.Tensor] = None, sm_scale: Optional[float] = None):
@@ -965,7 +965,8 @@ class BatchSharedPrefixDecodeWrapper:
     back.  The plan holds until the page table's contents change; `replan()` rebuilds it from the same tensors.  Both
     only launch kernels on the current stream, so plan / replan and any number of run() calls (one per layer) can be
     captured in a CUDA graph together.  The plan lives in a buffer of its own; the workspace may be shared with other
-    wrappers whose calls are ordered on the same stream."""
+    wrappers whose calls are ordered on the same stream (a prefill wrapper keeps its plan in its workspace: plan it again
+    after a call of another wrapper on the same one)."""
 
     def __init__(self, float_workspace_buffer: torch.Tensor, kv_layout: str = "NHD") -> None:
         if kv_layout != "NHD":
@@ -1189,6 +1190,19 @@ class BatchPrefillWithPagedKVCacheWrapper:
                           brle=brle, causal=bool(causal), dtype=q_data_type, planned_for=None,
                           window_left=int(window_left), first_tokens=first_tokens,
                           sm_scale=float(sm_scale) if sm_scale is not None else 1.0 / math.sqrt(head_dim_qk))
+        if first_tokens > 0:
+            dev = qo_indptr.device
+            for t, name in ((paged_kv_indptr, "paged_kv_indptr"), (paged_kv_indices, "paged_kv_indices"),
+                            (paged_kv_last_page_len, "paged_kv_last_page_len"), (self.workspace_buffer, "workspace_buffer")):
+                if t.device != dev:
+                    raise ValueError(f"{name} is on {t.device}, qo_indptr on {dev}")
+            self._plan["first_call"] = (
+                qo_indptr.get_device(),
+                (qo_indptr.data_ptr(), paged_kv_indptr.data_ptr(), paged_kv_indices.data_ptr(),
+                 paged_kv_last_page_len.data_ptr(), None, 0, 1 if causal else 0, 1, batch),
+                (int(num_qo_heads), int(num_kv_heads), int(head_dim_qk), int(page_size)),
+                (self.workspace_buffer.data_ptr(), self.workspace_buffer.numel(), _err_ptr(qo_indptr.get_device())),
+                _attn_options(int(window_left), None, int(num_qo_heads), first_tokens))
 
     def _device_plan(self, n: int, num_pages: int) -> None:
         """Build the work list (and pack the mask) on the device once per plan(); later run() calls
@@ -1223,6 +1237,8 @@ class BatchPrefillWithPagedKVCacheWrapper:
         if self._plan is None:
             raise RuntimeError("Must call plan() before run()")
         pl = self._plan
+        if pl["first_tokens"] > 0:
+            return self._run_first_tokens(q, paged_kv_cache, out, return_lse, sinks, sm_scale)
         _require_cuda(q, "q")
         num_pages, page_size, hkv, d = _check_pool(paged_kv_cache)
         qs = _rows(q, "q")
@@ -1240,7 +1256,7 @@ class BatchPrefillWithPagedKVCacheWrapper:
         lse = torch.empty((n, pl["hq"]), dtype=torch.float32, device=q.device) if return_lse else None
         ws = self.workspace_buffer
         self._device_plan(n, num_pages)
-        opt = _attn_options(pl["window_left"], sinks, pl["hq"], pl["first_tokens"])
+        opt = _attn_options(pl["window_left"], sinks, pl["hq"])
         check(lib.piekv_prefill_run_opt(q.data_ptr(), qs[0], qs[1], paged_kv_cache.data_ptr(), out.data_ptr(),
                                         lse.data_ptr() if lse is not None else None, pl["qo_indptr"].data_ptr(),
                                         pl["indptr"].data_ptr(), pl["indices"].data_ptr(),
@@ -1255,6 +1271,41 @@ class BatchPrefillWithPagedKVCacheWrapper:
         return (out, lse) if return_lse else out
 
     forward = run
+
+    def _run_first_tokens(self, q, paged_kv_cache, out, return_lse, sinks, sm_scale):
+        """run() of a plan with a window and first tokens: the same checks, what the plan fixes prepared once."""
+        pl = self._plan
+        device, tables, sizes, tail, options = pl["first_call"]
+        if not isinstance(q, torch.Tensor):
+            _require_cuda(q, "q")
+        q_rows = _device_rows(q, "q", device)
+        num_pages, page_size, hkv, d = _check_pool(paged_kv_cache)
+        n, hq, dim = q.shape
+        if hq != pl["hq"] or dim != pl["d"]:
+            raise ValueError(f"q shape {tuple(q.shape)} differs from the plan (*, {pl['hq']}, {pl['d']})")
+        if page_size != pl["page_size"] or hkv != pl["hkv"] or d != pl["d"]:
+            raise ValueError("paged_kv_cache shape differs from the plan")
+        if q.dtype != paged_kv_cache.dtype:
+            raise ValueError(f"q dtype {q.dtype} differs from the cache dtype {paged_kv_cache.dtype}")
+        if paged_kv_cache.get_device() != device:
+            raise ValueError(f"the cache is on {paged_kv_cache.device}, the plan on cuda:{device}")
+        if out is None:
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        elif out.shape != q.shape or out.dtype != q.dtype or out.get_device() != device or not out.is_contiguous():
+            raise ValueError("out must be a contiguous tensor shaped and typed like q")
+        lse = torch.empty((n, hq), dtype=torch.float32, device=q.device) if return_lse else None
+        if pl["planned_for"] != (n, num_pages):
+            self._device_plan(n, num_pages)
+        if sinks is not None:
+            options = _attn_options(pl["window_left"], sinks, hq, pl["first_tokens"])
+        status = lib.piekv_prefill_run_opt(q.data_ptr(), *q_rows, paged_kv_cache.data_ptr(), out.data_ptr(),
+                                           lse.data_ptr() if return_lse else None, *tables, n, *sizes, num_pages,
+                                           _dtype_code(q.dtype, "prefill run"),
+                                           pl["sm_scale"] if sm_scale is None else float(sm_scale), *tail,
+                                           _stream_of(device), options)
+        if status:
+            check(status, "BatchPrefill.run")
+        return (out, lse) if return_lse else out
 
     def export_custom_mask(self, num_query_tokens: int, num_pages: int) -> torch.Tensor:
         """The mask this plan holds on the device (from bytes, run lengths and / or a window) in the reference's
