@@ -47,6 +47,7 @@ constexpr int kPage = 16;
 constexpr int kTileBytes = 8192;  // one (page, head): K 4 KiB + V 4 KiB
 constexpr int kCounterBytes = 65536;
 constexpr int kMaxSlice = 512;   // requests per launch: the line is kept in shared memory
+static_assert(kMaxSlice * 128 <= 65536 && PIEKV_SHARED_PREFIX_MAX_SPLITS < 128, "sh_closed packs a request and a count");
 constexpr int kOpenCost = 4;     // pages
 constexpr int kMinUnits = 4;     // a share is not made smaller than this
 
@@ -130,7 +131,8 @@ __global__ void __launch_bounds__(Shape<HB>::kThreads, Shape<HB>::kCtasPerSm)
   __shared__ __align__(8) uint64_t full_bar[kStages], empty_bar[kStages];
   __shared__ int sh_cost[kMaxSlice + 1];  // prefix sums of pages + kOpenCost
   __shared__ int sh_warp[kThreads / 32];
-  __shared__ short sh_closed[HB][kMaxSlice];  // requests whose own pages a warp has finished, for the prefix's join
+  // requests whose own pages a warp has finished, for the prefix's join: request * 128 + partial results to fold
+  __shared__ unsigned short sh_closed[HB][kMaxSlice];
   __shared__ int sh_abort;
 
   const AttnArgs &a = p.a;
@@ -465,7 +467,7 @@ __global__ void __launch_bounds__(Shape<HB>::kThreads, Shape<HB>::kCtasPerSm)
     if (!whole) {
       pend_b[c == s_first ? 1 : 0] = b;
     } else if (later) {
-      if (lane == 0) sh_closed[warp][closed] = (short)b;
+      if (lane == 0) sh_closed[warp][closed] = (unsigned short)(b * 128);
       ++closed;
     }
   });
@@ -496,52 +498,49 @@ __global__ void __launch_bounds__(Shape<HB>::kThreads, Shape<HB>::kCtasPerSm)
       later = has_prefix(b);
     } else {
       if (!prefixed) break;
-      if (x == 2) {  // (also without work: the launch must not end before the one it was allowed to overtake)
+      if (x == 2) {
+        // how many partial results each request has, looked up while the prefix kernel may still be at work
+        __syncwarp();
+        const int problem = sprefix::problem_rows(group);
+        for (int i = lane; i < closed; i += 32) {
+          const int e = sh_closed[warp][i], request = p.b0 + (e >> 7);
+          const sprefix::Group g = p.prefix.groups[__ldg(&p.prefix.requests[request].y)];
+          const int block = (request - g.first) * group / (2 * problem);  // a request's rows lie in one block
+          const sprefix::Segment &seg = p.prefix.segments[g.segment + block * a.hkv + hk];
+          sh_closed[warp][i] = (unsigned short)(e + sprefix::partials_of(seg, problem, p.prefix.max_splits));
+        }
+        // (also without work: the launch must not end before the one it was allowed to overtake)
         asm volatile("griddepcontrol.wait;" ::: "memory");
         __syncwarp();
       }
       if (x - 2 >= closed) break;
-      b = sh_closed[warp][x - 2];
+      b = sh_closed[warp][x - 2] >> 7;
     }
     const size_t request = (size_t)(p.b0 + b) * a.hq + head0;
-    sprefix::Group g{};
-    int n = 0;
-    if (x < 2)
-      n = last_share(b) - first_share(b) + 1;
-    else
-      g = p.prefix.groups[__ldg(&p.prefix.requests[p.b0 + b].y)];
-    // partial i of row r: at + (x < 2 ? max(2 i - 1, 0) : i) * step + r
+    // Row r's results: partial i of the share slots at `at` + max(2 i - 1, 0) * step + r; behind a prefix the own one
+    // first (written above by this warp), then partial i - 1 of the prefix.
+    const int n = x < 2 ? last_share(b) - first_share(b) + 1 : 1 + (sh_closed[warp][x - 2] & 127);
     const size_t at = x < 2 ? slot_base(first_share(b), true) : request;
     const size_t step = x < 2 ? (size_t)a.hq : (size_t)a.batch * a.hq;
-    const float *po = x < 2 ? p.part_o : p.prefix.part_o;
-    const float2 *pml = x < 2 ? p.part_ml : p.prefix.part_ml;
+    const float *po = x < 2 ? p.part_o : p.prefix.part_o, *po0 = x < 2 ? p.part_o : p.prefix.own_o;
+    const float2 *pml = x < 2 ? p.part_ml : p.prefix.part_ml, *pml0 = x < 2 ? p.part_ml : p.prefix.own_ml;
 #pragma unroll 1
     for (int r0 = 0; r0 < group; r0 += 4) {
       const int r = min(r0 + (lane >> 3), group - 1), sub = lane & 7;
       Rows acc;
       acc.clear();
-      if (x >= 2) {
-        const int block = ((p.b0 + b - g.first) * group + r) / sprefix::kRowsPerBlock;
-        n = sprefix::partials_of(p.prefix.segments[g.segment + block * a.hkv + hk], p.prefix.max_splits);
-        const float2 ml = ld_batch_cg(p.prefix.own_ml + request + r);  // written above by this warp
-        float4 v[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          v[k] = ld_batch_cg(reinterpret_cast<const float4 *>(p.prefix.own_o + (request + r) * kDim) + k * 8 + sub);
-        acc.fold(ml, v, true);
-      }
-      const int most = __reduce_max_sync(0xffffffffu, n);
 #pragma unroll 1
-      for (int i0 = 0; i0 < most; i0 += 4) {
+      for (int i0 = 0; i0 < n; i0 += 4) {
         float2 ml[4];
         float4 v[4][4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const int i = max(min(i0 + j, n - 1), 0);
-          const size_t row = at + (size_t)(x < 2 ? max(2 * i - 1, 0) : i) * step + r;
-          ml[j] = ld_batch_cg(pml + row);
+          const int i = min(i0 + j, n - 1);
+          const size_t row = at + (size_t)max(x < 2 ? 2 * i - 1 : i - 1, 0) * step + r;
+          ml[j] = ld_batch_cg((i == 0 ? pml0 : pml) + row);
+          const float4 *src = reinterpret_cast<const float4 *>((i == 0 ? po0 : po) + row * kDim) + sub;
 #pragma unroll
-          for (int k = 0; k < 4; ++k) v[j][k] = ld_batch_cg(reinterpret_cast<const float4 *>(po + row * kDim) + k * 8 + sub);
+          for (int k = 0; k < 4; ++k) v[j][k] = ld_batch_cg(src + k * 8);
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc.fold(ml[j], v[j], i0 + j < n);
@@ -566,7 +565,7 @@ __global__ void __launch_bounds__(Shape<HB>::kThreads, Shape<HB>::kCtasPerSm)
       }
     }
     if (later) {
-      if (lane == 0) sh_closed[warp][closed] = (short)b;
+      if (lane == 0) sh_closed[warp][closed] = (unsigned short)(b * 128);
       ++closed;
     }
   }

@@ -1,28 +1,32 @@
 // Attention of many requests to the pages they share, on the sm_100a tensor cores (tcgen05 / TMEM).
 //
 // The query rows of a group and kv head are packed, row = request * (heads per kv head) + head, so a prefix is read
-// once for all of them.  A segment is (group, kv head, block of 256 rows); CTAs have equal shares of all segments' tiles
-// (the plan, shared_prefix.cu) and work through the pieces of segments in theirs.  Two 128-row problems "A" and "B" run against each other on one SM - while the softmax warps of one work on its scores, the tensor pipe runs
-// the other's MMAs:
-//   more than 128 rows    A and B are the two halves of the block and share every K and V tile
-//   at most 128 rows      A and B are the same rows over the two halves of the piece
+// once for all of them.  A segment is (group, kv head, block of up to 256 rows); it is cut into items, which persistent
+// CTAs claim (the plan, shared_prefix.cu).  Two 128-row problems "A" and "B" run against each other on one SM - while the
+// softmax warps of one work on its scores, the tensor pipe runs the other's MMAs:
+//   more than one problem's rows   A and B are the two halves of the block and share every K and V tile
+//   otherwise                      A and B are the same rows over the two halves of the item
 // Every problem leaves a partial result (m, l, O) per row, unnormalised and in fp32, for the kernel that folds it with
 // the request's own pages (decode_span.cu): M = max m_i, L = sum l_i 2^(m_i - M), O = sum O_i 2^(m_i - M).
 //
 // What bounds it: with R rows per kv head a prefix token costs 4 * 128 * R flops and 512 bytes, so the tensor and
-// special-function pipes from about 200 rows on, HBM below.
+// special-function pipes from about 200 rows on, HBM below.  A tile against two problems takes 2.0 us on the faster SMs
+// and 2.7 on the slower ones (half of them, under this load), which is why items are claimed: with equal shares per CTA
+// the fast ones stood idle for a third of the launch (67 against 110 us on 16384 shared tokens, 128 requests of 64 heads).
 //
 //   TMEM (512 columns): S_A/P_A [0,128)  S_B/P_B [128,256)  O_A [256,384)  O_B [384,512)
 //   smem: Q_A, Q_B (32 KiB each), K ring (3 x 32 KiB), V ring (2 x 32 KiB)
-// P stays in TMEM (packed 16-bit pairs over the scores' columns) and the MMA order per step t is
-//   O_A(t) S_A(t + 1) O_B(t) S_B(t + 1), as in the prefill kernel (prefill_tc2.cu).
+// P stays in TMEM (packed 16-bit pairs over the scores' columns).  One thread issues every MMA, per step t
+//   O_A(t) S_A(next) O_B(t) S_B(next),  next = tile t + 1 or the following item's first,
+// so the streams run across item boundaries: the rings keep filling, a problem's query rows are replaced once its last
+// scores are computed, and the next item's first scores run while the softmax warps store the finished one's rows.
 //
 // Precision: S, m, l, O in fp32; P is rounded to the storage type because it meets V in one MMA type.
 //
 // Roles (384 threads): warps 0-3 softmax of A (thread = row = TMEM lane), 4-7 of B, 8 K producer, 9 MMA issuer and
-// TMEM owner, 10 V producer, 11 none; the last four give registers to the softmax warps.  The softmax threads bring
-// their own query row into shared memory (256 bytes, any strides).  Every wait is bounded; on a timeout the CTA reports,
-// all roles leave, bulk copies are drained and TMEM is released.
+// TMEM owner, 10 V producer, 11 scheduler (claims items, describes them in a ring that every role reads, brings query
+// rows in); the last four give registers to the softmax warps.  Every wait is bounded; on a timeout the CTA reports, all
+// roles leave, bulk copies are drained and TMEM is released.
 #include <cuda.h>
 
 #include <type_traits>
@@ -45,60 +49,20 @@ constexpr int kPxThreads = 384;
 constexpr int kPxRegsLaunch = 168, kPxRegsSoftmax = 200, kPxRegsOther = 96;
 static_assert(256 * kPxRegsSoftmax + 128 * kPxRegsOther <= kPxThreads * kPxRegsLaunch, "registers the CTA owns");
 constexpr int kPxSmemBytes = kTileBytes * (2 + kKStages + kVStages) + 1024;
-constexpr int kPxVWarp = kMmaWarp + 1;
-static_assert(kTileTokens == kBN && kRowsPerBlock == 2 * kBM, "plan and kernel cut the work alike");
-static_assert(sizeof(Segment) == 32, "a segment is read as two vectors");
+constexpr int kPxVWarp = kMmaWarp + 1, kPxSchedWarp = kMmaWarp + 2;
+constexpr int kPxSlots = 4;                         // items the scheduler may describe ahead of the slowest reader
+constexpr int kPxReaders = kSoftmaxWarps + 1 + 3;   // softmax warps, MMA thread, K, V and query-row cursors
+static_assert(kTileTokens == kBN, "plan and kernel cut the work alike");
+static_assert(sizeof(Segment) == 32 && sizeof(Item) == 16, "read as vectors");
 
-// A piece of a segment as every role reads it off the plan.
+// An item as the scheduler publishes it.
 struct Work {
-  int request, list, pages;    // the group's first request, its page list, pages of the prefix
-  int kv_head, row0;
-  int rows[2];                 // rows of A and B
-  int n[2], t0[2], split[2];   // tiles, first tile and partial index of A and B
-  bool pair;                   // A and B share their tiles
+  int valid;                  // 0: nothing is left
+  int list, pages, kv_head;   // the group's page list and its pages
+  int request[2], rows[2];    // first request and rows of A and B
+  int n[2], t0[2], split[2];  // tiles, first tile and partial index of A and B
+  int pair;                   // A and B share their tiles
 };
-__device__ __forceinline__ int4 ld_int4(const void *p) { return __ldg(reinterpret_cast<const int4 *>(p)); }
-// tiles [t0, t1) of segment `seg`, by CTA `cta`; t1 < 0: to its end
-__device__ __forceinline__ Work work_of(const PrefixTcParams &p, int cta, int seg, int t0, int t1) {
-  const int4 a = ld_int4(p.segments + seg), b = ld_int4(reinterpret_cast<const int4 *>(p.segments + seg) + 1);
-  Segment s;
-  s.request = a.x, s.list = a.y, s.pages = a.z, s.kv_head = a.w;
-  s.row0 = b.x, s.rows = b.y, s.first_cta = b.z, s.pieces = b.w;
-  Work w;
-  w.request = s.request;
-  w.list = s.list;
-  w.pages = s.pages;
-  w.kv_head = s.kv_head;
-  w.row0 = s.row0;
-  if (t1 < 0) t1 = (s.pages * kPage + kBN - 1) / kBN;
-  const int piece = s.pieces > 1 ? cta - s.first_cta : 0;
-  w.pair = s.rows > kBM;
-  w.t0[0] = t0;
-  if (w.pair) {
-    w.rows[0] = kBM;
-    w.rows[1] = min(kBM, s.rows - kBM);
-    w.n[0] = w.n[1] = t1 - t0;
-    w.t0[1] = t0;
-    w.split[0] = w.split[1] = piece;
-  } else {
-    const bool two = p.max_splits >= 2;
-    w.rows[0] = w.rows[1] = s.rows;
-    w.n[0] = two ? (t1 - t0 + 1) / 2 : t1 - t0;
-    w.n[1] = t1 - t0 - w.n[0];
-    w.t0[1] = t0 + w.n[0];
-    w.split[0] = two ? 2 * piece : piece;
-    w.split[1] = 2 * piece + 1;
-    if (!two) w.rows[1] = 0;
-  }
-  return w;
-}
-// the pieces of a CTA's share in order: fn(piece) until it returns false
-template <typename F>
-__device__ __forceinline__ void for_pieces(const PrefixTcParams &p, int cta, int2 from, int2 to, F fn) {
-#pragma unroll 1
-  for (int seg = from.x; seg < to.x || (seg == to.x && to.y > 0); ++seg)
-    if (!fn(work_of(p, cta, seg, seg == from.x ? from.y : 0, seg == to.x ? to.y : -1))) return;
-}
 
 __device__ __forceinline__ void store_v8(float *dst, const uint32_t *r) {
   asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(r[0]), "r"(r[1]), "r"(r[2]),
@@ -108,22 +72,23 @@ __device__ __forceinline__ void store_v8(float *dst, const uint32_t *r) {
 
 template <typename T>
 __global__ void __launch_bounds__(kPxThreads, 1)
-    prefix_tc_kernel(const __grid_constant__ CUtensorMap tmap_kv, const __grid_constant__ PrefixTcParams p) {
+    prefix_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_kv,
+                     const __grid_constant__ PrefixTcParams p) {
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t q_full[2], k_full[kKStages], k_empty[kKStages], v_full[kVStages], v_empty[kVStages],
-      s_full[2], p_full[2][2], o_done[2];
+  __shared__ __align__(8) uint64_t q_full[2], q_empty[2], k_full[kKStages], k_empty[kKStages], v_full[kVStages],
+      v_empty[kVStages], s_full[2], p_full[2][2], o_done[2], item_full[kPxSlots], item_empty[kPxSlots];
+  __shared__ __align__(16) Work sh_item[kPxSlots];
   __shared__ uint32_t tmem_slot;
   __shared__ int sh_abort;
 
   // The kernel behind this one reads its own pages first and waits for these results only then.
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int2 share_from = __ldg(p.starts + blockIdx.x), share_to = __ldg(p.starts + blockIdx.x + 1);
-  if (share_from.x == share_to.x && share_from.y == share_to.y) return;
+  const int ctas = __ldg(p.header);
+  if ((int)blockIdx.x >= ctas) return;
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  uint8_t *base_ptr = smem_raw + (base - smem_u32(smem_raw));
   const uint32_t q_smem = base;
   const uint32_t k_smem0 = base + 2 * kTileBytes;
   const uint32_t v_smem0 = base + (2 + kKStages) * kTileBytes;
@@ -138,11 +103,16 @@ __global__ void __launch_bounds__(kPxThreads, 1)
       mbar_init(&v_empty[s], 1);
     }
     for (int x = 0; x < 2; ++x) {
-      mbar_init(&q_full[x], 4);  // one arrival per softmax warp
+      mbar_init(&q_full[x], 1);
+      mbar_init(&q_empty[x], 1);
       mbar_init(&s_full[x], 1);
-      mbar_init(&p_full[x][0], 4);
+      mbar_init(&p_full[x][0], 4);  // one arrival per softmax warp
       mbar_init(&p_full[x][1], 4);
       mbar_init(&o_done[x], 1);
+    }
+    for (int s = 0; s < kPxSlots; ++s) {
+      mbar_init(&item_full[s], 1);
+      mbar_init(&item_empty[s], kPxReaders);
     }
     sh_abort = 0;
     mbar_fence_init();
@@ -161,10 +131,129 @@ __global__ void __launch_bounds__(kPxThreads, 1)
     if (lane == 0 && atomicExch(&sh_abort, 1) == 0)
       report_error(p.err, PIEKV_ERR_WAIT_TIMEOUT, KID_SHARED_PREFIX, blockIdx.x, where);
   };
+  // item number `n` of this CTA, read by a whole warp; false after a timeout
+  auto read_item = [&](int n, Work &w, int where) -> bool {
+    const int slot = n % kPxSlots;
+    if (!wait_or_abort(&item_full[slot], (n / kPxSlots) & 1, abort_flag)) {
+      give_up(where);
+      return false;
+    }
+    w = sh_item[slot];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&item_empty[slot]);
+    return true;
+  };
 
   if (warp >= kSoftmaxWarps) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPxRegsOther));
-    if (warp == kProducerWarp || warp == kPxVWarp) {
+    if (warp == kPxSchedWarp) {
+      // ================================================================ scheduler and query rows
+      // Neither is urgent: this warp polls and sleeps instead of occupying issue slots.
+      const int items = __ldg(p.header + 2);
+      int n = 0, sched_done = 0;             // items described
+      int qn = 0, q_x = 2, q_done = 0;       // query-row cursor: item, problem (2: the item is still to be read)
+      int q_cnt[2] = {0, 0};                 // query tiles requested
+      Work qw{};
+      uint64_t idle_since = 0;
+      while (!(sched_done && q_done)) {
+        bool progressed = false;
+        if (!sched_done && __any_sync(0xffffffffu, mbar_test_wait(&item_empty[n % kPxSlots], ((n / kPxSlots) & 1) ^ 1))) {
+          int idx = blockIdx.x;  // the first item is the CTA's own, the others are claimed
+          if (n > 0) {
+            if (lane == 0) idx = ctas + atomicAdd(p.header + 4, 1);
+            idx = __shfl_sync(0xffffffffu, idx, 0);
+          }
+          Work w{};
+          if (idx < items) {
+            const int4 it = __ldg(reinterpret_cast<const int4 *>(p.items + idx));  // segment, t0, t1, piece
+            const int4 sa = __ldg(reinterpret_cast<const int4 *>(p.segments + it.x));
+            const int2 sb = __ldg(reinterpret_cast<const int2 *>(p.segments + it.x) + 2);  // (request, list, pages, head), rows
+            w.valid = 1;
+            w.list = sa.y;
+            w.pages = sa.z;
+            w.kv_head = sa.w;
+            w.pair = sb.x > p.problem;
+            w.request[0] = w.request[1] = sa.x;
+            w.rows[0] = w.rows[1] = min(sb.x, p.problem);
+            w.t0[0] = w.t0[1] = it.y;
+            w.n[0] = w.n[1] = it.z - it.y;
+            w.split[0] = w.split[1] = it.w;
+            if (w.pair) {
+              w.request[1] += p.problem / p.group;
+              w.rows[1] = min(sb.x - p.problem, p.problem);
+            } else if (p.max_splits >= 2) {
+              w.n[0] = (it.z - it.y + 1) / 2;
+              w.n[1] -= w.n[0];
+              w.t0[1] += w.n[0];
+              w.split[0] = 2 * it.w;
+              w.split[1] = 2 * it.w + 1;
+            } else {
+              w.n[1] = w.rows[1] = 0;
+            }
+          }
+          if (lane == 0) {
+            sh_item[n % kPxSlots] = w;
+            mbar_arrive(&item_full[n % kPxSlots]);  // release: the description is visible to whoever sees the phase
+          }
+          __syncwarp();
+          if (w.valid)
+            ++n;
+          else
+            sched_done = 1;
+          progressed = true;
+        }
+        if (!q_done) {
+          if (q_x == 2) {
+            if (__any_sync(0xffffffffu, mbar_test_wait(&item_full[qn % kPxSlots], (qn / kPxSlots) & 1))) {
+              qw = sh_item[qn % kPxSlots];
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&item_empty[qn % kPxSlots]);
+              ++qn;
+              if (qw.valid)
+                q_x = 0;
+              else
+                q_done = 1;
+              progressed = true;
+            }
+          } else if (qw.n[q_x] == 0) {
+            ++q_x;
+            progressed = true;
+          } else if (__any_sync(0xffffffffu, mbar_test_wait(&q_empty[q_x], (q_cnt[q_x] & 1) ^ 1))) {
+            if (lane == 0) {
+              mbar_arrive_expect_tx(&q_full[q_x], (uint32_t)(p.problem * 256));
+              const uint32_t dst = q_smem + q_x * kTileBytes;
+              tma_load_4d(dst, &tmap_q, 0, qw.kv_head * p.group, qw.request[q_x], 0, &q_full[q_x]);
+              tma_load_4d(dst + kHalfBytes, &tmap_q, 0, qw.kv_head * p.group, qw.request[q_x], 1, &q_full[q_x]);
+            }
+            ++q_cnt[q_x];
+            ++q_x;
+            progressed = true;
+          }
+        }
+        if (progressed) {
+          idle_since = 0;
+        } else {
+          __nanosleep(100);
+          if (*abort_flag) break;
+          const uint64_t now = global_timer_ns();
+          if (idle_since == 0) idle_since = now;
+          if (now - idle_since > 2000000000ull) {
+            give_up(400);
+            break;
+          }
+        }
+      }
+      // The last scheduler to leave (for want of items, or after a timeout) puts the counters back to zero for the next
+      // run: every CTA has made its final claim by then.
+      if (lane == 0 && atomicAdd(p.header + 5, 1) == ctas - 1) {
+        p.header[4] = 0;
+        p.header[5] = 0;
+      }
+      // drain: the CTA must not retire while a bulk copy may still be landing
+      if (lane == 0)
+        for (int x = 0; x < 2; ++x)
+          if (q_cnt[x] > 0) mbar_wait(&q_full[x], (q_cnt[x] - 1) & 1, 200000000ull);
+    } else if (warp == kProducerWarp || warp == kPxVWarp) {
       // ================================================================ TMA producers: K tiles / V tiles
       const bool is_v = warp == kPxVWarp;
       const uint32_t ring0 = is_v ? v_smem0 : k_smem0;
@@ -172,7 +261,10 @@ __global__ void __launch_bounds__(kPxThreads, 1)
       uint64_t *full = is_v ? v_full : k_full, *empty = is_v ? v_empty : k_empty;
       int armed = 0;
       bool ok = true;
-      for_pieces(p, blockIdx.x, share_from, share_to, [&](const Work &w) {
+      Work w;
+      for (int n = 0; ok; ++n) {
+        ok = read_item(n, w, is_v ? 120 : 100);
+        if (!ok || !w.valid) break;
         // tiles in the order they are used: shared ones, or A's and B's in turn.  A tile's page ids are loaded while the
         // ring still waits for room.
         const int total = w.pair ? w.n[0] : w.n[0] + w.n[1];
@@ -205,8 +297,7 @@ __global__ void __launch_bounds__(kPxThreads, 1)
           }
           ++armed;
         }
-        return ok;
-      });
+      }
       // drain: the CTA must not retire while a bulk copy may still be landing
       __syncwarp();
       if (lane == 0)
@@ -222,12 +313,15 @@ __global__ void __launch_bounds__(kPxThreads, 1)
         const uint64_t v_desc0 = tc::desc_mn_major(v_smem0, kHalfBytes);
         int kt = 0, vt = 0;        // tiles of the two streams consumed so far
         int done[2] = {0, 0};      // probability tiles of A and B consumed: phases of p_full
+        int qi[2] = {0, 0};        // query tiles of A and B taken so far: phases of q_full
         auto wait = [&](uint64_t *bar, int phase) { return wait_or_abort(bar, phase & 1, abort_flag); };
         auto wait_k = [&]() { return wait(&k_full[kt % kKStages], kt / kKStages); };
         auto wait_v = [&]() { return wait(&v_full[vt % kVStages], vt / kVStages); };
-        auto scores = [&](int x) {
+        // the next scores of problem x; `last` of the item's: its query rows are then no longer needed
+        auto scores = [&](int x, bool last) {
           tc::fence_after_sync();
           issue_scores(tmem + x * 128, q_desc[x], k_desc0 + (uint64_t)(((kt % kKStages) * kTileBytes) >> 4), idesc_qk, &s_full[x]);
+          if (last) tc::commit(&q_empty[x]);
         };
         auto release_k = [&]() {
           tc::commit(&k_empty[kt % kKStages]);
@@ -249,48 +343,77 @@ __global__ void __launch_bounds__(kPxThreads, 1)
           ++done[x];
           return true;
         };
-        bool ok = true;
-        int qi[2] = {0, 0};  // query tiles of A and B taken so far: phases of q_full
-        for_pieces(p, blockIdx.x, share_from, share_to, [&](const Work &w) {
-          const int na = w.n[0], nb = w.n[1];
-          ok = wait(&q_full[0], qi[0]++) && wait_k();
-          if (!ok) return false;
-          scores(0);
-          if (!w.pair) release_k();
-          if (nb > 0) {
-            ok = wait(&q_full[1], qi[1]++) && wait_k();
-            if (!ok) return false;
-            scores(1);
-            release_k();
-          }
-#pragma unroll 1
-          for (int t = 0; t < na; ++t) {
-            ok = wait_v() && pv(0, t > 0);
-            if (!ok) return false;
-            if (!w.pair) release_v();
-            if (t + 1 < na) {
-              ok = wait_k();
-              if (!ok) return false;
-              scores(0);
-              if (!w.pair) release_k();
-            } else {
-              tc::commit(&o_done[0]);
-            }
-            if (t >= nb) continue;
-            ok = wait_v() && pv(1, t > 0);
-            if (!ok) return false;
-            release_v();
-            if (t + 1 < nb) {
-              ok = wait_k();
-              if (!ok) return false;
-              scores(1);
-              release_k();
-            } else {
-              tc::commit(&o_done[1]);
-            }
-          }
+        int n = 0;
+        // the tiles of A and B of the following item; 0 when there is none, false after a timeout
+        auto next_item = [&](int &na, int &nb, bool &pair) -> bool {
+          const int slot = n % kPxSlots;
+          if (!wait(&item_full[slot], n / kPxSlots)) return false;
+          const bool valid = sh_item[slot].valid != 0;
+          na = valid ? sh_item[slot].n[0] : 0;
+          nb = valid ? sh_item[slot].n[1] : 0;
+          pair = sh_item[slot].pair != 0;
+          mbar_arrive(&item_empty[slot]);
+          ++n;
           return true;
-        });
+        };
+        // an item's first scores: A has tiles always; B's tile is A's (pair) or the next one of the stream
+        auto first_a = [&](int na, bool pair) -> bool {
+          if (!wait(&q_full[0], qi[0]++) || !wait_k()) return false;
+          scores(0, na == 1);
+          if (!pair) release_k();
+          return true;
+        };
+        auto first_b = [&](int nb) -> bool {
+          if (nb == 0) return true;
+          if (!wait(&q_full[1], qi[1]++) || !wait_k()) return false;
+          scores(1, nb == 1);
+          release_k();
+          return true;
+        };
+        int na = 0, nb = 0;
+        bool pair = false;
+        bool ok = next_item(na, nb, pair);
+        if (ok && na > 0) ok = first_a(na, pair) && first_b(nb);
+        while (ok && na > 0) {
+          int na2 = 0, nb2 = 0;
+          bool pair2 = false;
+#pragma unroll 1
+          for (int t = 0; ok && t < na; ++t) {
+            const bool last = t + 1 == na;
+            if (last) ok = next_item(na2, nb2, pair2);
+            ok = ok && wait_v() && pv(0, t > 0);
+            if (!ok) break;
+            if (!pair) release_v();
+            if (!last) {
+              ok = wait_k();
+              if (!ok) break;
+              scores(0, t + 2 == na);
+              if (!pair) release_k();
+            } else {
+              tc::commit(&o_done[0]);  // all of A's MMAs of this item
+              if (na2 > 0) ok = first_a(na2, pair2);
+              if (!ok) break;
+            }
+            if (t < nb) {
+              ok = wait_v() && pv(1, t > 0);
+              if (!ok) break;
+              release_v();
+              if (t + 1 < nb) {
+                ok = wait_k();
+                if (!ok) break;
+                scores(1, t + 2 == nb);
+                release_k();
+              } else {
+                tc::commit(&o_done[1]);
+              }
+            }
+            // (behind A's, as the tiles come: B may have ended a tile earlier)
+            if (last && na2 > 0) ok = first_b(nb2);
+          }
+          na = na2;
+          nb = nb2;
+          pair = pair2;
+        }
         if (!ok) give_up(200);
       }
     }
@@ -304,37 +427,29 @@ __global__ void __launch_bounds__(kPxThreads, 1)
     const uint32_t s_addr = tmem + lane_base + x * 128;
     const uint32_t o_addr = tmem + lane_base + 256 + x * 128;
     const float c = p.scale_log2;
+    const int member = row / p.group, g = row - member * p.group;
     int sc = 0, oc = 0;  // score tiles and items (with tiles) finished: phases of s_full and o_done
     bool ok = true;
 
-    for_pieces(p, blockIdx.x, share_from, share_to, [&](const Work &w) {
-      const int rows = w.rows[x], n = w.n[x];
+    for (int item = 0; ok; ++item) {
+      const int slot = item % kPxSlots;
+      if (!wait_or_abort(&item_full[slot], (item / kPxSlots) & 1, abort_flag)) {
+        ok = false;
+        break;
+      }
+      const int valid = sh_item[slot].valid, rows = sh_item[slot].rows[x], n = sh_item[slot].n[x];
+      const int first_tile = sh_item[slot].t0[x], limit = sh_item[slot].pages * kPage - 1;
+      const int request = sh_item[slot].request[x] + member, head = sh_item[slot].kv_head * p.group + g;
+      const size_t at = ((size_t)sh_item[slot].split[x] * p.batch + request) * p.hq + head;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&item_empty[slot]);
+      if (!valid) break;
       const bool row_valid = row < rows;
       const bool warp_valid = q4 * 32 < rows;
-      const int r = w.row0 + (w.pair ? x * kBM : 0) + row;  // row of the group
-      const int member = r / p.group, g = r - member * p.group;
-      const int request = w.request + member, head = w.kv_head * p.group + g;
-      if (n == 0) {  // (nothing is announced for it: the barriers' phases count pieces with tiles)
-        if (row_valid) p.part_ml[((size_t)w.split[x] * p.batch + request) * p.hq + head] = make_float2(-INFINITY, 0.f);
-        return true;
+      if (n == 0) {
+        if (row_valid) p.part_ml[at] = make_float2(-INFINITY, 0.f);
+        continue;
       }
-      // ---- the query row into shared memory: K-major, 128-byte swizzle.  Every MMA that read the last item's is done:
-      // this warp has seen the scores of all its tiles.
-      if (warp_valid) {
-        const uint4 *src = reinterpret_cast<const uint4 *>(reinterpret_cast<const T *>(p.q) + (int64_t)request * p.q_sn +
-                                                           (int64_t)head * p.q_sh);
-        uint4 v[16];
-#pragma unroll
-        for (int ch = 0; ch < 16; ++ch) v[ch] = row_valid ? __ldg(src + ch) : make_uint4(0, 0, 0, 0);
-        uint8_t *dst = base_ptr + x * kTileBytes + row * 128;
-#pragma unroll
-        for (int ch = 0; ch < 16; ++ch)
-          *reinterpret_cast<uint4 *>(dst + (ch >> 3) * kHalfBytes + (((ch & 7) ^ (row & 7)) << 4)) = v[ch];
-        fence_proxy_async_smem();
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&q_full[x]);
-      const int limit = w.pages * kPage - 1;
       float m_ref = -INFINITY, l = 0.f;
       for (int t = 0; t < n; ++t) {
         ok = wait_or_abort(&s_full[x], sc & 1, abort_flag);
@@ -348,7 +463,7 @@ __global__ void __launch_bounds__(kPxThreads, 1)
           continue;
         }
         tc::fence_after_sync();
-        const int k0 = (w.t0[x] + t) * kBN;
+        const int k0 = (first_tile + t) * kBN;
         const bool full_tile = k0 + kBN - 1 <= limit;
         uint4 mw = make_uint4(0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu);
         if (!full_tile) mw = band_bits(k0, 0, 0, limit);
@@ -421,11 +536,10 @@ __global__ void __launch_bounds__(kPxThreads, 1)
       // ---- the partial result.  The next item's O_x is not written before this warp has delivered that item's first
       // probabilities.
       if (ok) ok = wait_or_abort(&o_done[x], oc & 1, abort_flag);
-      if (!ok) return false;
+      if (!ok) break;
       ++oc;
-      if (!warp_valid) return true;
+      if (!warp_valid) continue;
       tc::fence_after_sync();
-      const size_t at = ((size_t)w.split[x] * p.batch + request) * p.hq + head;
 #pragma unroll 1
       for (int ch = 0; ch < 4; ++ch) {
         uint32_t oreg[32];
@@ -443,8 +557,7 @@ __global__ void __launch_bounds__(kPxThreads, 1)
         }
       }
       if (row_valid) p.part_ml[at] = make_float2(m_ref, l);
-      return true;
-    });
+    }
     if (!ok) give_up(300 + warp);
   }
 
@@ -458,11 +571,11 @@ __global__ void __launch_bounds__(kPxThreads, 1)
 }
 
 template <typename T>
-int launch_t(const CUtensorMap &tkv, const PrefixTcParams &p, cudaStream_t st) {
+int launch_t(const CUtensorMap &tq, const CUtensorMap &tkv, const PrefixTcParams &p, cudaStream_t st) {
   static unsigned char configured[kMaxDevices] = {0};
   if (int rc = opt_in_dynamic_smem(prefix_tc_kernel<T>, kPxSmemBytes, configured, "shared prefix: cudaFuncSetAttribute"))
     return rc;
-  prefix_tc_kernel<T><<<sm_count(), kPxThreads, kPxSmemBytes, st>>>(tkv, p);
+  prefix_tc_kernel<T><<<sm_count(), kPxThreads, kPxSmemBytes, st>>>(tq, tkv, p);
   PIEKV_LAUNCH_CHECK("prefix_tc_kernel");
   return 0;
 }
@@ -470,9 +583,10 @@ int launch_t(const CUtensorMap &tkv, const PrefixTcParams &p, cudaStream_t st) {
 }  // namespace
 
 int launch_prefix_tc(const PrefixTcParams &p, const void *pool, int hkv, int dtype, cudaStream_t st) {
-  CUtensorMap tkv;
+  CUtensorMap tq, tkv;
+  if (int rc = make_q_rows_tensor_map(&tq, p.q, p.batch, p.hq, p.q_sn, p.q_sh, dtype, p.group, p.problem / p.group)) return rc;
   if (int rc = make_page_tensor_map(&tkv, pool, p.num_pages, hkv, dtype, 1, 1, 1)) return rc;
-  return dtype == PIEKV_BF16 ? launch_t<__nv_bfloat16>(tkv, p, st) : launch_t<__half>(tkv, p, st);
+  return dtype == PIEKV_BF16 ? launch_t<__nv_bfloat16>(tq, tkv, p, st) : launch_t<__half>(tq, tkv, p, st);
 }
 
 }  // namespace piekv

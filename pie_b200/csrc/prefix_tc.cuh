@@ -8,11 +8,13 @@ struct PrefixTcParams {
   const void *q;  // [batch, Hq, 128], rows 16-byte aligned
   int64_t q_sn, q_sh;
   const int32_t *kv_indices;
-  const int2 *starts;  // the plan's
+  int *header;  // the plan's
   const sprefix::Segment *segments;
+  const sprefix::Item *items;
   float *part_o;    // [split][batch][Hq][128], unnormalised
   float2 *part_ml;  // [split][batch][Hq]: reference maximum (log2 units), sum
   int batch, hq, group, num_pages, max_splits;
+  int problem;      // rows of one MMA problem: whole requests
   float scale_log2;
   int32_t *err;
 };

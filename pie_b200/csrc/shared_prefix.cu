@@ -60,34 +60,34 @@ __global__ void __launch_bounds__(128) sp_match_kernel(const int32_t *__restrict
   if (threadIdx.x == 0) match[b] = sh_first;
 }
 
-// The line that the CTAs' shares divide, in units of 0.3 us as measured on the prefix kernel: a tile against at most 128
-// rows (bound by its stream) or more (by the tensor and special-function pipes), and opening and closing a piece.
-constexpr int kTileSingle = 5, kTilePair = 8, kOpen = 22;
-// The same units for the choice of how many SMs work on prefixes: starting that kernel, starting the other one beside it
-// or behind it, a tile's worth of own pages there, and one row of partial results folded by an SM.  Two kernels that
-// stream at the same time slow each other down by up to kContention.
-constexpr float kStartPrefix = 16.f, kStartBeside = 24.f, kStartBehind = 90.f, kOwnTile = 6.f, kFoldRow = 0.03f;
-constexpr float kContention = 0.3f;
+// Costs in units of 0.3 us, as measured on the two attention kernels.  Prefix kernel: starting it, a tile against one
+// problem's rows (bound by its stream) or two (by the tensor and special-function pipes), an item's own costs.  The
+// other kernel: starting it beside the prefix kernel or behind it, a tile's worth of own pages; a warp's step of the join
+// (four rows, four partial results), of which an SM has kFoldWarps under way.  Two kernels that stream at the same time
+// slow each other down by up to kContention.
+constexpr float kStartPrefix = 16.f, kTileSingle = 5.f, kTilePair = 7.5f, kOpenItem = 6.f;
+constexpr float kStartBeside = 24.f, kStartBehind = 90.f, kOwnTile = 6.f, kFoldStep = 4.5f, kFoldWarps = 8.f, kContention = 0.3f;
+constexpr int kMaxSearchGroups = 256;
 
-// Checks the grouping, decides what every group reads once, how many SMs work on that while the others stream the
-// requests' own pages, and where each CTA's share of the prefixes starts.  One block.
+// Checks the grouping, decides what every group reads once, how many CTAs work on that while the other SMs stream the
+// requests' own pages, and into how many items each prefix is cut; CTAs claim items.  One block.
 //
-// More CTAs on the prefixes leave fewer SMs to the other kernel, which runs at the same time, and cut them into more
-// pieces, whose partial results have to be folded.  Thread x costs x + 1 CTAs with the constants above; the cheapest
-// is taken.  Shares are equal parts of the line, so no CTA has more than its part whatever the prefixes' lengths.
+// More CTAs on the prefixes leave fewer SMs to the other kernel, which runs at the same time; more items balance the
+// CTAs (not all SMs are equally fast under this load: by a third on some parts) but leave more partial results to fold.
+// Each thread costs one (CTAs, tiles per item) pair with the constants above; the cheapest is taken.
 __global__ void __launch_bounds__(1024) sp_plan_kernel(const int32_t *__restrict__ kv_indptr,
                                                        const int32_t *__restrict__ group_indptr, int batch, int groups,
                                                        int page_size, int heads_per_kv, int hkv, int max_splits,
                                                        int sms, PlanView v, int32_t *err) {
-  __shared__ unsigned long long sh_own, sh_best, sh_longest, sh_rows, sh_row_len;
-  __shared__ long long sh_scan[32][2], sh_carry[2];
-  __shared__ int sh_used;
+  __shared__ unsigned long long sh_own, sh_best;
+  __shared__ int sh_scan[32], sh_carry, sh_most, sh_used, sh_items;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (tid == 0) {
-    sh_own = sh_longest = sh_rows = sh_row_len = 0;
+    sh_own = 0;
     sh_best = ~0ull;
-    sh_used = 0;
-    sh_carry[0] = sh_carry[1] = 0;
+    sh_carry = sh_most = sh_used = sh_items = 0;
+    for (int i = 0; i < 6; ++i) v.header[i] = 0;
+    v.header[3] = sms;
   }
   int bad = -1;
   for (int g = tid; g < groups; g += 1024) {
@@ -98,21 +98,16 @@ __global__ void __launch_bounds__(1024) sp_plan_kernel(const int32_t *__restrict
   const bool refused = __syncthreads_or(bad >= 0) != 0;
   if (refused) {  // every request on its own
     for (int b = tid; b < batch; b += 1024) v.requests[b] = make_int2(0, 0);
-    for (int c = tid; c <= sms; c += 1024) v.starts[c] = make_int2(0, 0);
-    if (tid == 0) {
-      v.header[0] = v.header[1] = v.header[2] = 0;
-      v.header[3] = sms;
-    }
     return;
   }
+  const int problem = problem_rows(heads_per_kv), block_members = 2 * problem / heads_per_kv;
   auto tiles_of = [&](int pages) { return (int)(((long long)pages * page_size + kTileTokens - 1) / kTileTokens); };
-  // blocks of more than 128 rows, and whether a smaller one is left
-  auto pair_blocks = [&](int members) { return (int)(((long long)members * heads_per_kv + kRowsPerBlock / 2 - 1) / kRowsPerBlock); };
-  auto single_blocks = [&](int members) {
-    const int left = (int)((long long)members * heads_per_kv % kRowsPerBlock);
-    return left > 0 && left <= kRowsPerBlock / 2 ? 1 : 0;
+  auto blocks_of = [&](int members) { return (members + block_members - 1) / block_members; };
+  // whether the last block is one problem
+  auto last_single = [&](int members) {
+    const int left = members % block_members;
+    return left > 0 && left * heads_per_kv <= problem ? 1 : 0;
   };
-  auto length = [&](int tiles, bool pair) { return (long long)tiles * (pair ? kTilePair : kTileSingle) + kOpen; };
   // ---- a warp per group: pages common to all its requests, pages left to each
   for (int g = warp; g < groups; g += 32) {
     const int a = group_indptr[g], m = group_indptr[g + 1] - a;
@@ -133,140 +128,104 @@ __global__ void __launch_bounds__(1024) sp_plan_kernel(const int32_t *__restrict
       v.groups[g] = Group{a, m, pages, 0};
       atomicAdd(&sh_own, (unsigned long long)(own - (long long)m * pages));
       if (pages > 0) {
-        const int tiles = tiles_of(pages), pb = pair_blocks(m), sb = single_blocks(m);
-        const long long rows_single = sb ? (long long)m * heads_per_kv - (long long)pb * kRowsPerBlock : 0;
-        const long long rows_pair = (long long)m * heads_per_kv - rows_single;
-        atomicMax(&sh_longest, (unsigned long long)length(tiles, pb > 0));
-        atomicAdd(&sh_rows, (unsigned long long)(rows_pair + 2 * rows_single));
-        atomicAdd(&sh_row_len, (unsigned long long)(rows_pair * length(tiles, true) + 2 * rows_single * length(tiles, false)));
+        atomicMax(&sh_most, tiles_of(pages));
         atomicAdd(&sh_used, 1);
       }
     }
   }
   __syncthreads();
-  // ---- the line: segments and lengths of the groups, scanned in order
+  // ---- segments, numbered in the groups' order
   for (int g0 = 0; g0 < groups; g0 += 1024) {
     const int g = g0 + tid;
-    long long x[2] = {0, 0};
-    if (g < groups && v.groups[g].pages > 0) {
+    const int own = g < groups && v.groups[g].pages > 0 ? blocks_of(v.groups[g].members) * hkv : 0;
+    int x = own;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, d);
+      if (lane >= d) x += y;
+    }
+    if (lane == 31) sh_scan[warp] = x;
+    __syncthreads();
+    for (int w = 0; w < warp; ++w) x += sh_scan[w];
+    x += sh_carry;
+    if (g < groups) v.groups[g].segment = x - own;
+    __syncthreads();
+    if (tid == 1023) sh_carry = x;
+    __syncthreads();
+  }
+  const int segments = sh_carry;
+  if (segments == 0) return;
+  // ---- thread = (CTAs: 32 steps up to all SMs, tiles per item: the longest prefix in 1 .. 32 pieces)
+  const int most = sh_most, max_pieces = max(1, max_splits / 2);
+  auto pieces_of = [&](int tiles, int per) { return min((tiles + per - 1) / per, max_pieces); };
+  int ctas = max(1, sms * (warp + 1) / 32), per = (most + lane) / (lane + 1);
+  if (groups <= kMaxSearchGroups) {
+    const float row_steps = (float)((heads_per_kv + 3) / 4);
+    float work = 0.f, folds = 0.f, longest = 0.f, longest_fold = 0.f;
+    long long items = 0;
+    for (int g = 0; g < groups; ++g) {
       const Group gr = v.groups[g];
-      const int tiles = tiles_of(gr.pages), pb = pair_blocks(gr.members), sb = single_blocks(gr.members);
-      x[0] = (long long)(pb + sb) * hkv;
-      x[1] = hkv * (pb * length(tiles, true) + sb * length(tiles, false));
+      if (gr.pages == 0) continue;
+      const int tiles = tiles_of(gr.pages), pieces = pieces_of(tiles, per), blocks = blocks_of(gr.members);
+      const int single = last_single(gr.members);
+      // join steps of a request: its own result and the prefix's
+      const int members_single = single ? gr.members % block_members : 0;
+      const float fold = row_steps * (float)((pieces + 4) / 4);
+      const float fold_single = row_steps * (float)(((max_splits >= 2 ? 2 : 1) * pieces + 4) / 4);
+      items += (long long)blocks * pieces;
+      work += (float)tiles * ((float)(blocks - single) * kTilePair + (float)single * kTileSingle);
+      folds += (float)(gr.members - members_single) * fold + (float)members_single * fold_single;
+      longest_fold = fmaxf(longest_fold, single ? fold_single : fold);
+      longest = fmaxf(longest, (float)tiles / (float)pieces * (blocks > single ? kTilePair : kTileSingle));
     }
-    const long long own[2] = {x[0], x[1]};
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const long long y = __shfl_up_sync(0xffffffffu, x[k], d);
-        if (lane >= d) x[k] += y;
-      }
-      if (lane == 31) sh_scan[warp][k] = x[k];
+    if (items * hkv <= segments + kSpareItems) {
+      const int n = (int)min((long long)ctas, items * hkv), left = n < sms ? sms - n : sms;
+      const float own = (n < sms ? kStartBeside : kStartBehind) +
+                        (float)((double)sh_own * page_size / kTileTokens * hkv) * kOwnTile / (float)left;
+      float prefix = (work + (float)items * kOpenItem) * (float)hkv / (float)n;
+      // claimed items end within one item of each other; fewer items than CTAs: one each
+      prefix = items * hkv <= n ? longest + kOpenItem : prefix + 0.5f * (longest + kOpenItem);
+      if (n < sms) prefix *= 1.f + kContention * fminf(1.f, own / prefix);
+      prefix += kStartPrefix;
+      const float cost = (n < sms ? fmaxf(prefix, own) : prefix + own) +
+                         kFoldStep * fmaxf(longest_fold, folds * (float)hkv / ((float)left * kFoldWarps));
+      atomicMin(&sh_best, ((unsigned long long)__float_as_uint(cost) << 32) | (unsigned)tid);
     }
-    __syncthreads();
-    for (int k = 0; k < 2; ++k) {
-      for (int w = 0; w < warp; ++w) x[k] += sh_scan[w][k];
-      x[k] += sh_carry[k];
-    }
-    if (g < groups) {
-      v.groups[g].segment = (int)(x[0] - own[0]);
-      v.line[g] = x[1] - own[1];
-    }
-    __syncthreads();
-    if (tid == 1023) {
-      sh_carry[0] = x[0];
-      sh_carry[1] = x[1];
-    }
-    __syncthreads();
-  }
-  const long long line = sh_carry[1];
-  const int segments = (int)sh_carry[0];
-  if (line == 0) {
-    for (int c = tid; c <= sms; c += 1024) v.starts[c] = make_int2(0, 0);
-    if (tid == 0) {
-      v.header[0] = v.header[1] = v.header[2] = 0;
-      v.header[3] = sms;
-    }
-    return;
-  }
-  // ---- how many CTAs.  A share holds a tile at least; no segment is cut into more pieces than there is room for.
-  const int max_pieces = max(1, max_splits / 2);
-  const bool cut = max_pieces >= 3;
-  long long most = min((long long)sms, max(1ll, line / (kOpen + kTilePair)));
-  if (cut) most = max(1ll, min(most, (max_pieces - 2) * line / (long long)sh_longest));
-  if (tid < (int)most) {
-    const int n = tid + 1, left = n < sms ? sms - n : sms;
-    const float own = (n < sms ? kStartBeside : kStartBehind) +
-                      (float)((double)sh_own * page_size / kTileTokens * hkv) * kOwnTile / (float)left;
-    // a share that starts inside a segment opens one piece more than the line counts, one that is not an even part of
-    // the segments (or a whole number of them) two
-    const bool even = n % segments == 0 || segments % n == 0;
-    float prefix = fmaxf((float)line / (float)n, cut ? 0.f : (float)sh_longest) + (even ? kOpen : 2 * kOpen);
-    if (n < sms) prefix *= 1.f + kContention * fminf(1.f, own / prefix);
-    prefix += kStartPrefix;
-    const float fold = kFoldRow * (float)hkv / (float)left * ((float)sh_rows + (cut ? (float)sh_row_len * (float)n / (float)line : 0.f));
-    const float cost = (n < sms ? fmaxf(prefix, own) : prefix + own) + fold;
-    atomicMin(&sh_best, ((unsigned long long)__float_as_uint(cost) << 32) | (unsigned)tid);
   }
   __syncthreads();
-  const int ctas = (int)(sh_best & 0xffffffffu) + 1;
-  auto share_of = [&](long long x) { return (int)(((x + 1) * ctas - 1) / line); };
+  // hundreds of groups are pieces enough: all SMs, whole prefixes
+  const int best = sh_best == ~0ull ? 31 * 32 : (int)(sh_best & 1023);
+  ctas = max(1, sms * (best / 32 + 1) / 32);
+  per = (most + best % 32) / (best % 32 + 1);
   for (int g = warp; g < groups; g += 32) {
     const Group gr = v.groups[g];
     if (gr.pages == 0) continue;
-    const int pb = pair_blocks(gr.members), blocks = pb + single_blocks(gr.members), tiles = tiles_of(gr.pages);
-    for (int i = lane; i < blocks * hkv; i += 32) {
+    const int blocks = blocks_of(gr.members), tiles = tiles_of(gr.pages), n = blocks * hkv;
+    int pieces = pieces_of(tiles, per), at = 0;
+    if (lane == 0) at = atomicAdd(&sh_items, n * pieces);
+    at = __shfl_sync(0xffffffffu, at, 0);
+    if (at + n * pieces > v.max_segments + kSpareItems) {  // (cannot happen: nothing is written out of range)
+      if (lane == 0) report_error(err, PIEKV_ERR_PAGE_CAPACITY, KID_SHARED_PREFIX, g, pieces);
+      pieces = 0;
+    }
+    for (int i = lane; i < n; i += 32) {
       const int block = i / hkv;
-      const bool pair = block < pb;
-      const long long at = v.line[g] + min(i, pb * hkv) * length(tiles, true) + max(0, i - pb * hkv) * length(tiles, false);
-      const int first = cut ? share_of(at + kOpen) : 0;
-      const int last = cut ? share_of(at + kOpen + (long long)(tiles - 1) * (pair ? kTilePair : kTileSingle)) : 0;
-      v.segments[gr.segment + i] = Segment{gr.first, kv_indptr[gr.first], gr.pages, i % hkv, block * kRowsPerBlock,
-                                           gr.members * heads_per_kv - block * kRowsPerBlock, first, last - first + 1};
+      v.segments[gr.segment + i] = Segment{gr.first + block * block_members, kv_indptr[gr.first], gr.pages, i % hkv,
+                                           (gr.members - block * block_members) * heads_per_kv, pieces, {0, 0}};
+    }
+    for (int i = lane; i < n * pieces; i += 32) {
+      const int piece = i / n;
+      v.items[at + i] = Item{gr.segment + i % n, (int)((long long)tiles * piece / pieces),
+                             (int)((long long)tiles * (piece + 1) / pieces), piece};
     }
   }
-  for (int c = tid; c <= sms; c += 1024) {  // (CTAs behind the last share start where they end)
-    const long long x = c < ctas ? line * c / ctas : 0;
-    int lo = 0, hi = groups - 1;  // last group whose start is <= x (of equal starts the one with a prefix: the last)
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (v.line[mid] <= x)
-        lo = mid;
-      else
-        hi = mid - 1;
-    }
-    int2 start = make_int2(segments, 0);
-    if (c < ctas) {
-      const Group gr = v.groups[lo];
-      const int tiles = tiles_of(gr.pages);
-      const long long in_pairs = (long long)pair_blocks(gr.members) * hkv * length(tiles, true);
-      long long y = x - v.line[lo];
-      int seg = gr.segment;
-      const bool pair = y < in_pairs;
-      if (!pair) {
-        seg += pair_blocks(gr.members) * hkv;
-        y -= in_pairs;
-      }
-      seg += (int)(y / length(tiles, pair));
-      y %= length(tiles, pair);
-      const int step = pair ? kTilePair : kTileSingle;
-      // tiles whose first unit lies before x belong to the share before
-      int tile = y <= kOpen ? 0 : (int)((y - kOpen + step - 1) / step);
-      if (!cut) tile = y > 0 ? tiles : 0;
-      if (tile >= tiles) {
-        ++seg;
-        tile = 0;
-      }
-      start = make_int2(seg, tile);
-    }
-    v.starts[c] = start;
-  }
+  __syncthreads();
   if (tid == 0) {
-    v.header[0] = ctas;
+    const int items = min(sh_items, v.max_segments + kSpareItems);
+    v.header[0] = min(ctas, items);
     v.header[1] = sh_used;
-    v.header[2] = segments;
-    v.header[3] = ctas < sms ? sms - ctas : sms;
+    v.header[2] = items;
+    v.header[3] = v.header[0] < sms ? sms - v.header[0] : sms;
   }
 }
 
@@ -317,14 +276,14 @@ extern "C" int piekv_shared_prefix_plan(const piekv_shared_prefix_args *args, vo
   if (int rc = check_args(args, "shared_prefix_plan")) return rc;
   const piekv_shared_prefix_args &a = *args;
   if (a.batch == 0) return 0;
-  PIEKV_REQUIRE(sm_count() <= kMaxCtas, "shared_prefix_plan: %d SMs, the plan holds %d shares", sm_count(), kMaxCtas);
   const PlanView v = plan_view(a.plan, a.batch, a.num_groups, a.num_qo_heads, a.num_kv_heads);
   cudaStream_t st = (cudaStream_t)stream;
   sp_match_kernel<<<a.batch, 128, 0, st>>>(a.kv_indptr, a.kv_indices, a.kv_last_page_len, a.group_indptr, a.batch,
                                            a.num_groups, a.page_size, v.match);
   PIEKV_LAUNCH_CHECK("sp_match_kernel");
+  const int group = a.num_qo_heads / a.num_kv_heads;  // (more than 16 heads run the general kernel, which needs no items)
   sp_plan_kernel<<<1, 1024, 0, st>>>(a.kv_indptr, a.group_indptr, a.batch, a.num_groups, a.page_size,
-                                     a.num_qo_heads / a.num_kv_heads, a.num_kv_heads, a.max_splits, sm_count(), v, a.err);
+                                     group < 16 ? group : 16, a.num_kv_heads, a.max_splits, sm_count(), v, a.err);
   PIEKV_LAUNCH_CHECK("sp_plan_kernel");
   return 0;
 }
@@ -354,8 +313,8 @@ extern "C" int piekv_shared_prefix_run(const piekv_shared_prefix_args *args, voi
   a.err = args->err;
   a.sinks = args->sinks;
   cudaStream_t st = (cudaStream_t)stream;
-  // a thread of the prefix kernel brings a query row in by 16-byte loads
-  const bool rows16 = (reinterpret_cast<uintptr_t>(a.q) & 15) == 0 && (a.q_sn & 7) == 0 && (a.q_sh & 7) == 0;
+  // the prefix kernel brings query rows in by TMA
+  const bool rows16 = (reinterpret_cast<uintptr_t>(a.q) & 15) == 0 && (a.q_sn & 7) == 0 && (a.q_sh & 7) == 0 && a.q_sn > 0 && a.q_sh > 0;
   if (!decode_span_supported(a, args->dtype) || !rows16) return launch_attn_generic(a, args->dtype, st);
   const int64_t need = piekv_shared_prefix_workspace_bytes(a.batch, a.hq, a.hkv, a.dim, args->max_splits);
   PIEKV_REQUIRE(args->workspace != nullptr && args->workspace_bytes >= need,
@@ -371,13 +330,15 @@ extern "C" int piekv_shared_prefix_run(const piekv_shared_prefix_args *args, voi
   px.q_sn = a.q_sn;
   px.q_sh = a.q_sh;
   px.kv_indices = a.kv_indices;
-  px.starts = v.starts;
+  px.header = v.header;
   px.segments = v.segments;
+  px.items = v.items;
   px.part_ml = reinterpret_cast<float2 *>(ws);
   px.part_o = reinterpret_cast<float *>(ws + prefix_ml_bytes(a.batch, a.hq, args->max_splits));
   px.batch = a.batch;
   px.hq = a.hq;
   px.group = a.hq / a.hkv;
+  px.problem = problem_rows(px.group);
   px.num_pages = a.num_pages;
   px.max_splits = args->max_splits;
   px.scale_log2 = a.sm_scale * 1.4426950408889634f;

@@ -56,6 +56,20 @@ int make_q_tensor_map(CUtensorMap *tm, const void *q, int64_t nnz, int hq, int64
 }
 
 
+int make_q_rows_tensor_map(CUtensorMap *tm, const void *q, int64_t n, int hq, int64_t q_sn, int64_t q_sh, int dtype,
+                           int box_heads, int box_tokens) {
+  EncodeTiledFn enc = get_encode_fn();
+  PIEKV_REQUIRE(enc != nullptr, "cuTensorMapEncodeTiled is not available from the driver");
+  cuuint64_t gdim[4] = {64, (cuuint64_t)hq, (cuuint64_t)n, 2};
+  cuuint64_t gstr[3] = {(cuuint64_t)q_sh * 2, (cuuint64_t)q_sn * 2, 128};
+  cuuint32_t box[4] = {64, (cuuint32_t)box_heads, (cuuint32_t)box_tokens, 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  CUresult r = enc(tm, tm_dtype(dtype), 4, const_cast<void *>(q), gdim, gstr, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  PIEKV_REQUIRE(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled (query rows) failed with CUresult %d", (int)r);
+  return 0;
+}
+
 int make_matrix_tensor_map(CUtensorMap *tm, const void *ptr, int64_t rows, int64_t cols, int64_t row_stride, int dtype,
                            int box_rows, int box_cols) {
   EncodeTiledFn enc = get_encode_fn();

@@ -16,6 +16,11 @@ int make_page_tensor_map(CUtensorMap *tm, const void *pool, int num_pages, int h
 int make_q_tensor_map(CUtensorMap *tm, const void *q, int64_t nnz, int hq, int64_t q_sn, int64_t q_sh, int dtype,
                       int box_rows, int box_heads = 1, int box_halves = 2);
 
+// q [n, Hq, 128] seen as {64 d, Hq, n, 2 d-halves}; box {64, heads, tokens, 1}: shared memory receives rows token * heads +
+// head of one d-half.
+int make_q_rows_tensor_map(CUtensorMap *tm, const void *q, int64_t n, int hq, int64_t q_sn, int64_t q_sh, int dtype,
+                           int box_heads, int box_tokens);
+
 // Row-major matrix [rows, cols] of 16-bit elements (row stride in elements) seen as {cols, rows}; box
 // {box_cols (64: one 128-byte swizzled row), box_rows}: shared memory receives [box_rows][64], K-major.
 int make_matrix_tensor_map(CUtensorMap *tm, const void *ptr, int64_t rows, int64_t cols, int64_t row_stride, int dtype,

@@ -208,6 +208,10 @@ def test_sinks_scale_strides_and_out():
     assert got[0] is out
     b.check(got, sinks=sinks, sm_scale=0.2)
     b.check(w.run(q, b.pool.cuda(), return_lse=True, sm_scale=0.05), sm_scale=0.05)
+    same = b.q[:1].cuda().expand(4, 8, 128)  # one row for all requests: stride 0
+    b2, b.q = b.q, same.cpu()
+    b.check(w.run(same, b.pool.cuda(), return_lse=True), sm_scale=0.2)
+    b.q = b2
     odd = torch.empty(4 * 8 * 128 + 1, dtype=torch.bfloat16, device="cuda")[1:].view(4, 8, 128)  # 2-byte aligned rows
     odd.copy_(q)
     b.check(w.run(odd, b.pool.cuda(), return_lse=True), sm_scale=0.2)
