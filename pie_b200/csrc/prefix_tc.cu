@@ -10,9 +10,13 @@
 // the request's own pages (decode_span.cu): M = max m_i, L = sum l_i 2^(m_i - M), O = sum O_i 2^(m_i - M).
 //
 // What bounds it: with R rows per kv head a prefix token costs 4 * 128 * R flops and 512 bytes, so the tensor and
-// special-function pipes from about 200 rows on, HBM below.  A tile against two problems takes 2.0 us on the faster SMs
-// and 2.7 on the slower ones (half of them, under this load), which is why items are claimed: with equal shares per CTA
-// the fast ones stood idle for a third of the launch (67 against 110 us on 16384 shared tokens, 128 requests of 64 heads).
+// special-function pipes from about 200 rows on, HBM below.  A tile against two problems takes 2.1 us; on some boards
+// half of the SMs take 2.7 under this load, which is why items are claimed instead of dealt out (with equal shares per
+// CTA the fast ones stood idle for a third of the launch there: ends between 67 and 110 us).
+// Measured, with the kernel beside it: 16384 shared tokens, 128 requests, 64 / 8 heads, fp16, up to 512 tokens of their
+// own (70 GFLOP, 202 MB): 112 us, 0.62 PFLOP/s; of it 3.5 until the first scores, 92 for 43 tiles (96 CTAs), 4 to store
+// rows, 12 for the joins.
+// 64 requests behind 4096 tokens with 1024 of their own, 32 / 8 heads: 43 us (158 MB); 16 prompts of 4 beams: 33 us.
 //
 //   TMEM (512 columns): S_A/P_A [0,128)  S_B/P_B [128,256)  O_A [256,384)  O_B [384,512)
 //   smem: Q_A, Q_B (32 KiB each), K ring (3 x 32 KiB), V ring (2 x 32 KiB)

@@ -223,7 +223,9 @@ __global__ void __launch_bounds__(kThreads, 3) rope_axes_rows_kernel(const __gri
 // for bandwidth: rows move by bulk copies, global to shared memory and back, a ring of stages per block, and only the
 // rotation itself passes through registers - in place in the stage; v never does.  A block's positions and page rows
 // are looked up 128 tokens at a time, (cos, sin) of the next token are formed while the copies of this one fly.
-// Measured (20480 tokens, 32 q / 8 kv heads, bf16, 504 MB): see kBulkBlocks.
+// Measured (20480 tokens, 32 q / 8 kv heads, bf16, 504 MB moved): 92.6 us, 5.4 TB/s, 0.83 of the copy rate.  Blocks per
+// SM: 3 of 50 KB 119.6 us, 5 92.8, 6 98.4; 256 threads 95.4, 64 threads and 8 blocks 108.5.  Rows through registers
+// instead of the ring (the kernel for few tokens): 297.
 constexpr int kBulkThreads = 128;
 constexpr int kBulkChunk = 128;
 constexpr int kMaxStages = 4;
