@@ -385,14 +385,16 @@ extern "C" int piekv_prefill_run_opt(const void *q, int64_t q_stride_n, int64_t 
     a.mask = reinterpret_cast<const uint8_t *>(workspace);  // marks "masked"; the packed form is what is read
     a.causal = 0;
   }
-  if (prefill_tc_supported(a, dtype)) {
+  // (with a band the tensor-core kernels take a row's maximum before they scale it)
+  if (prefill_tc_supported(a, dtype) && (a.first_tokens == 0 || a.sm_scale > 0.f)) {
     if (!planned) {
       AttnArgs pa = a;
       if (a.first_tokens > 0) pa.window_left = -1;  // the kernel applies the window itself
       if (int rc = launch_prefill_plan(pa, mask_bytes, workspace, workspace_bytes, (cudaStream_t)stream)) return rc;
     }
     // with a window alone the plan holds a packed mask even when the caller passed none
-    if (a.first_tokens == 0 && a.window_left >= 0 && a.mask == nullptr && mask_bytes > 0) a.mask = reinterpret_cast<const uint8_t *>(workspace);
+    if (a.first_tokens == 0 && a.window_left >= 0 && a.mask == nullptr && mask_bytes > 0)
+      a.mask = reinterpret_cast<const uint8_t *>(workspace);
     return launch_prefill_tc(a, dtype, mask_bytes, workspace, workspace_bytes, (cudaStream_t)stream);
   }
   return launch_attn_generic(a, dtype, (cudaStream_t)stream);

@@ -313,9 +313,11 @@ extern "C" int piekv_shared_prefix_run(const piekv_shared_prefix_args *args, voi
   a.err = args->err;
   a.sinks = args->sinks;
   cudaStream_t st = (cudaStream_t)stream;
-  // the prefix kernel brings query rows in by TMA
-  const bool rows16 = (reinterpret_cast<uintptr_t>(a.q) & 15) == 0 && (a.q_sn & 7) == 0 && (a.q_sh & 7) == 0 && a.q_sn > 0 && a.q_sh > 0;
-  if (!decode_span_supported(a, args->dtype) || !rows16) return launch_attn_generic(a, args->dtype, st);
+  // the prefix kernel brings query rows in by TMA, and takes the maximum of a row before it scales it
+  const bool rows16 = (reinterpret_cast<uintptr_t>(a.q) & 15) == 0 && (a.q_sn & 7) == 0 && (a.q_sh & 7) == 0 &&
+                      a.q_sn > 0 && a.q_sh > 0;
+  if (!decode_span_supported(a, args->dtype) || !rows16 || !(a.sm_scale > 0.f))
+    return launch_attn_generic(a, args->dtype, st);
   const int64_t need = piekv_shared_prefix_workspace_bytes(a.batch, a.hq, a.hkv, a.dim, args->max_splits);
   PIEKV_REQUIRE(args->workspace != nullptr && args->workspace_bytes >= need,
                 "shared_prefix_run: workspace too small (%lld < %lld bytes)", (long long)args->workspace_bytes,

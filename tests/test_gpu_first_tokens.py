@@ -267,6 +267,19 @@ def test_prefill_long_context():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("scale", [-0.1, 0.0])
+@pytest.mark.parametrize("hq, hkv", [(8, 2), (6, 2)])
+def test_scales_that_are_not_positive(scale, hq, hkv):
+    for new in (1, 40):
+        sc = make_scenario(hq, hkv, 128, torch.bfloat16, [(200, new), (0, new), (33, new)])
+        m = sc.meta
+        got = (_decode if new == 1 else _prefill)(sc, 50, 5, sm_scale=scale)
+        ref = P.attend(sc.q, sc.pool, m.qo_indptr, m.kv_indptr, m.kv_indices, m.kv_last_page_len, sm_scale=scale,
+                       window_left=50, first_tokens=5)
+        P.check_attention(got[0], got[1], sc.q, sc.pool, ref, scale=abs(scale))
+
+
+@pytest.mark.gpu
 def test_prefill_sinks_and_the_sink_wrapper():
     sc = make_scenario(8, 2, 128, torch.bfloat16, [(300, 40), (0, 150)])
     g = torch.Generator().manual_seed(1)

@@ -218,6 +218,14 @@ def test_sinks_scale_strides_and_out():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("scale", [-0.1, 0.0, 1e-30])
+def test_scales_that_are_not_positive(scale):
+    b = Batch([(30, [5, 40, 0]), (0, [9])], 8, 2)
+    got = _run(b, sm_scale=scale)
+    P.check_attention(got[0], got[1], b.q, b.pool, b.reference(sm_scale=scale), scale=abs(scale))
+
+
+@pytest.mark.gpu
 def test_large_scores_and_peaked_rows():
     """Scores in the hundreds: the join of prefix and suffix must not overflow, whichever part holds the maximum."""
     b = Batch([(40, [20, 50, 0])], 8, 2, seed=8)
