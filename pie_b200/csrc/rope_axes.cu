@@ -282,7 +282,8 @@ __global__ void __launch_bounds__(kBulkThreads) rope_axes_bulk_kernel(const __gr
   const int ch = threadIdx.x;
   const int e0 = kNeighbours ? 2 * ch * VEC : ch * VEC, e1 = kNeighbours ? e0 + VEC : e0 + half;
   bool ok = true;
-  for (int i = 0; i < count; ++i) {
+  int i = 0;
+  for (; i < count; ++i) {
     if (i % kBulkChunk == 0) {
       __syncthreads();  // nobody still reads the last chunk's (and, the first time, the barriers are ready)
       for (int j = tid; j < kBulkChunk && i + j < count; j += threads) {
@@ -296,7 +297,7 @@ __global__ void __launch_bounds__(kBulkThreads) rope_axes_bulk_kernel(const __gr
     }
     const int s = i % stages;
     uint8_t *stage = smem + s * stage_bytes;
-    if (ok) ok = mbar_wait(&full[s], (i / stages) & 1);
+    ok = mbar_wait(&full[s], (i / stages) & 1);
     float c[VEC], sn[VEC];
 #pragma unroll
     for (int j = 0; j < VEC; j += 4) {
@@ -321,20 +322,17 @@ __global__ void __launch_bounds__(kBulkThreads) rope_axes_bulk_kernel(const __gr
     }
     if (i + 1 < count && (i + 1) % kBulkChunk != 0) form(i + 1);
     fence_proxy_async_smem();  // the rotated rows before the bulk stores that read them
-    __syncthreads();
+    ok = __syncthreads_and(ok);
+    if (!ok) break;
     if (tid == 0) {
       const int64_t tok = token(i);
       const uint32_t src = smem_u32(stage);
-      if (ok) {
-        if (q_bytes) bulk_store(reinterpret_cast<T *>(p.q_out) + tok * p.qo_sn, src, q_bytes);
-        if (p.k_out != nullptr) bulk_store(reinterpret_cast<T *>(p.k_out) + tok * p.ko_sn, src + q_bytes, k_bytes);
-        T *krow = sh_row[i % kBulkChunk];
-        if (krow != nullptr) {
-          bulk_store(krow, src + q_bytes, k_bytes);
-          bulk_store(krow + (size_t)p.page_size * p.hkv * p.dim, src + q_bytes + k_bytes, v_bytes);
-        }
-      } else {
-        report_error(p.err, PIEKV_ERR_WAIT_TIMEOUT, KID_ROPE_AXES, blockIdx.x, i);
+      if (q_bytes) bulk_store(reinterpret_cast<T *>(p.q_out) + tok * p.qo_sn, src, q_bytes);
+      if (p.k_out != nullptr) bulk_store(reinterpret_cast<T *>(p.k_out) + tok * p.ko_sn, src + q_bytes, k_bytes);
+      T *krow = sh_row[i % kBulkChunk];
+      if (krow != nullptr) {
+        bulk_store(krow, src + q_bytes, k_bytes);
+        bulk_store(krow + (size_t)p.page_size * p.hkv * p.dim, src + q_bytes + k_bytes, v_bytes);
       }
       asm volatile("cp.async.bulk.commit_group;" ::: "memory");
       // the stage of the token before is free once its stores have read it
@@ -344,7 +342,14 @@ __global__ void __launch_bounds__(kBulkThreads) rope_axes_bulk_kernel(const __gr
       }
     }
   }
-  if (tid == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // shared memory outlives the copies
+  if (tid == 0) {  // shared memory outlives the copies
+    if (!ok) {
+      report_error(p.err, PIEKV_ERR_WAIT_TIMEOUT, KID_ROPE_AXES, blockIdx.x, i);
+      // loaded so far: up to token i + stages - 2, at the start stages - 1
+      for (int x = i; x < count && x <= max(i - 1, 0) + stages - 1; ++x) mbar_wait(&full[x % stages], (x / stages) & 1, 200000000ull);
+    }
+    asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+  }
 }
 
 template <typename T>
