@@ -1,14 +1,17 @@
-"""Build libpiekv.so (sm_100a) in-tree with nvcc.
+"""Build libpiekv.so (sm_100a) in-tree with nvcc, and _calls.so with the host compiler.
 
-`python pie_b200/build.py` compiles every translation unit under pie_b200/csrc into
+`python pie_b200/build.py` compiles every CUDA translation unit under pie_b200/csrc into
 pie_b200/libpiekv.so.  nvcc cross-compiles without a GPU.  Objects are cached under
-pie_b200/csrc/build/ and rebuilt when a source or header is newer.
+pie_b200/csrc/build/ and rebuilt when a source or header is newer.  csrc/calls.cpp, the native way from Python to the
+short calls of that library, becomes the extension module pie_b200/_calls.so against the installed torch's headers.
 """
 from __future__ import annotations
 
+import importlib.util
 import os
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -16,6 +19,7 @@ PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 OBJ = CSRC / "build"
 LIB = PKG / "libpiekv.so"
+CALLS = PKG / "_calls.so"
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -47,6 +51,16 @@ def _stale(target: Path, deps: list[Path]) -> bool:
     return any(d.stat().st_mtime > t for d in deps)
 
 
+def _calls_command() -> list[str]:
+    torch = Path(importlib.util.find_spec("torch").submodule_search_locations[0])
+    cuda = Path(os.environ.get("CUDA_HOME", "/usr/local/cuda"))
+    return [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+            "-D_GLIBCXX_USE_CXX11_ABI=1", "-I", str(PKG.parent / "include"), "-I", sysconfig.get_paths()["include"],
+            *(x for d in (torch / "include", torch / "include/torch/csrc/api/include", cuda / "include") for x in ("-isystem", str(d))),
+            str(CSRC / "calls.cpp"), "-o", str(CALLS), "-L", str(torch / "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu",
+            "-ltorch_python"]
+
+
 def build(verbose: bool = False, force: bool = False, ptxas_info: bool = False) -> Path:
     OBJ.mkdir(parents=True, exist_ok=True)
     nvcc = _nvcc()
@@ -67,12 +81,13 @@ def build(verbose: bool = False, force: bool = False, ptxas_info: bool = False) 
             print(" ".join(cmd), flush=True)
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
-            raise RuntimeError(f"nvcc failed: {' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
+            raise RuntimeError(f"compiler failed: {' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
         if (verbose or ptxas_info) and (r.stderr.strip() or r.stdout.strip()):
             print(r.stdout + r.stderr, flush=True)
 
-    with ThreadPoolExecutor(max_workers=min(8, max(1, len(jobs)))) as ex:
-        list(ex.map(run, jobs))
+    calls = [_calls_command()] if force or _stale(CALLS, [CSRC / "calls.cpp"] + hdrs) else []
+    with ThreadPoolExecutor(max_workers=min(8, max(1, len(jobs) + len(calls)))) as ex:
+        list(ex.map(run, calls + jobs))
     if jobs or force or _stale(LIB, objs):
         run([nvcc, "-shared", "-o", str(LIB), *map(str, objs), "-gencode", "arch=compute_100a,code=sm_100a",
              "-cudart", "static"])

@@ -27,8 +27,11 @@ from typing import Optional, Sequence, Tuple
 
 import torch
 
-from . import _lib
+from . import _calls, _lib
 from ._lib import RopeParams, check, lib
+
+_calls.bind(*(C.cast(f, C.c_void_p).value
+              for f in (lib.piekv_rope_axes, lib.piekv_shared_prefix_run, lib.piekv_decode_run_opt)))
 
 __all__ = [
     "BatchPrefillWithPagedKVCacheWrapper",
@@ -474,7 +477,10 @@ class AxisRopeConfig(RopeConfig):
 
     def __setattr__(self, name, value) -> None:
         self.__dict__["_table"] = None  # laid out again at the next use
-        object.__setattr__(self, name, value)
+        object.__setattr__(self, name, tuple(value) if isinstance(value, list) else value)
+
+    def __getstate__(self):
+        return {**self.__dict__, "_table": None}  # a copy lays out its own
 
     def to_c(self, head_dim: int) -> RopeParams:
         raise ValueError("an AxisRopeConfig is taken by rope_axes_append_paged_kv_cache and apply_rope_axes_inplace only")
@@ -525,6 +531,7 @@ def _err_ptr(index: int) -> int:
     ptr = _ERR_PTRS.get(index)
     if ptr is None:
         ptr = _ERR_PTRS[index] = _err_word(torch.device("cuda", index)).data_ptr()
+        _calls.set_error_word(index, ptr)
     return ptr
 
 
@@ -613,6 +620,11 @@ def rope_axes_append_paged_kv_cache(q: Optional[torch.Tensor], k: torch.Tensor, 
     with another q_out, q are read only).  `positions` are the tokens' slots in their contexts, as in
     append_paged_kv_cache; a token whose request, slot or page does not exist is skipped and reported
     (`device_error`), its q is still rotated."""
+    if rope.__class__ is AxisRopeConfig and rope.__dict__["_table"] is not None and rope.mode != "table":
+        done = _calls.rope_axes_append(C.addressof(rope.__dict__["_table"]), q, k, v, pos_ids, batch_indices, positions,
+                                       paged_kv_cache, kv_indices, kv_indptr, q_out)
+        if done is not False:
+            return done
     if q is not None and q_out is None:
         q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
     _rope_axes(q, k, v, pos_ids, rope, q_out, None, "rope_axes_append_paged_kv_cache",
@@ -784,6 +796,12 @@ class BatchDecodeWithPagedKVCacheWrapper:
                                  pl["hkv"], pl["d"], pl["page_size"]),
                                 (self.workspace_buffer.data_ptr(), self.workspace_buffer.numel(),
                                  _err_ptr(indptr.get_device())), indptr.get_device())
+            a = _lib.SharedPrefixArgs(kv_indptr=indptr.data_ptr(), kv_indices=indices.data_ptr(),
+                                      kv_last_page_len=last_page_len.data_ptr(), batch=batch, num_qo_heads=pl["hq"],
+                                      num_kv_heads=pl["hkv"], head_dim=pl["d"], page_size=pl["page_size"],
+                                      sm_scale=pl["sm_scale"], workspace=self.workspace_buffer.data_ptr(),
+                                      workspace_bytes=self.workspace_buffer.numel(), err=_err_ptr(indptr.get_device()))
+            pl["native"] = _calls.decode_plan(indptr.get_device(), a, pl["first_options"])
 
     def run(self, q: torch.Tensor, paged_kv_cache: torch.Tensor, out: Optional[torch.Tensor] = None,
             return_lse: bool = False, sinks: Optional[torch.Tensor] = None, sm_scale: Optional[float] = None):
@@ -826,6 +844,10 @@ class BatchDecodeWithPagedKVCacheWrapper:
     def _run_first_tokens(self, q, paged_kv_cache, out, return_lse, sinks, sm_scale):
         """run() of a plan with a window and first tokens: the same checks, what the plan fixes prepared once."""
         pl = self._plan
+        if sinks is None and sm_scale is None and not return_lse:
+            done = _calls.decode_run(pl["native"], q, paged_kv_cache, out)
+            if done is not False:
+                return done
         head, tail, device = pl["first_call"]
         if not isinstance(q, torch.Tensor):
             _require_cuda(q, "q")
@@ -1047,7 +1069,8 @@ class BatchSharedPrefixDecodeWrapper:
         self._plan = dict(shape=torch.Size((batch, int(num_qo_heads), int(head_dim))), dtype=q_data_type, device=dev,
                           index=indptr.get_device(),
                           cache=(int(page_size), int(num_kv_heads), int(head_dim)), sm_scale=a.sm_scale,
-                          keep=(indptr, indices, last_page_len, group_indptr))
+                          keep=(indptr, indices, last_page_len, group_indptr),
+                          native=_calls.decode_plan(indptr.get_device(), a, None))
         self.replan()
 
     def replan(self) -> None:
@@ -1062,6 +1085,10 @@ class BatchSharedPrefixDecodeWrapper:
         if self._plan is None:
             raise RuntimeError("Must call plan() before run()")
         pl = self._plan
+        if sinks is None and sm_scale is None and not return_lse:
+            done = _calls.decode_run(pl["native"], q, paged_kv_cache, out)
+            if done is not False:
+                return done
         device = pl["index"]
         if not isinstance(q, torch.Tensor):
             _require_cuda(q, "q")
