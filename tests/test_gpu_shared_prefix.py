@@ -226,6 +226,33 @@ def test_scales_that_are_not_positive(scale):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("hq, hkv", [(32, 8), (8, 1), (6, 2), (5, 1), (16, 1), (4, 4), (14, 2), (3, 1)])
+def test_few_rows_behind_long_prefixes(dtype, hq, hkv):
+    """Groups whose rows fill a quarter of a tile or less, and one more than that; prefixes that end inside a quarter."""
+    full = 32 // (hq // hkv)
+    b = Batch([(32, [3, 40]), (33, [1] * full), (130, [5, 0, 70]), (67, [2] * (full + 1)), (300, [1, 2, 3, 4]), (40, [9])],
+              hq, hkv, dtype=dtype, seed=hq)
+    got = _run(b)
+    assert ops.device_error("cuda") is None
+    b.check(got)
+    again = _run(b)
+    assert torch.equal(got[0], again[0]) and torch.equal(got[1], again[1])
+
+
+@pytest.mark.gpu
+def test_nan_behind_few_rows_comes_out():
+    b = Batch([(80, [5, 20, 3]), (64, [1, 9])], 8, 2)
+    for page, part in ((int(b.lists[0][37]), 0), (int(b.lists[0][70]), 1)):
+        pool = b.pool.clone()
+        pool[page, part, 3, 1, 11] = float("nan")
+        w = b.plan(ops.BatchSharedPrefixDecodeWrapper(_workspace()))
+        got = w.run(b.q.cuda(), pool.cuda()).cpu().float()
+        bad = torch.isnan(got)
+        assert bool(bad[:3, 4:, 11].all()) and not bool(bad[3:].any()) and not bool(bad[:3, :4].any())
+
+
+@pytest.mark.gpu
 def test_large_scores_and_peaked_rows():
     """Scores in the hundreds: the join of prefix and suffix must not overflow, whichever part holds the maximum."""
     b = Batch([(40, [20, 50, 0])], 8, 2, seed=8)
