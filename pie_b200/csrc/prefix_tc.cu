@@ -57,7 +57,7 @@ constexpr int kPxVWarp = kMmaWarp + 1, kPxSchedWarp = kMmaWarp + 2;
 constexpr int kPxSlots = 4;                         // items the scheduler may describe ahead of the slowest reader
 constexpr int kPxReaders = kSoftmaxWarps + 1 + 3;   // softmax warps, MMA thread, K, V and query-row cursors
 static_assert(kTileTokens == kBN, "plan and kernel cut the work alike");
-static_assert(sizeof(Segment) == 32 && sizeof(Item) == 16, "read as vectors");
+static_assert(sizeof(Item) == 32, "read as two vectors");
 
 // An item as the scheduler publishes it.
 struct Work {
@@ -87,11 +87,18 @@ __global__ void __launch_bounds__(kPxThreads, 1)
 
   // The kernel behind this one reads its own pages first and waits for these results only then.
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  // The first item is the CTA's own: it is loaded together with the header (there is room for more items than CTAs).
+  const int4 *first = reinterpret_cast<const int4 *>(p.items + blockIdx.x);
+  int4 it0 = make_int4(0, 0, 0, 0), it1 = it0;
+  if (warp == kPxSchedWarp) {
+    it0 = __ldg(first);
+    it1 = __ldg(first + 1);
+  }
   const int ctas = __ldg(p.header);
   if ((int)blockIdx.x >= ctas) return;
 
-  const int warp = threadIdx.x >> 5;
-  const int lane = threadIdx.x & 31;
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const uint32_t q_smem = base;
   const uint32_t k_smem0 = base + 2 * kTileBytes;
@@ -166,31 +173,32 @@ __global__ void __launch_bounds__(kPxThreads, 1)
           if (n > 0) {
             if (lane == 0) idx = ctas + atomicAdd(p.header + 4, 1);
             idx = __shfl_sync(0xffffffffu, idx, 0);
+            if (idx < items) {
+              it0 = __ldg(reinterpret_cast<const int4 *>(p.items + idx));
+              it1 = __ldg(reinterpret_cast<const int4 *>(p.items + idx) + 1);
+            }
           }
           Work w{};
-          if (idx < items) {
-            const int4 it = __ldg(reinterpret_cast<const int4 *>(p.items + idx));  // segment, t0, t1, piece
-            const int4 sa = __ldg(reinterpret_cast<const int4 *>(p.segments + it.x));
-            const int2 sb = __ldg(reinterpret_cast<const int2 *>(p.segments + it.x) + 2);  // (request, list, pages, head), rows
+          if (idx < items) {  // it0 = request, list, pages, kv head; it1 = rows, t0, t1, piece
             w.valid = 1;
-            w.list = sa.y;
-            w.pages = sa.z;
-            w.kv_head = sa.w;
-            w.pair = sb.x > p.problem;
-            w.request[0] = w.request[1] = sa.x;
-            w.rows[0] = w.rows[1] = min(sb.x, p.problem);
-            w.t0[0] = w.t0[1] = it.y;
-            w.n[0] = w.n[1] = it.z - it.y;
-            w.split[0] = w.split[1] = it.w;
+            w.list = it0.y;
+            w.pages = it0.z;
+            w.kv_head = it0.w;
+            w.pair = it1.x > p.problem;
+            w.request[0] = w.request[1] = it0.x;
+            w.rows[0] = w.rows[1] = min(it1.x, p.problem);
+            w.t0[0] = w.t0[1] = it1.y;
+            w.n[0] = w.n[1] = it1.z - it1.y;
+            w.split[0] = w.split[1] = it1.w;
             if (w.pair) {
               w.request[1] += p.problem / p.group;
-              w.rows[1] = min(sb.x - p.problem, p.problem);
+              w.rows[1] = min(it1.x - p.problem, p.problem);
             } else if (p.max_splits >= 2) {
-              w.n[0] = (it.z - it.y + 1) / 2;
+              w.n[0] = (it1.z - it1.y + 1) / 2;
               w.n[1] -= w.n[0];
               w.t0[1] += w.n[0];
-              w.split[0] = 2 * it.w;
-              w.split[1] = 2 * it.w + 1;
+              w.split[0] = 2 * it1.w;
+              w.split[1] = 2 * it1.w + 1;
             } else {
               w.n[1] = w.rows[1] = 0;
             }

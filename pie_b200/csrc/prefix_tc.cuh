@@ -9,7 +9,6 @@ struct PrefixTcParams {
   int64_t q_sn, q_sh;
   const int32_t *kv_indices;
   int *header;  // the plan's
-  const sprefix::Segment *segments;
   const sprefix::Item *items;
   float *part_o;    // [split][batch][Hq][128], unnormalised
   float2 *part_ml;  // [split][batch][Hq]: reference maximum (log2 units), sum

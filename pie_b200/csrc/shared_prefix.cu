@@ -208,15 +208,14 @@ __global__ void __launch_bounds__(1024) sp_plan_kernel(const int32_t *__restrict
       if (lane == 0) report_error(err, PIEKV_ERR_PAGE_CAPACITY, KID_SHARED_PREFIX, g, pieces);
       pieces = 0;
     }
-    for (int i = lane; i < n; i += 32) {
-      const int block = i / hkv;
-      v.segments[gr.segment + i] = Segment{gr.first + block * block_members, kv_indptr[gr.first], gr.pages, i % hkv,
-                                           (gr.members - block * block_members) * heads_per_kv, pieces, {0, 0}};
-    }
-    for (int i = lane; i < n * pieces; i += 32) {
-      const int piece = i / n;
-      v.items[at + i] = Item{gr.segment + i % n, (int)((long long)tiles * piece / pieces),
-                             (int)((long long)tiles * (piece + 1) / pieces), piece};
+    const int list = kv_indptr[gr.first];
+    for (int i = lane; i < max(n, n * pieces); i += 32) {
+      const int piece = i / n, segment = i % n, block = segment / hkv;
+      const int request = gr.first + block * block_members, rows = (gr.members - block * block_members) * heads_per_kv;
+      if (piece == 0) v.segments[gr.segment + segment] = Segment{rows, pieces};
+      if (piece < pieces)
+        v.items[at + i] = Item{request, list, gr.pages, segment % hkv, rows, (int)((long long)tiles * piece / pieces),
+                               (int)((long long)tiles * (piece + 1) / pieces), piece};
     }
   }
   __syncthreads();
@@ -333,7 +332,6 @@ extern "C" int piekv_shared_prefix_run(const piekv_shared_prefix_args *args, voi
   px.q_sh = a.q_sh;
   px.kv_indices = a.kv_indices;
   px.header = v.header;
-  px.segments = v.segments;
   px.items = v.items;
   px.part_ml = reinterpret_cast<float2 *>(ws);
   px.part_o = reinterpret_cast<float *>(ws + prefix_ml_bytes(a.batch, a.hq, args->max_splits));

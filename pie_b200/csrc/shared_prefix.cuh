@@ -20,13 +20,14 @@ struct Group {
 
 // A prefix against a block of rows of one kv head, cut into `pieces` items.
 struct Segment {
-  int request, list, pages;  // first request of the block, the group's page list's first entry, pages
-  int kv_head, rows;         // rows from `request` on (at most two problems' worth are this segment's)
+  int rows;  // from the block's first request to the group's end (at most two problems' worth are this segment's)
   int pieces;
-  int pad[2];
 };
+// One piece of a segment, with what the segment says about it: a CTA starts on its first item after one load.
 struct Item {
-  int segment, t0, t1, piece;  // tiles [t0, t1)
+  int request, list, pages;  // first request of the block, the group's page list's first entry, pages
+  int kv_head, rows;
+  int t0, t1, piece;  // tiles [t0, t1)
 };
 
 struct PlanView {
