@@ -148,6 +148,7 @@ __global__ void __launch_bounds__(Shape<HB>::kThreads, Shape<HB>::kCtasPerSm)
   uint8_t *stage0_ptr = smem_raw + (stage0 - smem_u32(smem_raw));
 
   if (tid == 0) {
+    tma_prefetch_map(&tmap);
     for (int s = 0; s < kStages; ++s) {
       mbar_init(&full_bar[s], 1);
       mbar_init(&empty_bar[s], HB);

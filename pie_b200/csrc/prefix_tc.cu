@@ -96,6 +96,10 @@ __global__ void __launch_bounds__(kPxThreads, 1)
     it0 = __ldg(first);
     it1 = __ldg(first + 1);
   }
+  if (threadIdx.x == 0) {
+    tma_prefetch_map(&tmap_q);
+    tma_prefetch_map(&tmap_kv);
+  }
   const int ctas = __ldg(p.header);
   if ((int)blockIdx.x >= ctas) return;
 

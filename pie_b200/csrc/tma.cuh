@@ -41,6 +41,10 @@ __device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap *tma
       "l"(reinterpret_cast<uint64_t>(tmap)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4), "r"(smem_u32(bar))
       : "memory");
 }
+// The descriptor on its way before the first copy asks for it.
+__device__ __forceinline__ void tma_prefetch_map(const CUtensorMap *tm) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(tm)) : "memory");
+}
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *tmap, int c0, int c1, int c2, int c3,
                                             uint64_t *bar) {
   asm volatile(
