@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import importlib.util
 import os
+import shutil
 import subprocess
 import sys
 import sysconfig
@@ -54,7 +55,8 @@ def _stale(target: Path, deps: list[Path]) -> bool:
 def _calls_command() -> list[str]:
     torch = Path(importlib.util.find_spec("torch").submodule_search_locations[0])
     cuda = Path(os.environ.get("CUDA_HOME", "/usr/local/cuda"))
-    return [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+    # the system's g++: exceptions of torch's libraries pass through, so there must be one C++ runtime
+    return [shutil.which("g++") or os.environ.get("CXX", "c++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
             "-D_GLIBCXX_USE_CXX11_ABI=1", "-I", str(PKG.parent / "include"), "-I", sysconfig.get_paths()["include"],
             *(x for d in (torch / "include", torch / "include/torch/csrc/api/include", cuda / "include") for x in ("-isystem", str(d))),
             str(CSRC / "calls.cpp"), "-o", str(CALLS), "-L", str(torch / "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu",

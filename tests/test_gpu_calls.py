@@ -115,6 +115,19 @@ def test_append_refuses_the_same_either_way():
     assert same.shape == (n, 8, 128)
 
 
+@pytest.mark.gpu
+def test_an_output_that_does_not_fit_raises_the_allocators_error():
+    sc = make_scenario(8, 2, 128, torch.bfloat16, [(20, 3), (4, 2)])
+    rope = _axes()
+    _append(sc, rope)
+    wide = torch.zeros((1, 1, 128), dtype=torch.bfloat16, device="cuda").expand(5, 1 << 29, 128)  # 687 GB of output
+    for config in (rope, _axes()):
+        with pytest.raises(torch.OutOfMemoryError):
+            _append(sc, config, q=wide)
+    again, _ = _append(sc, rope)
+    assert again.shape == (5, 8, 128) and ops.device_error("cuda") is None
+
+
 def _decode_wrapper(sc, kind):
     m = sc.meta
     ws = torch.empty(64 << 20, dtype=torch.uint8, device="cuda")
