@@ -5,7 +5,8 @@
 // launches, or returns False without side effects when any of them does not hold: the Python function then goes on with
 // its own checks, which say what is wrong, and with the rare forms that are not taken here.  Nothing is kept from
 // call to call but what a plan holds.  Host time of a call, checks in Python and here: multi-axis append 13.7 and 6.8 us,
-// decode with first tokens 10.4 and 5.0, shared-prefix decode 11.2 and 7.4 (two launches, two tensor maps).
+// decode with first tokens 10.4 and 5.0, prefill with first tokens 11.9 and 8.2, shared-prefix decode 11.2 and 7.4 (two
+// launches, two tensor maps).
 #include <Python.h>
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAFunctions.h>
@@ -25,6 +26,7 @@ constexpr int kDevices = 64;
 decltype(&piekv_rope_axes) rope_axes_fn = nullptr;
 decltype(&piekv_shared_prefix_run) shared_prefix_fn = nullptr;
 decltype(&piekv_decode_run_opt) decode_fn = nullptr;
+decltype(&piekv_prefill_run_opt) prefill_fn = nullptr;
 int32_t *error_words[kDevices] = {nullptr};
 
 // A plain tensor on CUDA device `device` (-1: any), or nullptr.
@@ -70,13 +72,14 @@ PyObject *set_error_word(PyObject *, PyObject *args) {
   Py_RETURN_NONE;
 }
 
-// bind(rope_axes, shared_prefix_run, decode_run_opt): addresses of the library's functions
+// bind(rope_axes, shared_prefix_run, decode_run_opt, prefill_run_opt): addresses of the library's functions
 PyObject *bind(PyObject *, PyObject *args) {
-  unsigned long long a, b, c;
-  if (!PyArg_ParseTuple(args, "KKK", &a, &b, &c)) return nullptr;
+  unsigned long long a, b, c, d;
+  if (!PyArg_ParseTuple(args, "KKKK", &a, &b, &c, &d)) return nullptr;
   rope_axes_fn = reinterpret_cast<decltype(rope_axes_fn)>(a);
   shared_prefix_fn = reinterpret_cast<decltype(shared_prefix_fn)>(b);
   decode_fn = reinterpret_cast<decltype(decode_fn)>(c);
+  prefill_fn = reinterpret_cast<decltype(prefill_fn)>(d);
   Py_RETURN_NONE;
 }
 
@@ -157,30 +160,35 @@ PyObject *rope_axes_append(PyObject *, PyObject *const *o, Py_ssize_t count) {
 }
 
 // What a plan fixes about its runs.
-struct DecodePlan {
+struct Plan {
   int device;
-  bool prefix;                // `args`, or the call with a window and first tokens
+  bool prefix;  // a shared-prefix run; otherwise a call with a window and first tokens, `options`
   piekv_shared_prefix_args args;
   piekv_attn_options options;
+  const int32_t *qo_indptr;  // of a prefill call
+  int causal;
 };
-const char *const kPlanName = "pie_b200.decode_plan";
-void free_plan(PyObject *capsule) { delete static_cast<DecodePlan *>(PyCapsule_GetPointer(capsule, kPlanName)); }
+const char *const kPlanName = "pie_b200.plan";
+void free_plan(PyObject *capsule) { delete static_cast<Plan *>(PyCapsule_GetPointer(capsule, kPlanName)); }
 
-// decode_plan(device, piekv_shared_prefix_args as bytes, piekv_attn_options as bytes | None): with options the plan of
-// a decode call with a window and first tokens (which uses the tables, sizes, workspace, err and sm_scale of the struct)
-PyObject *decode_plan(PyObject *, PyObject *args) {
-  int device;
+// plan(device, piekv_shared_prefix_args as bytes, piekv_attn_options as bytes | None, qo_indptr address, causal): with
+// options the plan of a call with a window and first tokens, which uses the tables, sizes, workspace, err and sm_scale of the struct
+PyObject *make_plan(PyObject *, PyObject *args) {
+  int device, causal = 0;
+  unsigned long long qo_indptr = 0;
   Py_buffer a, opt;
   std::memset(&opt, 0, sizeof(opt));
-  if (!PyArg_ParseTuple(args, "iy*z*", &device, &a, &opt)) return nullptr;
+  if (!PyArg_ParseTuple(args, "iy*z*|Ki", &device, &a, &opt, &qo_indptr, &causal)) return nullptr;
   PyObject *capsule = nullptr;
   if (a.len != (Py_ssize_t)sizeof(piekv_shared_prefix_args) || (opt.buf != nullptr && opt.len != (Py_ssize_t)sizeof(piekv_attn_options))) {
-    PyErr_SetString(PyExc_ValueError, "decode_plan: struct sizes differ from the library's");
-  } else if (DecodePlan *plan = new (std::nothrow) DecodePlan()) {
+    PyErr_SetString(PyExc_ValueError, "plan: struct sizes differ from the library's");
+  } else if (Plan *plan = new (std::nothrow) Plan()) {
     plan->device = device;
     plan->prefix = opt.buf == nullptr;
     std::memcpy(&plan->args, a.buf, sizeof(plan->args));
     if (opt.buf != nullptr) std::memcpy(&plan->options, opt.buf, sizeof(plan->options));
+    plan->qo_indptr = reinterpret_cast<const int32_t *>(qo_indptr);
+    plan->causal = causal;
     capsule = PyCapsule_New(plan, kPlanName, free_plan);
     if (capsule == nullptr) delete plan;
   } else {
@@ -191,6 +199,33 @@ PyObject *decode_plan(PyObject *, PyObject *args) {
   return capsule;
 }
 
+// What the runs of a plan ask of q, pool and out; `rows` is q's first size.  False: declined.
+bool fill(const Plan &plan, int64_t rows, PyObject *q_object, PyObject *pool_object, PyObject *given, piekv_shared_prefix_args &a,
+          at::Tensor &out) {
+  const at::Tensor *q = tensor_on(q_object, plan.device), *pool = tensor_on(pool_object, plan.device);
+  if (q == nullptr || !is_rows(*q) || !is_pool(pool) || !is_current(plan.device)) return false;
+  a = plan.args;
+  const int dtype = dtype_code(*q);
+  if (dtype < 0 || dtype_code(*pool) != dtype || (plan.prefix && dtype != a.dtype)) return false;
+  if (q->size(0) != rows || q->size(1) != a.num_qo_heads || q->size(2) != a.head_dim) return false;
+  if (pool->size(2) != a.page_size || pool->size(3) != a.num_kv_heads || pool->size(4) != a.head_dim) return false;
+  out = output_like(*q, given);
+  if (!out.defined()) return false;
+  a.dtype = dtype;
+  a.q = q->data_ptr();
+  a.q_stride_n = q->stride(0);
+  a.q_stride_h = q->stride(1);
+  a.pool = pool->data_ptr();
+  a.num_pages = (int32_t)pool->size(0);
+  a.out = out.data_ptr();
+  return true;
+}
+PyObject *result(const at::Tensor &out, PyObject *given) {
+  if (given == Py_None) return THPVariable_Wrap(out);
+  Py_INCREF(given);
+  return given;
+}
+
 // decode_run(plan, q, pool, out | None)
 PyObject *decode_run(PyObject *, PyObject *const *o, Py_ssize_t count) {
   HANDLE_TH_ERRORS
@@ -198,38 +233,49 @@ PyObject *decode_run(PyObject *, PyObject *const *o, Py_ssize_t count) {
     PyErr_SetString(PyExc_TypeError, "decode_run takes 4 arguments");
     return nullptr;
   }
-  const auto *plan = static_cast<const DecodePlan *>(PyCapsule_GetPointer(o[0], kPlanName));
+  const auto *plan = static_cast<const Plan *>(PyCapsule_GetPointer(o[0], kPlanName));
   if (plan == nullptr) return nullptr;
-  const at::Tensor *q = tensor_on(o[1], plan->device), *pool = tensor_on(o[2], plan->device);
-  if (q == nullptr || !is_rows(*q) || !is_pool(pool) || !is_current(plan->device)) return declined();
-  piekv_shared_prefix_args a = plan->args;
-  const int dtype = dtype_code(*q);
-  if (dtype < 0 || dtype_code(*pool) != dtype || (plan->prefix && dtype != a.dtype)) return declined();
-  if (q->size(0) != a.batch || q->size(1) != a.num_qo_heads || q->size(2) != a.head_dim) return declined();
-  if (pool->size(2) != a.page_size || pool->size(3) != a.num_kv_heads || pool->size(4) != a.head_dim) return declined();
-  at::Tensor out = output_like(*q, o[3]);
-  if (!out.defined()) return declined();
-  a.q = q->data_ptr();
-  a.q_stride_n = q->stride(0);
-  a.q_stride_h = q->stride(1);
-  a.pool = pool->data_ptr();
-  a.num_pages = (int32_t)pool->size(0);
-  a.out = out.data_ptr();
+  piekv_shared_prefix_args a;
+  at::Tensor out;
+  if (!fill(*plan, plan->args.batch, o[1], o[2], o[3], a, out)) return declined();
   void *stream = stream_of(plan->device);
   int status;
   Py_BEGIN_ALLOW_THREADS;
   status = plan->prefix
                ? shared_prefix_fn(&a, stream)
                : decode_fn(a.q, a.q_stride_n, a.q_stride_h, a.pool, a.out, nullptr, a.kv_indptr, a.kv_indices, a.kv_last_page_len, a.batch,
-                           a.num_qo_heads, a.num_kv_heads, a.head_dim, a.page_size, a.num_pages, dtype, a.sm_scale, a.workspace,
+                           a.num_qo_heads, a.num_kv_heads, a.head_dim, a.page_size, a.num_pages, a.dtype, a.sm_scale, a.workspace,
                            a.workspace_bytes, a.err, stream, &plan->options);
   Py_END_ALLOW_THREADS;
   if (status != 0) return declined();
-  if (o[3] != Py_None) {
-    Py_INCREF(o[3]);
-    return o[3];
+  return result(out, o[3]);
+  END_HANDLE_TH_ERRORS
+}
+
+// prefill_run(plan, (query tokens, pages) that the device's work list was built for, q, pool, out | None)
+PyObject *prefill_run(PyObject *, PyObject *const *o, Py_ssize_t count) {
+  HANDLE_TH_ERRORS
+  if (count != 5) {
+    PyErr_SetString(PyExc_TypeError, "prefill_run takes 5 arguments");
+    return nullptr;
   }
-  return THPVariable_Wrap(out);
+  const auto *plan = static_cast<const Plan *>(PyCapsule_GetPointer(o[0], kPlanName));
+  if (plan == nullptr) return nullptr;
+  long long rows, pages;
+  if (!PyTuple_Check(o[1])) return declined();  // not built yet
+  if (!PyArg_ParseTuple(o[1], "LL", &rows, &pages)) return nullptr;
+  piekv_shared_prefix_args a;
+  at::Tensor out;
+  if (plan->qo_indptr == nullptr || !fits(rows) || !fill(*plan, rows, o[2], o[3], o[4], a, out) || a.num_pages != pages) return declined();
+  void *stream = stream_of(plan->device);
+  int status;
+  Py_BEGIN_ALLOW_THREADS;
+  status = prefill_fn(a.q, a.q_stride_n, a.q_stride_h, a.pool, a.out, nullptr, plan->qo_indptr, a.kv_indptr, a.kv_indices,
+                      a.kv_last_page_len, nullptr, 0, plan->causal, 1, a.batch, (int32_t)rows, a.num_qo_heads, a.num_kv_heads, a.head_dim,
+                      a.page_size, a.num_pages, a.dtype, a.sm_scale, a.workspace, a.workspace_bytes, a.err, stream, &plan->options);
+  Py_END_ALLOW_THREADS;
+  if (status != 0) return declined();
+  return result(out, o[4]);
   END_HANDLE_TH_ERRORS
 }
 
@@ -237,7 +283,8 @@ PyMethodDef methods[] = {
     {"bind", bind, METH_VARARGS, nullptr},
     {"set_error_word", set_error_word, METH_VARARGS, nullptr},
     {"rope_axes_append", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(rope_axes_append)), METH_FASTCALL, nullptr},
-    {"decode_plan", decode_plan, METH_VARARGS, nullptr},
+    {"plan", make_plan, METH_VARARGS, nullptr},
+    {"prefill_run", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(prefill_run)), METH_FASTCALL, nullptr},
     {"decode_run", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(decode_run)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

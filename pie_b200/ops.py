@@ -31,7 +31,7 @@ from . import _calls, _lib
 from ._lib import RopeParams, check, lib
 
 _calls.bind(*(C.cast(f, C.c_void_p).value
-              for f in (lib.piekv_rope_axes, lib.piekv_shared_prefix_run, lib.piekv_decode_run_opt)))
+              for f in (lib.piekv_rope_axes, lib.piekv_shared_prefix_run, lib.piekv_decode_run_opt, lib.piekv_prefill_run_opt)))
 
 __all__ = [
     "BatchPrefillWithPagedKVCacheWrapper",
@@ -801,7 +801,7 @@ class BatchDecodeWithPagedKVCacheWrapper:
                                       num_kv_heads=pl["hkv"], head_dim=pl["d"], page_size=pl["page_size"],
                                       sm_scale=pl["sm_scale"], workspace=self.workspace_buffer.data_ptr(),
                                       workspace_bytes=self.workspace_buffer.numel(), err=_err_ptr(indptr.get_device()))
-            pl["native"] = _calls.decode_plan(indptr.get_device(), a, pl["first_options"])
+            pl["native"] = _calls.plan(indptr.get_device(), a, pl["first_options"])
 
     def run(self, q: torch.Tensor, paged_kv_cache: torch.Tensor, out: Optional[torch.Tensor] = None,
             return_lse: bool = False, sinks: Optional[torch.Tensor] = None, sm_scale: Optional[float] = None):
@@ -1070,7 +1070,7 @@ class BatchSharedPrefixDecodeWrapper:
                           index=indptr.get_device(),
                           cache=(int(page_size), int(num_kv_heads), int(head_dim)), sm_scale=a.sm_scale,
                           keep=(indptr, indices, last_page_len, group_indptr),
-                          native=_calls.decode_plan(indptr.get_device(), a, None))
+                          native=_calls.plan(indptr.get_device(), a, None))
         self.replan()
 
     def replan(self) -> None:
@@ -1230,6 +1230,13 @@ class BatchPrefillWithPagedKVCacheWrapper:
                 (int(num_qo_heads), int(num_kv_heads), int(head_dim_qk), int(page_size)),
                 (self.workspace_buffer.data_ptr(), self.workspace_buffer.numel(), _err_ptr(qo_indptr.get_device())),
                 _attn_options(int(window_left), None, int(num_qo_heads), first_tokens))
+            pl = self._plan
+            a = _lib.SharedPrefixArgs(kv_indptr=paged_kv_indptr.data_ptr(), kv_indices=paged_kv_indices.data_ptr(),
+                                      kv_last_page_len=paged_kv_last_page_len.data_ptr(), batch=batch, num_qo_heads=pl["hq"],
+                                      num_kv_heads=pl["hkv"], head_dim=pl["d"], page_size=pl["page_size"],
+                                      sm_scale=pl["sm_scale"], workspace=self.workspace_buffer.data_ptr(),
+                                      workspace_bytes=self.workspace_buffer.numel(), err=_err_ptr(qo_indptr.get_device()))
+            pl["native"] = _calls.plan(qo_indptr.get_device(), a, pl["first_call"][4], qo_indptr.data_ptr(), 1 if causal else 0)
 
     def _device_plan(self, n: int, num_pages: int) -> None:
         """Build the work list (and pack the mask) on the device once per plan(); later run() calls
@@ -1302,6 +1309,10 @@ class BatchPrefillWithPagedKVCacheWrapper:
     def _run_first_tokens(self, q, paged_kv_cache, out, return_lse, sinks, sm_scale):
         """run() of a plan with a window and first tokens: the same checks, what the plan fixes prepared once."""
         pl = self._plan
+        if sinks is None and sm_scale is None and not return_lse:
+            done = _calls.prefill_run(pl["native"], pl["planned_for"], q, paged_kv_cache, out)
+            if done is not False:
+                return done
         device, tables, sizes, tail, options = pl["first_call"]
         if not isinstance(q, torch.Tensor):
             _require_cuda(q, "q")

@@ -19,22 +19,25 @@ def test_what_is_not_a_cuda_tensor_is_declined():
     args = (t, t, t, i.view(1, 2), i, i, torch.zeros(1, 2, 16, 2, 8), i, i, None)
     assert _calls.rope_axes_append(C.addressof(table), *args) is False
     assert _calls.rope_axes_append(C.addressof(table), None, 3, "x", *args[3:]) is False
-    plan = _calls.decode_plan(0, _lib.SharedPrefixArgs(), None)
+    plan = _calls.plan(0, _lib.SharedPrefixArgs(), None)
     assert _calls.decode_run(plan, t, t, None) is False
     assert _calls.decode_run(plan, None, 1, None) is False
+    assert _calls.prefill_run(plan, None, t, t, None) is False and _calls.prefill_run(plan, (2, 1), t, t, None) is False
 
 
 def test_wrong_counts_sizes_and_capsules_raise():
     with pytest.raises(ValueError, match="sizes"):
-        _calls.decode_plan(0, _lib.AttnOptions(), None)
+        _calls.plan(0, _lib.AttnOptions(), None)
     with pytest.raises(ValueError, match="sizes"):
-        _calls.decode_plan(0, _lib.SharedPrefixArgs(), _lib.SharedPrefixArgs())
+        _calls.plan(0, _lib.SharedPrefixArgs(), _lib.SharedPrefixArgs())
     with pytest.raises(TypeError):
         _calls.decode_run(None)
     with pytest.raises(ValueError):
         _calls.decode_run(object(), None, None, None)
     with pytest.raises(TypeError):
         _calls.rope_axes_append(1, 2)
+    with pytest.raises(TypeError):
+        _calls.prefill_run(_calls.plan(0, _lib.SharedPrefixArgs(), _lib.AttnOptions()), (1,), None, None, None)
 
 
 def test_a_copied_config_lays_out_its_own_table():
@@ -187,3 +190,30 @@ def test_decode_refuses_the_same_either_way(kind):
         for lse in (False, True):
             with pytest.raises(ValueError):
                 w.run(q, pool, out=out, return_lse=lse)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("dtype, hq, hkv, d", [(torch.bfloat16, 8, 2, 128), (torch.float16, 6, 2, 128), (torch.float32, 4, 4, 64)])
+def test_prefill_is_the_same_either_way(causal, dtype, hq, hkv, d):
+    sc = make_scenario(hq, hkv, d, dtype, [(3, 5), (200, 70), (0, 130)])
+    m = sc.meta
+    w = ops.BatchPrefillWithPagedKVCacheWrapper(torch.empty(64 << 20, dtype=torch.uint8, device="cuda"))
+    w.plan(dev(m.qo_indptr), dev(m.kv_indptr), dev(m.kv_indices), dev(m.kv_last_page_len), hq, hkv, d, sc.page_size,
+           causal=causal, window_left=60, first_tokens=3, q_data_type=dtype)
+    q, pool = sc.q.cuda(), sc.pool.cuda()
+    slow, _ = w.run(q, pool, return_lse=True)
+    assert torch.equal(w.run(q, pool), slow)
+    out = torch.empty_like(q)
+    assert w.run(q, pool, out=out) is out and torch.equal(out, slow)
+    wide = torch.zeros((q.shape[0], hq, 2, d), dtype=dtype, device="cuda")
+    wide[:, :, 1] = q
+    assert torch.equal(w.run(wide[:, :, 1], pool), slow)
+    bigger = torch.cat([pool, pool[:3]])  # another number of pages: the work list is built again
+    assert torch.equal(w.run(q, bigger), slow) and torch.equal(w.run(q, pool), slow)
+    for args in ((q[:, :2], pool), (sc.q, pool), (q, sc.pool), (q, (pool, pool)), (None, pool), (q.double(), pool),
+                 (q, pool[:, :, :8])):
+        for lse in (False, True):
+            with pytest.raises((ValueError, AttributeError) if args[0] is None else ValueError):
+                w.run(*args, return_lse=lse)
+    assert ops.device_error("cuda") is None
