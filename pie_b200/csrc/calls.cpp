@@ -10,6 +10,7 @@
 #include <Python.h>
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAFunctions.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -209,6 +210,8 @@ bool fill(const Plan &plan, int64_t rows, PyObject *q_object, PyObject *pool_obj
   if (dtype < 0 || dtype_code(*pool) != dtype || (plan.prefix && dtype != a.dtype)) return false;
   if (q->size(0) != rows || q->size(1) != a.num_qo_heads || q->size(2) != a.head_dim) return false;
   if (pool->size(2) != a.page_size || pool->size(3) != a.num_kv_heads || pool->size(4) != a.head_dim) return false;
+  // the wrapper keeps a shared-prefix plan that a captured call points to
+  if (plan.prefix && c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None) return false;
   out = output_like(*q, given);
   if (!out.defined()) return false;
   a.dtype = dtype;

@@ -986,9 +986,10 @@ class BatchSharedPrefixDecodeWrapper:
     full pages the requests of a group share is found on the device by comparing their page lists; nothing is read
     back.  The plan holds until the page table's contents change; `replan()` rebuilds it from the same tensors.  Both
     only launch kernels on the current stream, so plan / replan and any number of run() calls (one per layer) can be
-    captured in a CUDA graph together.  The plan lives in a buffer of its own; the workspace may be shared with other
-    wrappers whose calls are ordered on the same stream (a prefill wrapper keeps its plan in its workspace: plan it again
-    after a call of another wrapper on the same one)."""
+    captured in a CUDA graph together.  The plan lives in a buffer of its own, which later plans use again; what a captured
+    call points to (its plan, page table and grouping) is kept, as it was, while the wrapper lives.  The workspace may be
+    shared with other wrappers whose calls are ordered on the same stream (a prefill wrapper keeps its plan in its
+    workspace: plan it again after a call of another wrapper on the same one)."""
 
     def __init__(self, float_workspace_buffer: torch.Tensor, kv_layout: str = "NHD") -> None:
         if kv_layout != "NHD":
@@ -998,8 +999,7 @@ class BatchSharedPrefixDecodeWrapper:
         self.kv_layout = kv_layout
         float_workspace_buffer[:COUNTER_BYTES].zero_()
         self._plan = None
-        self._args = None
-        self._buffers = []  # plan buffers; earlier ones stay alive, a captured graph may still use them
+        self._captured = []  # plans that captured calls point to
 
     def plan(self, indptr: torch.Tensor, indices: torch.Tensor, last_page_len: torch.Tensor, num_qo_heads: int,
              num_kv_heads: int, head_dim: int, page_size: int, group_indptr: Optional[torch.Tensor] = None,
@@ -1047,15 +1047,18 @@ class BatchSharedPrefixDecodeWrapper:
             raise ValueError(f"workspace_buffer too small: {have} < {base} bytes")
         splits = min(_lib.SHARED_PREFIX_MAX_SPLITS, 1 + (have - base) // each if each > 0 else 1)
         plan_bytes = lib.piekv_shared_prefix_plan_bytes(batch, groups, num_qo_heads, num_kv_heads)
-        if not self._buffers or self._buffers[-1].numel() < plan_bytes or self._buffers[-1].device != dev:
-            self._buffers.append(torch.empty(max(plan_bytes, 4096), dtype=torch.uint8, device=dev))
+        old, buffer = self._plan, None
+        if old is not None and not old["captured"] and old["buffer"].numel() >= plan_bytes and old["device"] == dev:
+            buffer = old["buffer"]
+        if buffer is None:
+            buffer = torch.empty(max(plan_bytes, 4096), dtype=torch.uint8, device=dev)
         a = _lib.SharedPrefixArgs()
         a.kv_indptr = indptr.data_ptr()
         a.kv_indices = indices.data_ptr()
         a.kv_last_page_len = last_page_len.data_ptr()
         a.group_indptr = group_indptr.data_ptr()
-        a.plan = self._buffers[-1].data_ptr()
-        a.plan_bytes = self._buffers[-1].numel()
+        a.plan = buffer.data_ptr()
+        a.plan_bytes = buffer.numel()
         a.workspace = self.workspace_buffer.data_ptr()
         a.workspace_bytes = have
         a.err = _err_word(dev).data_ptr()
@@ -1065,19 +1068,34 @@ class BatchSharedPrefixDecodeWrapper:
         a.dtype = _dtype_code(q_data_type, "plan")
         a.max_splits = splits
         a.sm_scale = float(sm_scale) if sm_scale is not None else 1.0 / math.sqrt(head_dim)
-        self._args = a
-        self._plan = dict(shape=torch.Size((batch, int(num_qo_heads), int(head_dim))), dtype=q_data_type, device=dev,
-                          index=indptr.get_device(),
-                          cache=(int(page_size), int(num_kv_heads), int(head_dim)), sm_scale=a.sm_scale,
-                          keep=(indptr, indices, last_page_len, group_indptr),
-                          native=_calls.plan(indptr.get_device(), a, None))
-        self.replan()
+        pl = dict(shape=torch.Size((batch, int(num_qo_heads), int(head_dim))), dtype=q_data_type, device=dev,
+                  index=indptr.get_device(),
+                  cache=(int(page_size), int(num_kv_heads), int(head_dim)), sm_scale=a.sm_scale,
+                  keep=(indptr, indices, last_page_len, group_indptr), args=a, buffer=buffer,
+                  native=_calls.plan(indptr.get_device(), a, None), captured=False, built=False)
+        self._plan = None  # until this one is built
+        self._build(pl)
+        self._plan = pl
 
     def replan(self) -> None:
         """Rebuild the plan from the tensors of the last plan() call, whose contents may have changed."""
         if self._plan is None:
             raise RuntimeError("Must call plan() before run()")
-        check(lib.piekv_shared_prefix_plan(C.byref(self._args), _stream(self._plan["device"])), "BatchSharedPrefixDecode.plan")
+        self._build(self._plan)
+
+    def _build(self, pl) -> None:
+        capturing = torch.cuda.is_current_stream_capturing()
+        if capturing:
+            self._keep(pl)
+        check(lib.piekv_shared_prefix_plan(C.byref(pl["args"]), _stream(pl["device"])), "BatchSharedPrefixDecode.plan")
+        if not capturing:
+            pl["built"] = True
+
+    def _keep(self, pl) -> None:
+        """A captured call points to `pl`: no later plan may use its buffer, and it lives on with its tables."""
+        if not pl["captured"]:
+            pl["captured"] = True
+            self._captured.append(pl)
 
     def run(self, q: torch.Tensor, paged_kv_cache: torch.Tensor, out: Optional[torch.Tensor] = None,
             return_lse: bool = False, sinks: Optional[torch.Tensor] = None, sm_scale: Optional[float] = None):
@@ -1085,8 +1103,8 @@ class BatchSharedPrefixDecodeWrapper:
         if self._plan is None:
             raise RuntimeError("Must call plan() before run()")
         pl = self._plan
-        if sinks is None and sm_scale is None and not return_lse:
-            done = _calls.decode_run(pl["native"], q, paged_kv_cache, out)
+        if pl["built"] and sinks is None and sm_scale is None and not return_lse:
+            done = _calls.decode_run(pl["native"], q, paged_kv_cache, out)  # (declines while the stream is captured)
             if done is not False:
                 return done
         device = pl["index"]
@@ -1107,7 +1125,11 @@ class BatchSharedPrefixDecodeWrapper:
         elif out.shape != q.shape or out.dtype != q.dtype or out.get_device() != device or not out.is_contiguous():
             raise ValueError("out must be a contiguous tensor shaped and typed like q")
         lse = torch.empty(pl["shape"][:2], dtype=torch.float32, device=q.device) if return_lse else None
-        a = _lib.SharedPrefixArgs.from_buffer_copy(self._args)  # host threads may run the same plan
+        if torch.cuda.is_current_stream_capturing():
+            self._keep(pl)
+        elif not pl["built"]:  # plan() was only captured: whether that graph has been replayed is not known here
+            self._build(pl)
+        a = _lib.SharedPrefixArgs.from_buffer_copy(pl["args"])  # host threads may run the same plan
         a.q = q.data_ptr()
         a.q_stride_n, a.q_stride_h = qs
         a.pool = paged_kv_cache.data_ptr()

@@ -476,3 +476,46 @@ def test_forked_contexts_from_the_device_page_table():
     got = plain.run(q, pool, return_lse=True)
     P.check_attention(got[0], got[1], args[0], args[1], P.attend(*args, window_left=63, first_tokens=4))
     assert ops.device_error("cuda") is None
+
+
+@pytest.mark.gpu
+def test_captured_runs_outlive_later_plans_of_other_batches():
+    first = Batch([(60, [9, 30, 2, 5] * 8)], 16, 4, seed=21)
+    others = [Batch([(20, [4, 40])], 8, 2, seed=22), Batch([(70, [3] * 64)], 32, 8, seed=23), first]
+    w = first.plan(ops.BatchSharedPrefixDecodeWrapper(_workspace()), groups=None)  # (a grouping that plan() makes itself)
+    q, pool = first.q.cuda(), first.pool.cuda()
+    out = torch.empty_like(q)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        w.replan()
+        w.run(q, pool, out=out)
+    layer = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(layer):
+        again = w.run(q, pool)
+    for b in others:
+        b.plan(w)
+        b.check(w.run(b.q.cuda(), b.pool.cuda(), return_lse=True))
+        for g, result in ((layer, again), (graph, out)):
+            result.fill_(9.0)
+            g.replay()
+            assert ops.device_error("cuda") is None
+            first.check((result, None))
+
+
+@pytest.mark.gpu
+def test_a_plan_that_was_only_captured_runs_eagerly_too():
+    b = Batch([(60, [9, 30, 2]), (5, [1, 2])], 16, 4, seed=24)
+    w = ops.BatchSharedPrefixDecodeWrapper(_workspace())
+    tables = [dev(x) for x in (b.indptr, b.indices, b.last)]
+    ends, q, pool = dev(b.ends), b.q.cuda(), b.pool.cuda()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        w.plan(*tables, 16, 4, 128, 16, group_indptr=ends, q_data_type=torch.bfloat16)
+        captured = w.run(q, pool)
+    b.check(w.run(q, pool, return_lse=True))
+    graph.replay()
+    b.check((captured, None))
+    b.check((w.run(q, pool), None))
+    assert ops.device_error("cuda") is None

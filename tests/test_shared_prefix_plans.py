@@ -1,0 +1,133 @@
+"""Whose memory a shared-prefix plan is: what a captured call points to stays as it was built, on the CPU with a stand-in
+for the device."""
+import weakref
+
+import pytest
+import torch
+
+from pie_b200 import _lib, ops
+
+
+class FakeLib:
+    """The library, with the two calls that would launch something recorded instead."""
+
+    def __init__(self):
+        self.calls, self.status = [], 0
+
+    def __getattr__(self, name):
+        return getattr(_lib.lib, name)
+
+    def _record(self, what, args):
+        args = getattr(args, "_obj", args)  # byref() or the struct
+        self.calls.append((what, _lib.SharedPrefixArgs.from_buffer_copy(args)))
+        return self.status
+
+    def piekv_shared_prefix_plan(self, args, stream):
+        return self._record("plan", args)
+
+    def piekv_shared_prefix_run(self, args, stream):
+        return self._record("run", args)
+
+
+@pytest.fixture
+def device(monkeypatch):
+    fake = FakeLib()
+    fake.capturing = False
+    word = torch.zeros(4, dtype=torch.int32)
+    monkeypatch.setattr(ops, "lib", fake)
+    monkeypatch.setattr(ops, "_require_cuda", lambda t, name: None)
+    monkeypatch.setattr(ops, "_err_word", lambda dev: word)
+    monkeypatch.setattr(ops, "_stream", lambda dev: 0)
+    monkeypatch.setattr(ops, "_stream_of", lambda index: 0)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: fake.capturing)
+    return fake
+
+
+HQ, HKV, D, PAGE = 8, 2, 128, 16
+POOL = torch.zeros((4, 2, PAGE, HKV, D), dtype=torch.bfloat16)
+
+
+def _wrapper():
+    return ops.BatchSharedPrefixDecodeWrapper(torch.empty(8 << 20, dtype=torch.uint8))
+
+
+def _plan(w, batch, groups=None):
+    i32 = lambda n: torch.zeros(n, dtype=torch.int32)  # noqa: E731
+    w.plan(i32(batch + 1), i32(batch + 1), i32(batch), HQ, HKV, D, PAGE, group_indptr=None if groups is None else i32(groups + 1),
+           q_data_type=torch.bfloat16)
+
+
+def _run(w, batch):
+    return w.run(torch.zeros((batch, HQ, D), dtype=torch.bfloat16), POOL)
+
+
+@pytest.mark.parametrize("what", ["run", "replan", "plan"])
+def test_what_was_captured_keeps_its_plan(device, what):
+    w = _wrapper()
+    if what != "plan":
+        _plan(w, 60)
+    device.capturing = True
+    if what == "plan":
+        _plan(w, 60)
+    elif what == "replan":
+        w.replan()
+    if what != "replan":
+        _run(w, 60)
+    device.capturing = False
+    captured = device.calls[-1][1]
+    tables = [weakref.ref(t) for t in w._plan["keep"]]
+    for batch in (7, 60, 61, 7):
+        _plan(w, batch)
+        _run(w, batch)
+        for _, later in device.calls[-2:]:
+            assert later.plan + later.plan_bytes <= captured.plan or captured.plan + captured.plan_bytes <= later.plan
+    assert all(t() is not None for t in tables)  # the page table, and the grouping that plan() made itself
+
+
+def test_plans_that_nothing_captured_share_one_buffer(device):
+    w = _wrapper()
+    _plan(w, 200)
+    for batch in range(1, 60):
+        _plan(w, batch)
+        _run(w, batch)
+    assert len({a.plan for _, a in device.calls}) == 1
+
+
+def test_a_captured_plan_is_kept_once(device):
+    w = _wrapper()
+    _plan(w, 20)
+    device.capturing = True
+    for _ in range(80):  # a layer each
+        _run(w, 20)
+    device.capturing = False
+    first = device.calls[-1][1].plan
+    _plan(w, 20)
+    _plan(w, 20)
+    assert device.calls[-1][1].plan == device.calls[-2][1].plan != first
+
+
+def test_a_plan_that_was_only_captured_is_built_before_an_eager_run(device):
+    w = _wrapper()
+    device.capturing = True
+    _plan(w, 9)
+    _run(w, 9)
+    device.capturing = False
+    assert [c for c, _ in device.calls] == ["plan", "run"]
+    _run(w, 9)  # the buffer holds nothing yet
+    _run(w, 9)
+    assert [c for c, _ in device.calls] == ["plan", "run", "plan", "run", "run"]
+    assert len({a.plan for _, a in device.calls}) == 1
+
+
+def test_a_plan_that_could_not_be_built_is_none(device):
+    w = _wrapper()
+    _plan(w, 9)
+    device.status = 1
+    with pytest.raises(ValueError):
+        _plan(w, 5)
+    device.status = 0
+    for batch in (5, 9):
+        with pytest.raises(RuntimeError, match="plan"):
+            _run(w, batch)
+    _plan(w, 5)
+    _run(w, 5)
