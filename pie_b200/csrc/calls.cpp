@@ -84,15 +84,21 @@ PyObject *bind(PyObject *, PyObject *args) {
   Py_RETURN_NONE;
 }
 
-// rope_axes_append(table address, q, k, v, pos_ids, batch_indices, positions, pool, kv_indices, kv_indptr, q_out | None)
+// rope_axes_append(piekv_rope_axes_table as bytes, q, k, v, pos_ids, batch_indices, positions, pool, kv_indices, kv_indptr, q_out | None)
 PyObject *rope_axes_append(PyObject *, PyObject *const *o, Py_ssize_t count) {
   HANDLE_TH_ERRORS
   if (count != 11) {
     PyErr_SetString(PyExc_TypeError, "rope_axes_append takes 11 arguments");
     return nullptr;
   }
-  const auto *table = static_cast<const piekv_rope_axes_table *>(PyLong_AsVoidPtr(o[0]));
-  if (table == nullptr) return PyErr_Occurred() ? nullptr : declined();
+  if (!PyObject_CheckBuffer(o[0])) return declined();
+  Py_buffer given_table;
+  if (PyObject_GetBuffer(o[0], &given_table, PyBUF_SIMPLE) != 0) return nullptr;
+  piekv_rope_axes_table table;  // a copy: the caller's may change once the interpreter runs other threads
+  const bool is_table = given_table.len == (Py_ssize_t)sizeof(table);
+  if (is_table) std::memcpy(&table, given_table.buf, sizeof(table));
+  PyBuffer_Release(&given_table);
+  if (!is_table) return declined();
   const at::Tensor *k = tensor_on(o[2], -1);
   if (k == nullptr || !is_rows(*k)) return declined();
   const int device = k->get_device(), dtype = dtype_code(*k);
@@ -103,13 +109,13 @@ PyObject *rope_axes_append(PyObject *, PyObject *const *o, Py_ssize_t count) {
   const int64_t n = k->size(0), hkv = k->size(1), d = k->size(2);
   if (q == nullptr || !is_rows(*q) || q->size(0) != n || q->size(2) != d || q->scalar_type() != k->scalar_type()) return declined();
   if (v == nullptr || !is_rows(*v) || v->sizes() != k->sizes() || v->scalar_type() != k->scalar_type()) return declined();
-  if (pos == nullptr || pos->scalar_type() != at::kInt || pos->dim() != 2 || pos->size(0) != table->num_axes || pos->size(1) < n ||
+  if (pos == nullptr || pos->scalar_type() != at::kInt || pos->dim() != 2 || pos->size(0) != table.num_axes || pos->size(1) < n ||
       (n > 1 && pos->stride(1) != 1))
     return declined();
   if (!is_pool(pool) || pool->size(3) != hkv || pool->size(4) != d || pool->scalar_type() != k->scalar_type()) return declined();
   if (!is_i32(batch_indices) || !is_i32(positions) || !is_i32(indices) || !is_i32(indptr)) return declined();
   if (batch_indices->numel() < n || positions->numel() < n || indptr->numel() < 1) return declined();
-  if (2 * (int64_t)table->half > d || !fits(n) || !fits(hkv) || !fits(d) || !fits(q->size(1)) || !fits(pool->size(2)) ||
+  if (2 * (int64_t)table.half > d || !fits(n) || !fits(hkv) || !fits(d) || !fits(q->size(1)) || !fits(pool->size(2)) ||
       !fits(indptr->numel()))
     return declined();
   at::Tensor out;
@@ -153,7 +159,7 @@ PyObject *rope_axes_append(PyObject *, PyObject *const *o, Py_ssize_t count) {
   void *stream = stream_of(device);
   int status;
   Py_BEGIN_ALLOW_THREADS;
-  status = rope_axes_fn(&a, table, stream);
+  status = rope_axes_fn(&a, &table, stream);
   Py_END_ALLOW_THREADS;
   if (status != 0) return declined();
   return THPVariable_Wrap(out);

@@ -620,8 +620,10 @@ def rope_axes_append_paged_kv_cache(q: Optional[torch.Tensor], k: torch.Tensor, 
     with another q_out, q are read only).  `positions` are the tokens' slots in their contexts, as in
     append_paged_kv_cache; a token whose request, slot or page does not exist is skipped and reported
     (`device_error`), its q is still rotated."""
-    if rope.__class__ is AxisRopeConfig and rope.__dict__["_table"] is not None and rope.mode != "table":
-        done = _calls.rope_axes_append(C.addressof(rope.__dict__["_table"]), q, k, v, pos_ids, batch_indices, positions,
+    # (another thread may change the configuration at any moment: its table is asked for once, and held)
+    table = rope.__dict__["_table"] if rope.__class__ is AxisRopeConfig else None
+    if table is not None and not table.cos_sin_table:
+        done = _calls.rope_axes_append(table, q, k, v, pos_ids, batch_indices, positions,
                                        paged_kv_cache, kv_indices, kv_indptr, q_out)
         if done is not False:
             return done
