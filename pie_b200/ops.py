@@ -20,6 +20,7 @@ Error behaviour follows the reference facade: wrong device / dtype / shape raise
 """
 from __future__ import annotations
 
+import copy
 import ctypes as C
 import math
 from dataclasses import dataclass
@@ -475,9 +476,12 @@ class AxisRopeConfig(RopeConfig):
     sections: Tuple[int, ...] = ()
     cyclic: bool = False
 
+    # A table belongs to the parameters it was laid out from: it names their state, which every assignment replaces AFTER
+    # the value is there, so that no thread that reads in the middle leaves an old table behind.
     def __setattr__(self, name, value) -> None:
-        self.__dict__["_table"] = None  # laid out again at the next use
         object.__setattr__(self, name, tuple(value) if isinstance(value, list) else value)
+        self.__dict__["_state"] = object()
+        self.__dict__["_table"] = None
 
     def __getstate__(self):
         return {**self.__dict__, "_table": None}  # a copy lays out its own
@@ -487,20 +491,22 @@ class AxisRopeConfig(RopeConfig):
 
     def prepared(self) -> "_lib.RopeAxesTable":
         """The host table the kernels take, laid out once per set of parameters."""
-        table = self.__dict__["_table"]
-        if table is not None:
-            if self.mode == "table":
-                table.cos_sin_table = self.cos_sin_table.data_ptr()
-            return table
-        sections = [int(x) for x in self.sections]
+        state, table = self.__dict__["_state"], self.__dict__["_table"]
+        if table is not None and table.state is state:
+            source = table.source
+            if source is None or (source.data_ptr() == table.cos_sin_table and source.shape[0] == table.table_len):
+                return table
+        now = copy.copy(self)
+        sections = [int(x) for x in now.sections]
         if not 1 <= len(sections) <= _lib.MAX_ROPE_AXES:
             raise ValueError(f"sections must name 1 to {_lib.MAX_ROPE_AXES} axes, got {len(sections)}")
-        if self.mode == "none":
+        if now.mode == "none":
             raise ValueError("rope mode 'none' has no angles; use append_paged_kv_cache")
-        rp = RopeConfig.to_c(self, 2 * sum(sections))
+        rp = RopeConfig.to_c(now, 2 * sum(sections))
         table = _lib.RopeAxesTable()
+        table.state, table.source = state, now.cos_sin_table if now.mode == "table" else None
         check(lib.piekv_rope_axes_prepare(C.byref(rp), (C.c_int32 * len(sections))(*sections), len(sections),
-                                          1 if self.cyclic else 0, C.byref(table)), "AxisRopeConfig")
+                                          1 if now.cyclic else 0, C.byref(table)), "AxisRopeConfig")
         self.__dict__["_table"] = table
         return table
 
@@ -556,8 +562,8 @@ def _rope_axes(q, k, v, pos_ids, rope: AxisRopeConfig, q_out, k_out, who: str, a
         raise ValueError(f"{who}: pos_ids is on {pos_ids.device}, k on {k.device}")
     if 2 * table.half > d:
         raise ValueError(f"{who}: sections of {table.half} pairs do not fit head_dim {d}")
-    if rope.mode == "table" and rope.cos_sin_table.get_device() != device:
-        raise ValueError(f"{who}: cos_sin_table on {rope.cos_sin_table.device}, k on {k.device}")
+    if table.source is not None and table.source.get_device() != device:
+        raise ValueError(f"{who}: cos_sin_table on {table.source.device}, k on {k.device}")
     q_ptr = qo_ptr = ko_ptr = v_ptr = None
     q_rows = qo_rows = ko_rows = v_rows = (0, 0)
     hq = 0
@@ -622,7 +628,7 @@ def rope_axes_append_paged_kv_cache(q: Optional[torch.Tensor], k: torch.Tensor, 
     (`device_error`), its q is still rotated."""
     # (another thread may change the configuration at any moment: its table is asked for once, and held)
     table = rope.__dict__["_table"] if rope.__class__ is AxisRopeConfig else None
-    if table is not None and not table.cos_sin_table:
+    if table is not None and table.state is rope.__dict__["_state"] and table.source is None:
         done = _calls.rope_axes_append(table, q, k, v, pos_ids, batch_indices, positions,
                                        paged_kv_cache, kv_indices, kv_indptr, q_out)
         if done is not False:
