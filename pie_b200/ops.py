@@ -1048,12 +1048,17 @@ class BatchSharedPrefixDecodeWrapper:
             if t.device != dev:
                 raise ValueError(f"{name} is on {t.device}, indptr on {dev}")
         # as many pieces per prefix as the workspace has room for
-        base = lib.piekv_shared_prefix_workspace_bytes(batch, num_qo_heads, num_kv_heads, head_dim, 1)
-        each = lib.piekv_shared_prefix_workspace_bytes(batch, num_qo_heads, num_kv_heads, head_dim, 2) - base
         have = self.workspace_buffer.numel()
+        base = lib.piekv_shared_prefix_workspace_bytes(batch, num_qo_heads, num_kv_heads, head_dim, 1)
         if have < base:
             raise ValueError(f"workspace_buffer too small: {have} < {base} bytes")
-        splits = min(_lib.SHARED_PREFIX_MAX_SPLITS, 1 + (have - base) // each if each > 0 else 1)
+        splits, above = 1, _lib.SHARED_PREFIX_MAX_SPLITS + 1  # (the bytes of a piece more are not always the same)
+        while above - splits > 1:
+            mid = (splits + above) // 2
+            if lib.piekv_shared_prefix_workspace_bytes(batch, num_qo_heads, num_kv_heads, head_dim, mid) <= have:
+                splits = mid
+            else:
+                above = mid
         plan_bytes = lib.piekv_shared_prefix_plan_bytes(batch, groups, num_qo_heads, num_kv_heads)
         old, buffer = self._plan, None
         if old is not None and not old["captured"] and old["buffer"].numel() >= plan_bytes and old["device"] == dev:

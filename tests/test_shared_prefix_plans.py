@@ -131,3 +131,50 @@ def test_a_plan_that_could_not_be_built_is_none(device):
             _run(w, batch)
     _plan(w, 5)
     _run(w, 5)
+
+
+# ---- into how many pieces a prefix may be cut: as many as the workspace has room for, and not one more
+@pytest.mark.parametrize("batch, hq, hkv", [(21, 1, 1), (14, 12, 4), (7, 24, 8), (23, 12, 2), (1, 1, 1), (5, 3, 1), (64, 32, 8)])
+def test_a_plan_has_room_for_the_pieces_it_names(device, batch, hq, hkv):
+    need = lambda splits: ops.lib.piekv_shared_prefix_workspace_bytes(batch, hq, hkv, D, splits)  # noqa: E731
+    most = _lib.SHARED_PREFIX_MAX_SPLITS
+    i32 = lambda n: torch.zeros(n, dtype=torch.int32)  # noqa: E731
+    sizes = {need(1), need(most), need(most) + 12345}
+    for splits in range(1, most):
+        sizes |= {need(splits + 1) - 1, need(splits + 1), (need(splits) + need(splits + 1)) // 2}
+    whole = torch.empty(max(sizes), dtype=torch.uint8)
+    w = ops.BatchSharedPrefixDecodeWrapper(whole)
+    for have in sorted(sizes):
+        w.workspace_buffer = whole[:have]
+        w.plan(i32(batch + 1), i32(batch + 1), i32(batch), hq, hkv, D, PAGE, q_data_type=torch.bfloat16)
+        splits = device.calls[-1][1].max_splits
+        assert need(splits) <= have and (splits == most or have < need(splits + 1)), (have, splits)
+    w.workspace_buffer = whole[:need(1) - 1]
+    with pytest.raises(ValueError, match="workspace_buffer too small"):
+        w.plan(i32(batch + 1), i32(batch + 1), i32(batch), hq, hkv, D, PAGE, q_data_type=torch.bfloat16)
+
+
+@pytest.mark.gpu
+def test_runs_where_the_workspace_holds_its_pieces_exactly():
+    lens = [3 + 5 * i for i in range(21)]
+    pages = torch.arange(400, dtype=torch.int32, device="cuda")
+    pool = torch.randn((400, 2, PAGE, 1, D), device="cuda").to(torch.bfloat16)
+    q = torch.randn((21, 1, D), device="cuda").to(torch.bfloat16)
+    lists = [list(range(300)) + [300 + i] for i in range(21)]
+    indptr = torch.arange(22, dtype=torch.int32, device="cuda") * 301
+    indices = pages[torch.tensor(sum(lists, []), device="cuda")]
+    last = torch.tensor([(n - 1) % 16 + 1 for n in lens], dtype=torch.int32, device="cuda")
+    results = []
+    for splits in (1, 2, 3, 33, 52, 63, 64):
+        have = _lib.lib.piekv_shared_prefix_workspace_bytes(21, 1, 1, D, splits)
+        for extra in (0, 1, 255, 10240):
+            w = ops.BatchSharedPrefixDecodeWrapper(torch.empty(have + extra, dtype=torch.uint8, device="cuda"))
+            w.plan(indptr, indices, last, 1, 1, D, PAGE, q_data_type=torch.bfloat16)
+            results.append(w.run(q, pool))
+    plain = ops.BatchDecodeWithPagedKVCacheWrapper(torch.empty(64 << 20, dtype=torch.uint8, device="cuda"))
+    plain.plan(indptr, indices, last, 1, 1, D, PAGE, q_data_type=torch.bfloat16)
+    want = plain.run(q, pool).float()
+    # both round P (2^-8 of |v| <= 6 at most, averaged over ~4800 tokens) and the output (half a step of bf16)
+    for got in results:
+        assert (got.float() - want).abs().max().item() <= 2 * (2 ** -8 * 6 + 2 ** -9)
+    assert ops.device_error("cuda") is None
