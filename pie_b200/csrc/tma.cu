@@ -20,6 +20,17 @@ static EncodeTiledFn get_encode_fn() {
   return fn;
 }
 
+// A host thread whose first use of the device this is has no context yet, and the driver's own functions, unlike a
+// launch, do not make the device's current.
+template <typename... Args>
+static CUresult encode_tiled(EncodeTiledFn enc, Args... args) {
+  CUresult r = enc(args...);
+  int dev = 0;
+  if (r == CUDA_ERROR_INVALID_CONTEXT && cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess)
+    r = enc(args...);
+  return r;
+}
+
 static CUtensorMapDataType tm_dtype(int dtype) {
   return dtype == PIEKV_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
 }
@@ -33,9 +44,9 @@ int make_page_tensor_map(CUtensorMap *tm, const void *pool, int num_pages, int h
   cuuint64_t gstr[4] = {row, 128, 256, 16 * row};
   cuuint32_t box[5] = {64, 16, (cuuint32_t)box_halves, (cuuint32_t)box_heads, (cuuint32_t)box_kv};
   cuuint32_t estr[5] = {1, 1, 1, 1, 1};
-  CUresult r = enc(tm, tm_dtype(dtype), 5, const_cast<void *>(pool), gdim, gstr, box, estr,
-                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  CUresult r = encode_tiled(enc, tm, tm_dtype(dtype), 5, const_cast<void *>(pool), gdim, gstr, box, estr,
+                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   PIEKV_REQUIRE(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled (pages) failed with CUresult %d", (int)r);
   return 0;
 }
@@ -48,9 +59,9 @@ int make_q_tensor_map(CUtensorMap *tm, const void *q, int64_t nnz, int hq, int64
   cuuint64_t gstr[3] = {(cuuint64_t)q_sn * 2, 128, (cuuint64_t)q_sh * 2};
   cuuint32_t box[4] = {64, (cuuint32_t)box_rows, (cuuint32_t)box_halves, (cuuint32_t)box_heads};
   cuuint32_t estr[4] = {1, 1, 1, 1};
-  CUresult r = enc(tm, tm_dtype(dtype), 4, const_cast<void *>(q), gdim, gstr, box, estr,
-                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  CUresult r = encode_tiled(enc, tm, tm_dtype(dtype), 4, const_cast<void *>(q), gdim, gstr, box, estr,
+                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   PIEKV_REQUIRE(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled (q) failed with CUresult %d", (int)r);
   return 0;
 }
@@ -64,8 +75,9 @@ int make_q_rows_tensor_map(CUtensorMap *tm, const void *q, int64_t n, int hq, in
   cuuint64_t gstr[3] = {(cuuint64_t)q_sh * 2, (cuuint64_t)q_sn * 2, 128};
   cuuint32_t box[4] = {64, (cuuint32_t)box_heads, (cuuint32_t)box_tokens, 1};
   cuuint32_t estr[4] = {1, 1, 1, 1};
-  CUresult r = enc(tm, tm_dtype(dtype), 4, const_cast<void *>(q), gdim, gstr, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  CUresult r = encode_tiled(enc, tm, tm_dtype(dtype), 4, const_cast<void *>(q), gdim, gstr, box, estr,
+                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   PIEKV_REQUIRE(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled (query rows) failed with CUresult %d", (int)r);
   return 0;
 }
@@ -78,8 +90,9 @@ int make_matrix_tensor_map(CUtensorMap *tm, const void *ptr, int64_t rows, int64
   cuuint64_t gstr[1] = {(cuuint64_t)row_stride * 2};
   cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows};
   cuuint32_t estr[2] = {1, 1};
-  CUresult r = enc(tm, tm_dtype(dtype), 2, const_cast<void *>(ptr), gdim, gstr, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  CUresult r = encode_tiled(enc, tm, tm_dtype(dtype), 2, const_cast<void *>(ptr), gdim, gstr, box, estr,
+                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   PIEKV_REQUIRE(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled (matrix) failed with CUresult %d", (int)r);
   return 0;
 }
