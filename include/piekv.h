@@ -430,7 +430,8 @@ int piekv_prefill_run_opt(const void *q, int64_t q_stride_n, int64_t q_stride_h,
  * piekv_shared_prefix_plan compares the lists and builds the work list in `plan`
  * (piekv_shared_prefix_plan_bytes, 256-byte aligned, private to the caller's batch); piekv_shared_prefix_run
  * uses it for every layer until the page table changes.  A run counts what its blocks have taken in the plan and
- * leaves the counts zero, so a plan, like a workspace, serves one run at a time.  `max_splits` (1 ..
+ * leaves the counts zero, so a plan, like a workspace, serves one run at a time (one stream; host threads may
+ * call at the same time, the launches of a call on a workspace stay together).  `max_splits` (1 ..
  * PIEKV_SHARED_PREFIX_MAX_SPLITS) bounds into how many pieces a prefix is cut; pass the same number to the
  * workspace size, the plan and the run.  The workspace starts with piekv_decode_counter_bytes zeros, left
  * zero.  Shapes the tuned kernels do not cover (fp32, head_dim other than 128, page size other than 16, more

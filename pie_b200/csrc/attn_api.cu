@@ -104,6 +104,7 @@ extern "C" int piekv_decode_run_opt(const void *q, int64_t q_stride_n, int64_t q
   if (int rc = check_common(a, dtype, "decode_run")) return rc;
   if (int rc = apply_options(a, opt, "decode_run")) return rc;
   if (batch == 0) return 0;
+  const WorkspaceTurn turn(workspace);
   if (a.first_tokens > 0) {
     if (decode_span_supported(a, dtype))
       return launch_decode_span(a, dtype, SpanPrefix{}, workspace, workspace_bytes, (cudaStream_t)stream);
@@ -162,6 +163,8 @@ static int decode_step_fused_impl(const void *q, const void *k, const void *v, i
   RopeDev rp;
   fill_inv_freq(rope, head_dim, &rp);
   cudaStream_t st = (cudaStream_t)stream;
+  // (ranks that wait for one another on the device must not wait for one another's launches here)
+  const WorkspaceTurn turn(peer == nullptr ? workspace : nullptr);
   if (decode_fused_tma_supported(a, dtype, k, v, k_stride_n, k_stride_h, v_stride_n, v_stride_h))
     return launch_decode_fused_tma(a, dtype, k, v, k_stride_n, k_stride_h, v_stride_n, v_stride_h, pos_ids, rp,
                                    workspace, workspace_bytes, st, peer);
@@ -305,6 +308,7 @@ extern "C" int piekv_prefill_plan(const int32_t *qo_indptr, const int32_t *kv_in
   AttnArgs a{};
   fill_prefill_args(a, nullptr, 0, 0, nullptr, nullptr, nullptr, qo_indptr, kv_indptr, nullptr, kv_last_page_len,
                     custom_mask, causal, batch, nnz, 1, 1, 128, page_size, num_pages, 1.f, err);
+  const WorkspaceTurn turn(workspace);
   return launch_prefill_plan(a, mask_bytes, workspace, workspace_bytes, (cudaStream_t)stream);
 }
 
@@ -320,6 +324,7 @@ extern "C" int piekv_prefill_plan_brle(const int32_t *qo_indptr, const int32_t *
   AttnArgs a{};
   fill_prefill_args(a, nullptr, 0, 0, nullptr, nullptr, nullptr, qo_indptr, kv_indptr, nullptr, kv_last_page_len,
                     nullptr, 0, batch, nnz, 1, 1, 128, page_size, num_pages, 1.f, err);
+  const WorkspaceTurn turn(workspace);
   return launch_prefill_plan(a, mask_bits, workspace, workspace_bytes, (cudaStream_t)stream, brle_runs, brle_indptr);
 }
 
@@ -345,6 +350,7 @@ extern "C" int piekv_prefill_plan_opt(const int32_t *qo_indptr, const int32_t *k
                     custom_mask, (custom_mask || brle) ? 0 : causal, batch, nnz, 1, 1, 128, page_size, num_pages, 1.f,
                     err);
   a.window_left = window_left;
+  const WorkspaceTurn turn(workspace);
   return launch_prefill_plan(a, mask_entries, workspace, workspace_bytes, (cudaStream_t)stream, brle_runs, brle_indptr);
 }
 
@@ -385,6 +391,7 @@ extern "C" int piekv_prefill_run_opt(const void *q, int64_t q_stride_n, int64_t 
     a.mask = reinterpret_cast<const uint8_t *>(workspace);  // marks "masked"; the packed form is what is read
     a.causal = 0;
   }
+  const WorkspaceTurn turn(workspace);
   // (with a band the tensor-core kernels take a row's maximum before they scale it)
   if (prefill_tc_supported(a, dtype) && (a.first_tokens == 0 || a.sm_scale > 0.f)) {
     if (!planned) {

@@ -31,6 +31,19 @@ int cuda_status(cudaError_t e, const char *what);  // 0 or -(int)e, records text
   } while (0)
 
 int sm_count();  // multiprocessors of the current device (cached per device)
+
+// Held by a call from its first launch on a workspace to its last: several host threads may work on one stream, and what
+// a call's first kernel leaves in the workspace has to be there for its second.  (nullptr: nothing is held.)
+class WorkspaceTurn {
+ public:
+  explicit WorkspaceTurn(const void *workspace);
+  ~WorkspaceTurn();
+  WorkspaceTurn(const WorkspaceTurn &) = delete;
+  WorkspaceTurn &operator=(const WorkspaceTurn &) = delete;
+
+ private:
+  unsigned slot_;
+};
 int current_device_slot();  // ordinal of the current device if it is in [0, kMaxDevices), else -1
 constexpr int kMaxDevices = 64;
 

@@ -2,6 +2,8 @@
 #include <stdarg.h>
 #include <stdio.h>
 
+#include <mutex>
+
 #include "common.cuh"
 
 namespace piekv {
@@ -37,6 +39,16 @@ int sm_count() {
     cached[dev] = n;
   }
   return cached[dev];
+}
+
+constexpr unsigned kTurns = 64;
+static std::mutex g_turns[kTurns];  // by address: workspaces may share one
+WorkspaceTurn::WorkspaceTurn(const void *workspace)
+    : slot_(workspace == nullptr ? kTurns : (unsigned)((reinterpret_cast<uintptr_t>(workspace) >> 9) % kTurns)) {
+  if (slot_ < kTurns) g_turns[slot_].lock();
+}
+WorkspaceTurn::~WorkspaceTurn() {
+  if (slot_ < kTurns) g_turns[slot_].unlock();
 }
 
 static int g_options[8] = {0};

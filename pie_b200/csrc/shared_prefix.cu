@@ -343,6 +343,7 @@ extern "C" int piekv_shared_prefix_run(const piekv_shared_prefix_args *args, voi
   px.max_splits = args->max_splits;
   px.scale_log2 = a.sm_scale * 1.4426950408889634f;
   px.err = a.err;
+  const WorkspaceTurn turn(args->workspace);
   if (int rc = launch_prefix_tc(px, a.pool, a.hkv, args->dtype, st)) return rc;
   SpanPrefix sp;
   sp.requests = v.requests;

@@ -997,7 +997,8 @@ class BatchSharedPrefixDecodeWrapper:
     captured in a CUDA graph together.  The plan lives in a buffer of its own, which later plans use again; what a captured
     call points to (its plan, page table and grouping) is kept, as it was, while the wrapper lives.  The workspace may be
     shared with other wrappers whose calls are ordered on the same stream (a prefill wrapper keeps its plan in its
-    workspace: plan it again after a call of another wrapper on the same one)."""
+    workspace: plan it again after a call of another wrapper on the same one).  Host threads may call wrappers on one
+    stream and workspace at the same time: the launches of a call stay together."""
 
     def __init__(self, float_workspace_buffer: torch.Tensor, kv_layout: str = "NHD") -> None:
         if kv_layout != "NHD":
@@ -1142,7 +1143,7 @@ class BatchSharedPrefixDecodeWrapper:
             self._keep(pl)
         elif not pl["built"]:  # plan() was only captured: whether that graph has been replayed is not known here
             self._build(pl)
-        a = _lib.SharedPrefixArgs.from_buffer_copy(pl["args"])  # host threads may run the same plan
+        a = _lib.SharedPrefixArgs.from_buffer_copy(pl["args"])  # host threads may run the same plan on one stream
         a.q = q.data_ptr()
         a.q_stride_n, a.q_stride_h = qs
         a.pool = paged_kv_cache.data_ptr()
