@@ -300,4 +300,12 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_calls", nullptr, -1, methods, nul
 
 }  // namespace
 
-extern "C" __attribute__((visibility("default"))) PyObject *PyInit__calls() { return PyModule_Create(&module); }
+extern "C" __attribute__((visibility("default"))) PyObject *PyInit__calls() {
+  PyObject *m = PyModule_Create(&module);
+  // ops.py compares it with the torch that is loaded
+  if (m != nullptr && PyModule_AddStringConstant(m, "torch_version", PIEKV_TORCH_VERSION) != 0) {
+    Py_DECREF(m);
+    return nullptr;
+  }
+  return m;
+}

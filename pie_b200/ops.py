@@ -23,13 +23,42 @@ from __future__ import annotations
 import copy
 import ctypes as C
 import math
+import warnings
 from dataclasses import dataclass
 from typing import Optional, Sequence, Tuple
 
 import torch
 
-from . import _calls, _lib
+from . import _lib
 from ._lib import RopeParams, check, lib
+
+
+class _NoCalls:
+    """In the place of the native way into the short calls where that does not load: it declines every call, and the
+    functions below go on themselves, with the same checks, to the same kernels."""
+
+    @staticmethod
+    def _decline(*_args) -> bool:
+        return False
+
+    bind = set_error_word = plan = rope_axes_append = decode_run = prefill_run = _decline
+
+
+try:
+    from . import _calls
+
+    if _calls.torch_version != str(torch.__version__):
+        raise ImportError(f"_calls.so was built for torch {_calls.torch_version}, this is {torch.__version__}")
+except ImportError as e:
+    warnings.warn(f"pie_b200: {e}; calls take 3 to 8 us more of the host's time until `python pie_b200/build.py` has built it "
+                  "again", RuntimeWarning, stacklevel=2)
+    _calls = _NoCalls()
+
+
+def native_calls_loaded() -> bool:
+    """Whether short calls go through the native module (`_calls.so`) instead of Python."""
+    return not isinstance(_calls, _NoCalls)
+
 
 _calls.bind(*(C.cast(f, C.c_void_p).value
               for f in (lib.piekv_rope_axes, lib.piekv_shared_prefix_run, lib.piekv_decode_run_opt, lib.piekv_prefill_run_opt)))
