@@ -1038,6 +1038,8 @@ class BatchSharedPrefixDecodeWrapper:
         float_workspace_buffer[:COUNTER_BYTES].zero_()
         self._plan = None
         self._captured = []  # plans that captured calls point to
+        self._buffers = []  # all plan buffers: one that became too small may still be read on another stream
+        self._free = None  # the one that the next plan may use again
 
     def plan(self, indptr: torch.Tensor, indices: torch.Tensor, last_page_len: torch.Tensor, num_qo_heads: int,
              num_kv_heads: int, head_dim: int, page_size: int, group_indptr: Optional[torch.Tensor] = None,
@@ -1065,15 +1067,14 @@ class BatchSharedPrefixDecodeWrapper:
         if last_page_len.shape[0] < batch:
             raise ValueError("last_page_len shorter than the batch")
         dev = indptr.device
-        if group_indptr is None:
-            group_indptr = torch.empty(2, dtype=torch.int32, device=dev)
-            group_indptr[:1].zero_()
-            group_indptr[1:].fill_(batch)
-        _require_i32(group_indptr, "group_indptr")
-        groups = group_indptr.shape[0] - 1
+        groups = 1
+        if group_indptr is not None:
+            _require_i32(group_indptr, "group_indptr")
+            groups = group_indptr.shape[0] - 1
         if groups < (1 if batch > 0 else 0):
             raise ValueError("group_indptr must hold groups + 1 entries")
-        for t, name in ((indices, "indices"), (last_page_len, "last_page_len"), (group_indptr, "group_indptr"),
+        for t, name in ((indices, "indices"), (last_page_len, "last_page_len"),
+                        (indptr if group_indptr is None else group_indptr, "group_indptr"),
                         (self.workspace_buffer, "workspace_buffer")):
             if t.device != dev:
                 raise ValueError(f"{name} is on {t.device}, indptr on {dev}")
@@ -1090,18 +1091,22 @@ class BatchSharedPrefixDecodeWrapper:
             else:
                 above = mid
         plan_bytes = lib.piekv_shared_prefix_plan_bytes(batch, groups, num_qo_heads, num_kv_heads)
-        old, buffer = self._plan, None
-        if old is not None and not old["captured"] and old["buffer"].numel() >= plan_bytes and old["device"] == dev:
-            buffer = old["buffer"]
-        if buffer is None:
-            buffer = torch.empty(max(plan_bytes, 4096), dtype=torch.uint8, device=dev)
+        own = (plan_bytes + 255) // 256 * 256  # (plan() keeps a grouping of its own behind the plan)
+        if self._free is None or self._free.numel() < own + 8 or self._free.device != dev:
+            self._free = torch.empty(1 << (own + 7).bit_length(), dtype=torch.uint8, device=dev)
+            self._buffers.append(self._free)
+        buffer = self._free
+        if group_indptr is None:
+            group_indptr = own_group = buffer[own:own + 8].view(torch.int32)
+        else:
+            own_group = None
         a = _lib.SharedPrefixArgs()
         a.kv_indptr = indptr.data_ptr()
         a.kv_indices = indices.data_ptr()
         a.kv_last_page_len = last_page_len.data_ptr()
         a.group_indptr = group_indptr.data_ptr()
         a.plan = buffer.data_ptr()
-        a.plan_bytes = buffer.numel()
+        a.plan_bytes = plan_bytes
         a.workspace = self.workspace_buffer.data_ptr()
         a.workspace_bytes = have
         a.err = _err_word(dev).data_ptr()
@@ -1116,7 +1121,10 @@ class BatchSharedPrefixDecodeWrapper:
                   cache=(int(page_size), int(num_kv_heads), int(head_dim)), sm_scale=a.sm_scale,
                   keep=(indptr, indices, last_page_len, group_indptr), args=a, buffer=buffer,
                   native=_calls.plan(indptr.get_device(), a, None), captured=False, built=False)
-        self._plan = None  # until this one is built
+        self._plan = None  # until this one is built: the buffer may be the last one's
+        if own_group is not None:
+            own_group[:1].zero_()
+            own_group[1:].fill_(batch)
         self._build(pl)
         self._plan = pl
 
@@ -1139,6 +1147,8 @@ class BatchSharedPrefixDecodeWrapper:
         if not pl["captured"]:
             pl["captured"] = True
             self._captured.append(pl)
+            if self._free is pl["buffer"]:
+                self._free = None
 
     def run(self, q: torch.Tensor, paged_kv_cache: torch.Tensor, out: Optional[torch.Tensor] = None,
             return_lse: bool = False, sinks: Optional[torch.Tensor] = None, sm_scale: Optional[float] = None):

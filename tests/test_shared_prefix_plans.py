@@ -178,3 +178,29 @@ def test_runs_where_the_workspace_holds_its_pieces_exactly():
     for got in results:
         assert (got.float() - want).abs().max().item() <= 2 * (2 ** -8 * 6 + 2 ** -9)
     assert ops.device_error("cuda") is None
+
+
+def test_a_buffer_that_became_too_small_stays(device):
+    """A run on another stream than the buffer's may still read it."""
+    w = ops.BatchSharedPrefixDecodeWrapper(torch.empty(256 << 20, dtype=torch.uint8))
+    _plan(w, 3)
+    first = weakref.ref(w._plan["buffer"])
+    small = device.calls[-1][1]
+    for batch in (20000, 100000, 3):
+        i32 = lambda n: torch.zeros(n, dtype=torch.int32)  # noqa: E731
+        w.plan(i32(batch + 1), i32(batch + 1), i32(batch), 1, 1, D, PAGE, q_data_type=torch.bfloat16)
+    assert first() is not None
+    for _, a in device.calls[1:]:
+        assert a.plan + a.plan_bytes <= small.plan or small.plan + small.plan_bytes <= a.plan
+    sizes = {a.plan: a.plan_bytes for _, a in device.calls}
+    assert len(sizes) <= 3
+
+
+def test_the_grouping_that_plan_makes_lives_in_the_plan_buffer(device):
+    w = _wrapper()
+    for batch in (5, 300, 0):
+        _plan(w, batch)
+        a, buffer = device.calls[-1][1], w._plan["buffer"]
+        assert a.plan + a.plan_bytes <= a.group_indptr <= buffer.data_ptr() + buffer.numel() - 8
+        assert w._plan["keep"][3].tolist() == [0, batch] and w._plan["keep"][3].data_ptr() == a.group_indptr
+        assert a.plan == buffer.data_ptr() and a.num_groups == 1
