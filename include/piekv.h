@@ -474,7 +474,8 @@ int piekv_shared_prefix_run(const piekv_shared_prefix_args *args, void *stream);
  *   cyclic = 0   blocks in order: the first sections[0] pairs axis 0, the next sections[1] axis 1, ...
  *   cyclic = 1   i mod num_axes for pairs i < num_axes * sections[i mod num_axes], else axis 0
  * and its angle pos[axis][token] * f_i with the f_i of `rope` taken over rotary_dim.  The angle is formed as
- * a 64-bit fixed-point fraction of a turn, so it is as exact at position 10^6 as at 10.  rope->mode PLAIN,
+ * a 64-bit fixed-point fraction of a turn, so it is as exact at position 10^6 as at 10
+ * (the frequency has 51 bits: 2^-22 turn at position 2^31).  rope->mode PLAIN,
  * LLAMA31 or TABLE (rows of rotary_dim floats; pair i reads row pos[axis]).
  *
  * piekv_rope_axes_prepare lays the pairs out once per configuration (host only, no launch); `table` is a

@@ -1,9 +1,11 @@
 // Rotary positions on several axes (time, height, width of an image or a video), with the append into the
 // paged cache.
 //
-// Pair i of a head row turns by the angle pos[axis(i)] * f_i.  Both factors are kept as fractions of a turn in
-// 64-bit fixed point: F_i = f_i / (2 pi) * 2^64, and pos * F_i modulo 2^64 IS the angle modulo a turn, exactly,
-// for every 32-bit position (an fp32 product of position and frequency is off by 0.01 rad at position 2^18).
+// Pair i of a head row turns by the angle pos[axis(i)] * f_i, kept as a fraction of a turn in 64-bit fixed point:
+// F_i = f_i / (2 pi) * 2^64, and pos * F_i modulo 2^64 is the angle modulo a turn, without a rounding of its own (an fp32
+// product of position and frequency is off by 0.01 rad at position 2^18).  F_i itself comes from a double, within 2^-51
+// of itself: the angle is off by up to |pos| * 2^-53 turn, less than the 2^-32 turn that are kept of it up to position
+// 2^21, 2^-22 turn (1.5e-6 rad) at position 2^31.
 // The nearest quarter turn is taken off as an integer, the rest (|r| <= 1/8 turn) goes through sincospif.
 // x' = x c - y s, y' = x s + y c with separately rounded products and sums, one rounding to the storage type,
 // as the one-axis kernels do (rope.cuh).
