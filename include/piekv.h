@@ -424,7 +424,7 @@ int piekv_prefill_run_opt(const void *q, int64_t q_stride_n, int64_t q_stride_h,
  * Groups are runs of consecutive requests: group g holds requests group_indptr[g] .. group_indptr[g + 1),
  * group_indptr[0] = 0, group_indptr[num_groups] = batch.  What a group shares is found on the device by
  * comparing the page lists (full pages only), so the result equals piekv_decode_run's for any grouping; a
- * grouping that shares nothing only costs the comparison.  A group_indptr that is not monotone from 0 to
+ * grouping that shares nothing costs the comparison, and per run the launch of a kernel that finds no work.  A group_indptr that is not monotone from 0 to
  * batch sets PIEKV_ERR_INDPTR and shares nothing.
  *
  * piekv_shared_prefix_plan compares the lists and builds the work list in `plan`

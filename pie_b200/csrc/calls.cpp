@@ -2,11 +2,12 @@
 //
 // A decode step's kernels take 5 to 10 us; asking eleven tensors for shape, strides, type and device from Python takes
 // as long again.  Each function here makes exactly the checks of the Python function of the same operator (ops.py) and
-// launches, or returns False without side effects when any of them does not hold: the Python function then goes on with
-// its own checks, which say what is wrong, and with the rare forms that are not taken here.  Nothing is kept from
-// call to call but what a plan holds.  Host time of a call, checks in Python and here: multi-axis append 13.7 and 6.8 us,
-// decode with first tokens 10.4 and 5.0, prefill with first tokens 11.9 and 8.2, shared-prefix decode 11.2 and 7.4 (two
-// launches, two tensor maps).
+// launches, or returns False: nothing is launched when a check does not hold, and the Python function then goes on with
+// its own checks, which say what is wrong, and with the rare forms that are not taken here.  It returns False too when the
+// library reports an error, for the Python function to make the call again and raise it; a first launch of two may then
+// run twice, which writes the same.  Nothing is kept from call to call but what a plan holds.  Host time of a call, checks
+// in Python and here: multi-axis append 13.7 and 6.8 us, decode with first tokens 10.4 and 5.0, prefill with first tokens
+// 11.9 and 5.2, shared-prefix decode 11.2 and 7.9 (two launches, three tensor maps, a look at the stream's capture).
 #include <Python.h>
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAFunctions.h>

@@ -33,7 +33,8 @@
 // streaming is 2.  More stages of one page, one head per CTA, or two shares per CTA changed the long cases by under 3 %.
 //
 // Precision: a GQA group of up to 8 heads fills rows 0-7 of the 16-row MMA.  Rows 8-15 then carry the part of each
-// probability that its 16-bit rounding drops, so P V is formed with 16 bits of P (bf16) at no extra MMA.
+// probability that its 16-bit rounding drops, so P V is formed with 16 bits of P (bf16) at no extra MMA.  Groups of 9 to
+// 16 heads (WIDE) need all rows: P is rounded to the storage type there, as in the prefix and prefill kernels.
 #include <cuda.h>
 
 #include <type_traits>

@@ -226,8 +226,11 @@ __global__ void __launch_bounds__(kThreads, 3) rope_axes_rows_kernel(const __gri
 // rotation itself passes through registers - in place in the stage; v never does.  A block's positions and page rows
 // are looked up 128 tokens at a time, (cos, sin) of the next token are formed while the copies of this one fly.
 // Measured (20480 tokens, 32 q / 8 kv heads, bf16, 504 MB moved): 92.6 us, 5.4 TB/s, 0.83 of the copy rate.  Blocks per
-// SM: 3 of 50 KB 119.6 us, 5 92.8, 6 98.4; 256 threads 95.4, 64 threads and 8 blocks 108.5.  Rows through registers
-// instead of the ring (the kernel for few tokens): 297.
+// SM: 3 of 50 KB 119.6 us, 5 92.8, 6 98.4; 256 threads 95.4, 64 threads and 8 blocks 108.5.  The same rows with the heads
+// eight elements apart, through the registers of the kernel above: 123 us; one element apart, through the element-wise
+// kernel: 294; 64 of 128 elements rotated, the same: 342.  A token of more than half of kBulkSmem (two stages have to
+// fit) goes through registers too: 8192 tokens of 64 / 8 heads of 256, bf16 (671 MB) 129 us, 5.2 TB/s; of 128, fp32, 115 us,
+// 5.8 TB/s; two stages, 64 / 8 heads of 128, bf16: 61 us, 5.5 TB/s.
 constexpr int kBulkThreads = 128;
 constexpr int kBulkChunk = 128;
 constexpr int kMaxStages = 4;

@@ -12,7 +12,10 @@ using namespace sprefix;
 namespace {
 
 constexpr int64_t kCounterBytes = 65536;
-// A prefix shorter than this is left to the requests: reading it once saves less than joining two parts costs.
+// A prefix shorter than this is left to the requests.  Measured (32 / 8 heads, bf16, up to 64 tokens of their own, in a
+// graph), 3 pages left and 4 read once: one group of 4 requests 11.0 and 9.6 us, of 64 13.3 and 13.9, 16 groups of 4 12.8
+// and 13.3.  Many small groups pay for the joins until the prefix is longer: 64 groups of 2, 3 pages left 19.0, 8 read once
+// 33.6 (the plain decode call 25.6), 32 pages 41.7 (42.7), 128 pages 105 (128).
 constexpr int kMinSharedPages = 4;
 
 // Full pages of request b (the partly filled last page of a fork is a copy of its own).
@@ -64,7 +67,8 @@ __global__ void __launch_bounds__(128) sp_match_kernel(const int32_t *__restrict
 // problem's rows (bound by its stream) or two (by the tensor and special-function pipes), an item's own costs.  The
 // other kernel: starting it beside the prefix kernel or behind it, a tile's worth of own pages; a warp's step of the join
 // (four rows, four partial results), of which an SM has kFoldWarps under way.  Two kernels that stream at the same time
-// slow each other down by up to kContention.
+// slow each other down by up to kContention.  Every thread walks all groups: 8 us for one group, 20 for 16, 57 for 64, 203 for
+// 256 (match and plan, in a graph).
 constexpr float kStartPrefix = 16.f, kTileSingle = 5.f, kTilePair = 7.5f, kOpenItem = 6.f;
 constexpr float kStartBeside = 24.f, kStartBehind = 90.f, kOwnTile = 6.f, kFoldStep = 4.5f, kFoldWarps = 8.f, kContention = 0.3f;
 constexpr int kMaxSearchGroups = 256;
@@ -193,7 +197,9 @@ __global__ void __launch_bounds__(1024) sp_plan_kernel(const int32_t *__restrict
     }
   }
   __syncthreads();
-  // hundreds of groups are pieces enough: all SMs, whole prefixes
+  // No search for more groups: all SMs, whole prefixes.  For groups alike that costs a little (groups of 2 behind 512 tokens: 256
+  // 116 us, 257 129); one long prefix among them is then one item per kv head (16384 tokens, the others 128: 87 and 203 us, the
+  // plain decode call 83 and 89).
   const int best = sh_best == ~0ull ? 31 * 32 : (int)(sh_best & 1023);
   ctas = max(1, sms * (best / 32 + 1) / 32);
   per = (most + best % 32) / (best % 32 + 1);

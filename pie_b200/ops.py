@@ -1019,9 +1019,10 @@ class BatchSharedPrefixDecodeWrapper:
     within rounding, for any grouping.
 
     `plan()` takes the page table of the decode wrapper and `group_indptr` (int32 [groups + 1]: group g holds the
-    consecutive requests group_indptr[g] .. group_indptr[g + 1) - 1; None: the whole batch is one group).  How many
-    full pages the requests of a group share is found on the device by comparing their page lists; nothing is read
-    back.  The plan holds until the page table's contents change; `replan()` rebuilds it from the same tensors.  Both
+    consecutive requests group_indptr[g] .. group_indptr[g + 1] - 1; None: the whole batch is one group).  How many
+    full pages ALL requests of a group share is found on the device by comparing their page lists; nothing is read back
+    (an empty request, or one without the prefix, leaves its group without sharing: put it into a group of its own).
+    The plan holds until the page table's contents change; `replan()` rebuilds it from the same tensors.  Both
     only launch kernels on the current stream, so plan / replan and any number of run() calls (one per layer) can be
     captured in a CUDA graph together.  The plan lives in a buffer of its own, which later plans use again; what a captured
     call points to (its plan, page table and grouping) is kept, as it was, while the wrapper lives.  The workspace may be
