@@ -1027,8 +1027,9 @@ class BatchSharedPrefixDecodeWrapper:
     captured in a CUDA graph together.  The plan lives in a buffer of its own, which later plans use again; what a captured
     call points to (its plan, page table and grouping) is kept, as it was, while the wrapper lives.  The workspace may be
     shared with other wrappers whose calls are ordered on the same stream (a prefill wrapper keeps its plan in its
-    workspace: plan it again after a call of another wrapper on the same one).  Host threads may call wrappers on one
-    stream and workspace at the same time: the launches of a call stay together."""
+    workspace: plan it again after a call of another wrapper on the same one).  Host threads may run wrappers on one
+    stream and workspace at the same time: the launches of a run stay together.  plan() replaces what run() uses: no
+    other thread may be in a call of the same wrapper meanwhile."""
 
     def __init__(self, float_workspace_buffer: torch.Tensor, kv_layout: str = "NHD") -> None:
         if kv_layout != "NHD":

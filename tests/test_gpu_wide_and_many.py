@@ -1,11 +1,12 @@
 """Shapes at which the kernels change over: wide tokens in the multi-axis append, and batches of more than one slice."""
+import numpy as np
 import pytest
 import torch
 
 from pie_b200 import ops
 from tests import plain64 as P
 from tests.test_gpu_shared_prefix import Batch, _workspace
-from tests.util import dev
+from tests.util import dev, make_scenario
 
 THETA = 500000.0
 
@@ -63,3 +64,63 @@ def test_a_group_with_an_outlier_is_right_and_one_apart_shares():
         w = b.plan(ops.BatchSharedPrefixDecodeWrapper(_workspace()), groups=dev(torch.tensor(ends, dtype=torch.int32).numpy()))
         b.check(w.run(b.q.cuda(), b.pool.cuda(), return_lse=True))
     assert ops.device_error("cuda") is None
+
+
+@pytest.fixture(scope="module")
+def far_pool():
+    """A cache of more than 2^31 elements (4.6 GB), of which the tests use the last pages."""
+    return torch.empty((70000, 2, 16, 8, 128), dtype=torch.bfloat16, device="cuda")
+
+
+def _far(pool, far):
+    """(`far` with the pages of `pool` at its end, what to add to a page id)"""
+    n = pool.shape[0]
+    far[-n:] = pool
+    return far, far.shape[0] - n
+
+
+@pytest.mark.gpu
+def test_shared_prefix_in_a_long_cache(far_pool):
+    b = Batch([(60, [9, 30, 2, 300]), (8, [1, 2])], 32, 8, seed=43)
+    near = b.plan(ops.BatchSharedPrefixDecodeWrapper(_workspace())).run(b.q.cuda(), b.pool.cuda())
+    far, shift = _far(b.pool.cuda(), far_pool)
+    b.indices = b.indices + shift
+    got = b.plan(ops.BatchSharedPrefixDecodeWrapper(_workspace())).run(b.q.cuda(), far)
+    assert torch.equal(got, near) and ops.device_error("cuda") is None
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("prefill", [False, True])
+def test_first_tokens_in_a_long_cache(far_pool, prefill):
+    sc = make_scenario(32, 8, 128, torch.bfloat16, [(200, 70), (0, 130)] if prefill else [(c, 1) for c in (3, 700, 77)])
+    m, outs = sc.meta, []
+    far, shift = _far(sc.pool.cuda(), far_pool)
+    for pool, add in ((sc.pool.cuda(), 0), (far, shift)):
+        tables = (dev(m.kv_indptr), dev(m.kv_indices + np.int32(add)), dev(m.kv_last_page_len), 32, 8, 128, 16)
+        extra = dict(window_left=60, first_tokens=3, q_data_type=torch.bfloat16)
+        if prefill:
+            w = ops.BatchPrefillWithPagedKVCacheWrapper(_workspace())
+            w.plan(dev(m.qo_indptr), *tables, causal=True, **extra)
+        else:
+            w = ops.BatchDecodeWithPagedKVCacheWrapper(_workspace())
+            w.plan(*tables, **extra)
+        outs.append(w.run(sc.q.cuda(), pool))
+    assert torch.equal(*outs) and ops.device_error("cuda") is None
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [5, 1300])
+def test_axes_in_a_long_cache(far_pool, n):
+    pages = -(-n // 16)
+    g = torch.Generator().manual_seed(n)
+    q, k, v = (torch.randn((n, h, 128), generator=g).to(torch.bfloat16).cuda() for h in (32, 8, 8))
+    pos = torch.randint(0, 50000, (3, n), generator=g, dtype=torch.int32).cuda()
+    slots = torch.arange(n, dtype=torch.int32, device="cuda")
+    rope = ops.AxisRopeConfig(mode="plain", theta=THETA, scale=1.0, sections=(16, 24, 24))
+    near = torch.zeros((pages, 2, 16, 8, 128), dtype=torch.bfloat16, device="cuda")
+    far, shift = _far(near, far_pool)
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    outs = [ops.rope_axes_append_paged_kv_cache(q, k, v, pos, torch.zeros_like(slots), slots, pool,
+                                                torch.arange(pages, dtype=torch.int32, device="cuda") + add, i32(0, pages),
+                                                i32((n - 1) % 16 + 1), rope) for pool, add in ((near, 0), (far, shift))]
+    assert torch.equal(*outs) and torch.equal(near, far[shift:]) and ops.device_error("cuda") is None
