@@ -1291,7 +1291,7 @@ class BatchPrefillWithPagedKVCacheWrapper:
                           last_page_len=paged_kv_last_page_len, batch=batch, hq=int(num_qo_heads),
                           hkv=int(num_kv_heads), d=int(head_dim_qk), page_size=int(page_size), mask=mask,
                           mask_bytes=int(mask.numel()) if mask is not None else (brle[2] if brle else window_entries),
-                          brle=brle, causal=bool(causal), dtype=q_data_type, planned_for=None,
+                          brle=brle, causal=bool(causal), dtype=q_data_type, planned_for=None, only_captured=False,
                           window_left=int(window_left), first_tokens=first_tokens,
                           sm_scale=float(sm_scale) if sm_scale is not None else 1.0 / math.sqrt(head_dim_qk))
         if first_tokens > 0:
@@ -1320,7 +1320,8 @@ class BatchPrefillWithPagedKVCacheWrapper:
         of the same batch - one per layer in the reference - reuse it."""
         pl = self._plan
         key = (n, num_pages)
-        if pl["planned_for"] == key:
+        # (a work list whose kernels were only captured is there after a replay, of which nothing is known here)
+        if pl["planned_for"] == key and not (pl["only_captured"] and not torch.cuda.is_current_stream_capturing()):
             return
         ws = self.workspace_buffer
         need = lib.piekv_prefill_workspace_bytes(pl["batch"], n, pl["hq"], pl["d"], num_pages, pl["mask_bytes"])
@@ -1340,7 +1341,7 @@ class BatchPrefillWithPagedKVCacheWrapper:
                                          pl["window_left"] if pl["first_tokens"] == 0 else -1, pl["batch"], n,
                                          pl["page_size"], num_pages, ws.data_ptr(), ws.numel(),
                                          _err_word(dev).data_ptr(), _stream(dev)), "BatchPrefill.plan")
-        pl["planned_for"] = key
+        pl["planned_for"], pl["only_captured"] = key, torch.cuda.is_current_stream_capturing()
 
     def run(self, q: torch.Tensor, paged_kv_cache: torch.Tensor, out: Optional[torch.Tensor] = None,
             return_lse: bool = False, sinks: Optional[torch.Tensor] = None, sm_scale: Optional[float] = None):
@@ -1387,7 +1388,7 @@ class BatchPrefillWithPagedKVCacheWrapper:
         """run() of a plan with a window and first tokens: the same checks, what the plan fixes prepared once."""
         pl = self._plan
         if sinks is None and sm_scale is None and not return_lse:
-            done = _calls.prefill_run(pl["native"], pl["planned_for"], q, paged_kv_cache, out)
+            done = _calls.prefill_run(pl["native"], None if pl["only_captured"] else pl["planned_for"], q, paged_kv_cache, out)
             if done is not False:
                 return done
         device, tables, sizes, tail, options = pl["first_call"]
@@ -1409,8 +1410,7 @@ class BatchPrefillWithPagedKVCacheWrapper:
         elif out.shape != q.shape or out.dtype != q.dtype or out.get_device() != device or not out.is_contiguous():
             raise ValueError("out must be a contiguous tensor shaped and typed like q")
         lse = torch.empty((n, hq), dtype=torch.float32, device=q.device) if return_lse else None
-        if pl["planned_for"] != (n, num_pages):
-            self._device_plan(n, num_pages)
+        self._device_plan(n, num_pages)
         if sinks is not None:
             options = _attn_options(pl["window_left"], sinks, hq, pl["first_tokens"])
         status = lib.piekv_prefill_run_opt(q.data_ptr(), *q_rows, paged_kv_cache.data_ptr(), out.data_ptr(),
