@@ -1210,7 +1210,10 @@ class BatchPrefillWithPagedKVCacheWrapper:
 
     Extension: `plan(..., brle_mask=(runs, indptr, mask_bits))` takes the mask in its wire form (per
     query token a list of alternating attend / skip run lengths, `pie_b200.batching.Batch.brle_inputs`)
-    and builds the bit-packed mask on the device; the flat boolean mask is never materialised."""
+    and builds the bit-packed mask on the device; the flat boolean mask is never materialised.
+
+    The work list of a plan lives in the workspace, built by the first run() after plan(): a captured run() reads the one that
+    is there when it is replayed.  Capture the first run() with it, or leave the workspace to that plan."""
 
     def __init__(self, float_workspace_buffer: torch.Tensor, kv_layout: str = "NHD", **_ignored) -> None:
         if kv_layout != "NHD":
