@@ -80,6 +80,7 @@ __all__ = [
     "AxisRopeConfig",
     "copy_kv_pages",
     "RopeConfig",
+    "native_calls_loaded",
     "device_error",
     "COUNTER_BYTES",
 ]
@@ -827,6 +828,7 @@ class BatchDecodeWithPagedKVCacheWrapper:
                 if t.device != indptr.device:
                     raise ValueError(f"{name} is on {t.device}, indptr on {indptr.device}")
             pl = self._plan
+            pl["workspace"] = self.workspace_buffer  # whose address the calls below hold
             pl["shape"] = torch.Size((batch, pl["hq"], pl["d"]))
             pl["first_options"] = _attn_options(pl["window_left"], None, pl["hq"], first_tokens)
             pl["first_call"] = ((indptr.data_ptr(), indices.data_ptr(), last_page_len.data_ptr(), batch, pl["hq"],
@@ -1121,7 +1123,7 @@ class BatchSharedPrefixDecodeWrapper:
         pl = dict(shape=torch.Size((batch, int(num_qo_heads), int(head_dim))), dtype=q_data_type, device=dev,
                   index=indptr.get_device(),
                   cache=(int(page_size), int(num_kv_heads), int(head_dim)), sm_scale=a.sm_scale,
-                  keep=(indptr, indices, last_page_len, group_indptr), args=a, buffer=buffer,
+                  keep=(indptr, indices, last_page_len, group_indptr, self.workspace_buffer), args=a, buffer=buffer,
                   native=_calls.plan(indptr.get_device(), a, None), captured=False, built=False)
         self._plan = None  # until this one is built: the buffer may be the last one's
         if own_group is not None:
@@ -1295,6 +1297,7 @@ class BatchPrefillWithPagedKVCacheWrapper:
                           hkv=int(num_kv_heads), d=int(head_dim_qk), page_size=int(page_size), mask=mask,
                           mask_bytes=int(mask.numel()) if mask is not None else (brle[2] if brle else window_entries),
                           brle=brle, causal=bool(causal), dtype=q_data_type, planned_for=None, only_captured=False,
+                          workspace=self.workspace_buffer,
                           window_left=int(window_left), first_tokens=first_tokens,
                           sm_scale=float(sm_scale) if sm_scale is not None else 1.0 / math.sqrt(head_dim_qk))
         if first_tokens > 0:
@@ -1326,7 +1329,7 @@ class BatchPrefillWithPagedKVCacheWrapper:
         # (a work list whose kernels were only captured is there after a replay, of which nothing is known here)
         if pl["planned_for"] == key and not (pl["only_captured"] and not torch.cuda.is_current_stream_capturing()):
             return
-        ws = self.workspace_buffer
+        ws = pl["workspace"]
         need = lib.piekv_prefill_workspace_bytes(pl["batch"], n, pl["hq"], pl["d"], num_pages, pl["mask_bytes"])
         if ws.numel() < need:
             raise ValueError(f"workspace_buffer too small: {ws.numel()} < {need} bytes")
@@ -1369,7 +1372,7 @@ class BatchPrefillWithPagedKVCacheWrapper:
         elif tuple(out.shape) != tuple(q.shape) or out.dtype != q.dtype or not out.is_contiguous():
             raise ValueError("out must be a contiguous tensor shaped and typed like q")
         lse = torch.empty((n, pl["hq"]), dtype=torch.float32, device=q.device) if return_lse else None
-        ws = self.workspace_buffer
+        ws = pl["workspace"]
         self._device_plan(n, num_pages)
         opt = _attn_options(pl["window_left"], sinks, pl["hq"])
         check(lib.piekv_prefill_run_opt(q.data_ptr(), qs[0], qs[1], paged_kv_cache.data_ptr(), out.data_ptr(),
@@ -1438,7 +1441,7 @@ class BatchPrefillWithPagedKVCacheWrapper:
             raise ValueError("the packed mask exists for page size 16 only")
         self._device_plan(int(num_query_tokens), int(num_pages))
         flat = torch.zeros(pl["mask_bytes"], dtype=torch.uint8, device=pl["qo_indptr"].device)
-        ws = self.workspace_buffer
+        ws = pl["workspace"]
         check(lib.piekv_prefill_export_mask(pl["qo_indptr"].data_ptr(), pl["indptr"].data_ptr(),
                                             pl["last_page_len"].data_ptr(), pl["mask_bytes"], pl["batch"],
                                             int(num_query_tokens), 16, int(num_pages), ws.data_ptr(), ws.numel(),

@@ -53,3 +53,24 @@ def test_a_plan_that_was_only_captured_is_built_before_an_eager_run(device, extr
     device.capturing = True
     w.run(q, pool)  # built: a graph may point to it
     assert device.calls[6:] == ["run"]
+
+
+@pytest.mark.parametrize("extra", [dict(), dict(window_left=60, first_tokens=3)])
+def test_work_list_and_run_use_the_workspace_of_the_plan(device, monkeypatch, extra):
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32)  # noqa: E731
+    pool, q = torch.zeros((4, 2, 16, 2, 128), dtype=torch.bfloat16), torch.zeros((20, 8, 128), dtype=torch.bfloat16)
+    named = []
+    monkeypatch.setattr(FakeLib, "piekv_prefill_plan_opt", lambda self, *args: named.append(args[-4]) or 0)
+    monkeypatch.setattr(FakeLib, "piekv_prefill_run_opt", lambda self, *args: named.append(args[-5]) or 0)
+    first, second = (torch.empty(32 << 20, dtype=torch.uint8) for _ in range(2))
+    w = ops.BatchPrefillWithPagedKVCacheWrapper(first)
+    tables = (i32(0, 20), i32(0, 2), i32(0, 1), i32(4), 8, 2, 128, 16)
+    w.plan(*tables, causal=True, q_data_type=torch.bfloat16, **extra)
+    w.run(q, pool)
+    w.workspace_buffer = second
+    w.run(q, pool)
+    w.run(q, torch.cat([pool, pool]))
+    assert set(named) == {first.data_ptr()} and len(named) == 5
+    w.plan(*tables, causal=True, q_data_type=torch.bfloat16, **extra)
+    w.run(q, pool)
+    assert set(named[5:]) == {second.data_ptr()} and len(named) == 7

@@ -204,3 +204,25 @@ def test_the_grouping_that_plan_makes_lives_in_the_plan_buffer(device):
         assert a.plan + a.plan_bytes <= a.group_indptr <= buffer.data_ptr() + buffer.numel() - 8
         assert w._plan["keep"][3].tolist() == [0, batch] and w._plan["keep"][3].data_ptr() == a.group_indptr
         assert a.plan == buffer.data_ptr() and a.num_groups == 1
+
+
+@pytest.mark.parametrize("kind", ["prefix", "decode", "prefill"])
+def test_a_plan_holds_the_workspace_that_it_names(device, monkeypatch, kind):
+    monkeypatch.setattr(ops, "_err_ptr", lambda index: 0)
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32)  # noqa: E731
+    ws = torch.empty(32 << 20, dtype=torch.uint8)
+    tables = (i32(0, 2), i32(0, 1), i32(4), HQ, HKV, D, PAGE)
+    extra = dict(window_left=60, first_tokens=3, q_data_type=torch.bfloat16)
+    if kind == "prefix":
+        w = ops.BatchSharedPrefixDecodeWrapper(ws)
+        w.plan(*tables, q_data_type=torch.bfloat16)
+    elif kind == "decode":
+        w = ops.BatchDecodeWithPagedKVCacheWrapper(ws)
+        w.plan(*tables, **extra)
+    else:
+        w = ops.BatchPrefillWithPagedKVCacheWrapper(ws)
+        w.plan(i32(0, 1), *tables, **extra)
+    held = weakref.ref(ws)
+    w.workspace_buffer = torch.empty(32 << 20, dtype=torch.uint8)  # for the next plan()
+    del ws
+    assert held() is not None
